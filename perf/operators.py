@@ -234,7 +234,7 @@ def prepare(case, seed):
         cache = pikv_b200.PagedKVCache(B, width * PAGE, H, bits=bits, symmetric=bits == 8, device=dev, identity_table=False, num_pages=pages)
         for n, t in cache.named_buffers():
             if n in s:                                                 # one copy of the cache: its buffers are the state's
-                setattr(cache, n, s[n])
+                setattr(cache, n, s[n].clone() if n == "length" else s[n])     # accept_tree writes the cache's own length
         s["cache"] = cache
         if kind in ("bounds", "sparse"):
             s["bounds"] = pikv_b200.PageBounds(s["bound_codes"], s["bound_scale"])
