@@ -539,6 +539,84 @@ size_t pikv_decode_attn_static_scratch_bytes(void);
 int    pikv_decode_attn_q8_static(const pikv_decode_params* p, pikv_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Speculative decoding and sparse decode attention over the paged cache.  They have no counterpart in the
+ * reference (its attention, core/single/pikv_attention.py:104-193, is dense and takes one token a step).
+ *
+ * The cache: pools and page table as above.  bits 8 is the symmetric int8 cache, bits 4 the asymmetric one
+ * (k_zp / v_zp required).  Page numbers outside the table or the pool raise PIKV_ST_BAD_PAGE, stream ids
+ * outside 0 .. num_seqs - 1 PIKV_ST_BAD_SEQ; such a stream has length 0 and a zero result.
+ * Streams of one call go to the GPU in chunks of PIKV_STREAMS_PER_LAUNCH, any number may be given.
+ * ---------------------------------------------------------------------- */
+#define PIKV_STREAMS_PER_LAUNCH 512
+#define PIKV_TREE_NODES 64            /* drafted tokens per stream, at most */
+
+typedef struct {
+    const int32_t* page_table; int32_t num_seqs, max_pages, num_pages, n_kv, bits, symmetric;
+    void* k_codes; void* v_codes; void* k_scale; void* v_scale; void* k_zp; void* v_zp;
+    uint32_t* status;
+} pikv_paged_cache;
+
+/* Attention of N drafted tokens per stream.  Node i of stream b is the row at position ctx_len[b] + i (the
+ * caller has appended it); its query sees positions 0 .. ctx_len[b] - 1 and the nodes j with mask[b][i][j] != 0:
+ *   out[b,i,h,:] = softmax over those rows of (q[b,i,h,:] . K / sqrt(128)) times V
+ *   q, out: [B, N, n_q, 128] bf16, N <= PIKV_TREE_NODES, n_q / n_kv <= 64
+ *   mask: bytes [N, N], or [B, N, N] with mask_per_stream != 0
+ *   nodes (optional) [B]: nodes of each stream, 0 .. N; those behind are neither seen nor computed, their rows
+ *   of out are zero and their lse -infinity, as for a node that sees nothing
+ *   lse (optional) [B, N, n_q] fp32 log-sum-exp of the scaled scores */
+typedef struct {
+    const void* q; void* out; float* lse;
+    int32_t B, N, n_q;
+    const int32_t* seq_ids; const int32_t* ctx_len; const int32_t* nodes;
+    const uint8_t* mask; int32_t mask_per_stream;
+    void* workspace; size_t workspace_bytes;      /* 16-byte aligned */
+} pikv_tree_params;
+size_t pikv_tree_attn_workspace_bytes(int32_t B, int32_t N, int32_t n_q, int32_t n_kv);
+int    pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params* p, pikv_stream_t stream);
+
+/* One path of every stream's tree becomes context: the rows at ctx_len[b] + path[b][i], i < path_len[b], move to
+ * ctx_len[b] + i (K and V, codes, scales and zero points, all heads), and new_len[b] = ctx_len[b] + path_len[b],
+ * also written to length[seq] if length is given.  path [B, depth], strictly ascending; path_len (optional) [B].
+ * A stream whose path is not ascending, leaves the cache or meets a bad page is left as it is (its new length is
+ * ctx_len[b]) and raises PIKV_ST_BAD_INDEX or PIKV_ST_BAD_PAGE; one that an earlier entry of seq_ids names already
+ * raises PIKV_ST_BAD_SEQ and has new_len 0.  Any cache format.  ctx_len may be the length array itself when
+ * seq_ids is NULL. */
+int pikv_tree_accept(const pikv_paged_cache* c, const int32_t* path, const int32_t* path_len, const int32_t* seq_ids,
+                     const int32_t* ctx_len, int32_t B, int32_t depth, int32_t* length, int32_t* new_len, pikv_stream_t stream);
+
+/* Bounds of the keys of every page, for pikv_sparse_attn: over the rows of a page inside its stream, the largest and
+ * the smallest key of each channel as whole steps of a power of two, rounded outwards:
+ *   bound_scale[page][h] = the smallest power of two s >= 2^-126 with |K| <= 127 s on the page
+ *   bound_codes[page][h][0][c] = ceil(max K_c / s),  [1][c] = floor(min K_c / s)      int8
+ * A page that holds something not finite has scale +infinity and codes 0.  The pages that hold positions
+ * start[b] .. seq_len[b] - 1 (start NULL: all) are computed anew.  Decodable formats (see bits). */
+int pikv_page_bounds_update(const pikv_paged_cache* c, void* bound_codes, float* bound_scale, const int32_t* seq_ids,
+                            const int32_t* start, const int32_t* seq_len, int32_t B, pikv_stream_t stream);
+
+/* Decode attention over at most `pages` pages of each (stream, KV head): the first `first`, the last `recent` (>= 1),
+ * and the best of those between them, ties going to the lower page.  A page's score is the largest logit that a query
+ * head of the group can reach inside the page's bounds, times sqrt(128):
+ *   score = max over the group's heads of  s_q s_page sum_c (max(u_c, 0) hi_c + min(u_c, 0) lo_c)
+ * with the query in whole steps too, u = rint(q / s_q), s_q as s above; the sum is a whole number and the products by
+ * powers of two are exact, so the choice does not depend on an order of summation.  A query head that is not finite
+ * has no say, a page with an infinite scale is taken before the finite ones.
+ *   q, out [B, n_q, 128] bf16, n_q / n_kv <= 8; lse as in pikv_decode_params
+ *   chosen (optional) [B, n_kv, pages] int32: the page numbers taken, ascending, -1 behind them
+ *   max_pages <= PIKV_SPARSE_MAX_PAGES */
+#define PIKV_SPARSE_MAX_PAGES 49152
+typedef struct {
+    const void* q; void* out; float* lse;
+    int32_t B, n_q;
+    const int32_t* seq_ids; const int32_t* seq_len;
+    const void* bound_codes; const float* bound_scale;
+    int32_t pages, first, recent;
+    int32_t* chosen;
+    void* workspace; size_t workspace_bytes;      /* 16-byte aligned */
+} pikv_sparse_params;
+size_t pikv_sparse_attn_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int32_t max_pages, int32_t pages);
+int    pikv_sparse_attn(const pikv_paged_cache* c, const pikv_sparse_params* p, pikv_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Decode step over the striped expert-sharded cache (pikv_kv_append_striped).  Stream s lives on its home
  * rank s / streams_per_rank, which holds its query, its top-k experts and weights and the lengths of its
  * pairs.  One step, the same three calls in the same order on every rank (all on one stream per rank):

@@ -141,6 +141,29 @@ class DecodeParams(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("page_table", vp), ("num_seqs", i32), ("max_pages", i32), ("num_pages", i32), ("n_kv", i32), ("bits", i32), ("symmetric", i32),
+        ("k_codes", vp), ("v_codes", vp), ("k_scale", vp), ("v_scale", vp), ("k_zp", vp), ("v_zp", vp), ("status", vp),
+    ]
+
+
+class TreeParams(C.Structure):
+    _fields_ = [
+        ("q", vp), ("out", vp), ("lse", vp), ("B", i32), ("N", i32), ("n_q", i32),
+        ("seq_ids", vp), ("ctx_len", vp), ("nodes", vp), ("mask", vp), ("mask_per_stream", i32),
+        ("workspace", vp), ("workspace_bytes", sz),
+    ]
+
+
+class SparseParams(C.Structure):
+    _fields_ = [
+        ("q", vp), ("out", vp), ("lse", vp), ("B", i32), ("n_q", i32), ("seq_ids", vp), ("seq_len", vp),
+        ("bound_codes", vp), ("bound_scale", vp), ("pages", i32), ("first", i32), ("recent", i32), ("chosen", vp),
+        ("workspace", vp), ("workspace_bytes", sz),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/pikv_b200.h declares
 SIGNATURES = {
     "pikv_abi_version": (i32, []),
@@ -184,6 +207,12 @@ SIGNATURES = {
     "pikv_decode_attn_q4": (i32, [C.POINTER(DecodeParams), vp]),
     "pikv_decode_attn_static_scratch_bytes": (sz, []),
     "pikv_decode_attn_q8_static": (i32, [C.POINTER(DecodeParams), vp]),
+    "pikv_tree_attn_workspace_bytes": (sz, [i32, i32, i32, i32]),
+    "pikv_tree_attn": (i32, [C.POINTER(PagedCache), C.POINTER(TreeParams), vp]),
+    "pikv_tree_accept": (i32, [C.POINTER(PagedCache), vp, vp, vp, vp, i32, i32, vp, vp, vp]),
+    "pikv_page_bounds_update": (i32, [C.POINTER(PagedCache), vp, vp, vp, vp, vp, i32, vp]),
+    "pikv_sparse_attn_workspace_bytes": (sz, [i32, i32, i32, i32, i32]),
+    "pikv_sparse_attn": (i32, [C.POINTER(PagedCache), C.POINTER(SparseParams), vp]),
     "pikv_h2o_accumulate_probs": (i32, [vp, i32, vp, i32, vp, vp, i32, i32, i32, vp, i32, vp]),
     "pikv_h2o_accumulate_attn": (i32, [vp, i32, vp, vp, i32, i32, i32, vp, i32, vp]),
     "pikv_lowrank_project": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp]),

@@ -66,6 +66,7 @@ struct DecodeDev {
     float* part_o;    // [(max_blocks + B) * n_kv][G][128]
     float* part_ml;   // [(max_blocks + B) * n_kv][G][2]  (running max in the log2 domain, denominator)
     int workers, max_blocks;
+    int nan_out;      // page lists: a result that is not a number comes out as one (the dense calls answer 0)
     unsigned* status;
 };
 
@@ -300,7 +301,10 @@ __global__ void __launch_bounds__(DA_PLAN_THREADS) decode_plan_kernel(DecodeDev 
 // into at most one block per worker of a head, down to DA_DIRECT_BLOCK pages, and worker w takes item w; CTA 0 leaves what
 // the merge kernel needs.  One stream of 1500 tokens: 48 items of 16 pages behind a 4 us plan kernel took 24 us a step; 192
 // items of 4 pages take 10.  24 streams of 3300 tokens, 4 bit: 69 -> 41 us.
-template <int BITS, bool GS, bool DIRECT>
+//
+// LIST: every (request, KV head) has a page list of its own (sparse attention), all heads of a request one of the same
+// length; only the look-up of a page differs.
+template <int BITS, bool GS, bool DIRECT, bool LIST>
 __global__ void __launch_bounds__(DA_THREADS, da_ctas_per_sm(BITS)) decode_attn_kernel(DecodeDev d) {
     using GEO = DAGeom<BITS>;
     constexpr int STAGES = GEO::STAGES, STAGE_BYTES = GEO::STAGE, PAGE_BYTES = GEO::PAGE, ROW = GEO::ROW;
@@ -432,11 +436,12 @@ __global__ void __launch_bounds__(DA_THREADS, da_ctas_per_sm(BITS)) decode_attn_
     // page ids of the issuing cursor, 32 at a time (lane l holds page pt_base + l of row pt_row): one at a time, every page
     // held up its warp for a trip to L2
     int pt_ids = -1, pt_row = -2, pt_base = 0;
-    auto page_id = [&](const DACursor& x) {
-        if (x.row != pt_row || x.p < pt_base || x.p >= pt_base + 32) {
-            pt_row = x.row;
+    auto page_id = [&](const DACursor& x, int h) {
+        const int row = LIST && x.row >= 0 ? x.row * n_kv + h : x.row;
+        if (row != pt_row || x.p < pt_base || x.p >= pt_base + 32) {
+            pt_row = row;
             pt_base = x.p;
-            pt_ids = x.row >= 0 && x.p + lane < d.max_pages ? __ldg(d.page_table + (size_t)x.row * d.max_pages + x.p + lane) : -1;
+            pt_ids = row >= 0 && x.p + lane < d.max_pages ? __ldg(d.page_table + (size_t)row * d.max_pages + x.p + lane) : -1;
         }
         return __shfl_sync(0xffffffffu, pt_ids, x.p - pt_base);
     };
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__(DA_THREADS, da_ctas_per_sm(BITS)) decode_attn_
                 pend_id = next_id;
                 next_id = claim();
             }
-            const int page = page_id(is.cur);
+            const int page = page_id(is.cur, is.h);
             if (lane == 0) issue(page, is.h, issued);
             advance(is.cur, 1);
             --is.left;
@@ -516,6 +521,13 @@ __global__ void __launch_bounds__(DA_THREADS, da_ctas_per_sm(BITS)) decode_attn_
         for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(qv[i]));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        float odd = 0.f;                              // NaN for a query head that is not finite: so are its scores then
+        if constexpr (LIST) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) odd = fmaf(qv[i], 0.f, odd);
+            odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+            odd += __shfl_xor_sync(0xffffffffu, odd, 2);
+        }
         if constexpr (GS) {
             const int e = amax > 0.f ? ilogbf(amax) + 1 : 0;          // amax < 2^e
             const float up = ldexpf(1.0f, 13 - e);
@@ -539,7 +551,7 @@ __global__ void __launch_bounds__(DA_THREADS, da_ctas_per_sm(BITS)) decode_attn_
                     qf[2 * m + 1] = pack4_s8(u[8 * m + 1], u[8 * m + 3], u[8 * m + 5], u[8 * m + 7]);
                 }
             }
-            const float qmul = ldexpf(1.0f, e - 13) * 0.08838834764831845f * 1.4426950408889634f;
+            const float qmul = ldexpf(1.0f, e - 13) * 0.08838834764831845f * 1.4426950408889634f + odd;
             qm0 = __shfl_sync(0xffffffffu, qmul, 8 * j);              // lane (column 2j = head j, channels 0..31)
             if (BITS == 4) {
                 usum += __shfl_xor_sync(0xffffffffu, usum, 1);
@@ -559,7 +571,7 @@ __global__ void __launch_bounds__(DA_THREADS, da_ctas_per_sm(BITS)) decode_attn_
             const int c2 = BITS == 8 ? cc + 1 : cc + 4;
             qf[i] = pack_h2(qv[cc] * down, qv[c2] * down);
         }
-        const float qmul = ldexpf(1.0f, e) * 0.08838834764831845f * 1.4426950408889634f;
+        const float qmul = ldexpf(1.0f, e) * 0.08838834764831845f * 1.4426950408889634f + odd;
         qm0 = __shfl_sync(0xffffffffu, qmul, 8 * j);          // lane of (head 2j, j = 0)
         qm1 = __shfl_sync(0xffffffffu, qmul, 8 * j + 4);
         if (BITS == 4) {
@@ -803,7 +815,11 @@ __global__ void __launch_bounds__(DA_THREADS, da_ctas_per_sm(BITS)) decode_attn_
             // P' = P * vscale, rounded to f16 as the tensor cores will see it; pbuf is [head][32 positions]
             auto page_probs = [&](const unsigned char* st, const float (&t)[4], float vw_lo, float vw_hi, int base, int pos0) {
                 const uint16_t* vsc = reinterpret_cast<const uint16_t*>(st + 2 * PAGE_BYTES + 32);
-                const float vs_lo = __uint_as_float((uint32_t)vsc[r] << 16), vs_hi = __uint_as_float((uint32_t)vsc[r + 8] << 16);
+                float vs_lo = __uint_as_float((uint32_t)vsc[r] << 16), vs_hi = __uint_as_float((uint32_t)vsc[r + 8] << 16);
+                if (pos0 + PIKV_PAGE_TOKENS > c.cur.len) {             // what lies behind the end need not be finite
+                    if (pos0 + r >= c.cur.len) vs_lo = vw_lo = 0.f;
+                    if (pos0 + r + 8 >= c.cur.len) vs_hi = vw_hi = 0.f;
+                }
                 if constexpr (GS) {
                     const float p0 = exp2f(t[0] - mu0), p2 = exp2f(t[2] - mu0);
                     if (d.probs16) {
@@ -1047,10 +1063,11 @@ __global__ void __launch_bounds__(DA_MERGE_THREADS) decode_merge_kernel(DecodeDe
     } else {
         da_merge_blocks(d, rq, h, qh, g0, g1, lane, M, acc, l);
     }
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(l > 0.f ? acc.x / l : 0.f, l > 0.f ? acc.y / l : 0.f);
-    const __nv_bfloat162 hi = __floats2bfloat162_rn(l > 0.f ? acc.z / l : 0.f, l > 0.f ? acc.w / l : 0.f);
+    const bool any = l > 0.f || (d.nan_out && l != 0.f);
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(any ? acc.x / l : 0.f, any ? acc.y / l : 0.f);
+    const __nv_bfloat162 hi = __floats2bfloat162_rn(any ? acc.z / l : 0.f, any ? acc.w / l : 0.f);
     *out2 = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    if (lane == 0 && d.lse) d.lse[bq] = (l > 0.f) ? M * 0.6931471805599453f + logf(l) : -INFINITY;
+    if (lane == 0 && d.lse) d.lse[bq] = any ? M * 0.6931471805599453f + logf(l) : -INFINITY;
 }
 
 // The same merge on an expert-sharded box: request i = (stream i / top_k, choice i % top_k) of a decode step
@@ -1165,7 +1182,7 @@ extern "C" size_t pikv_decode_attn_workspace_bytes(int32_t B, int32_t n_q, int32
 }
 
 int pikv::decode_attn_run(const pikv_decode_params* p, cudaStream_t st, int bits, const int* q_rows, const ShardReturn* ret,
-                          const ShardPlan* plan) {
+                          const ShardPlan* plan, bool lists) {
     PIKV_REQUIRE(p != nullptr, PIKV_EINVAL, "decode_attn: null params");
     PIKV_REQUIRE(p->q && (p->out || ret) && p->seq_len && p->page_table, PIKV_EINVAL, "decode_attn: null pointer");
     PIKV_REQUIRE(p->k_codes && p->v_codes && p->k_scale && p->v_scale, PIKV_EINVAL, "decode_attn: null cache pointer");
@@ -1197,6 +1214,7 @@ int pikv::decode_attn_run(const pikv_decode_params* p, cudaStream_t st, int bits
     PIKV_REQUIRE(p->workspace != nullptr, PIKV_EINVAL, "decode_attn: null workspace");
     PIKV_REQUIRE((reinterpret_cast<uintptr_t>(p->workspace) & 15) == 0, PIKV_EINVAL, "decode_attn: workspace must be 16-byte aligned");
     d.workers = da_workers(bits);
+    d.nan_out = lists;
     d.max_blocks = da_blocks_for(p->workspace_bytes, p->B, p->n_q, p->n_kv);
     PIKV_REQUIRE(d.max_blocks >= 1, PIKV_EINVAL, "decode_attn: workspace too small (%zu bytes at least, %zu for full speed)",
                  da_layout(p->B, p->n_q, p->n_kv, 1).total, da_layout(p->B, p->n_q, p->n_kv, da_default_blocks(p->n_kv)).total);
@@ -1221,17 +1239,19 @@ int pikv::decode_attn_run(const pikv_decode_params* p, cudaStream_t st, int bits
     }
     const int grid = d.workers / DA_WARPS;
     const bool gs = d.G <= 4;      // integer first product (see decode_attn_kernel)
-#define PIKV_DA_LAUNCH(BITS, GS, DIRECT)                                                                                  \
+#define PIKV_DA_LAUNCH(BITS, GS, DIRECT, LIST)                                                                            \
     do {                                                                                                                  \
         const size_t smem = da_smem_bytes<BITS>() + (DIRECT ? (size_t)(p->B + 1) * sizeof(int) : 0);                      \
-        if (!allow_smem<decode_attn_kernel<BITS, GS, DIRECT>>((int)da_smem_bytes<BITS>() + (DA_DIRECT_REQ + 1) * 4))      \
+        if (!allow_smem<decode_attn_kernel<BITS, GS, DIRECT, LIST>>((int)da_smem_bytes<BITS>() + (DA_DIRECT_REQ + 1) * 4)) \
             return check_launch("decode_attn smem attribute");                                                            \
-        launch_dependent(decode_attn_kernel<BITS, GS, DIRECT>, grid, DA_THREADS, smem, st, d);                            \
+        launch_dependent(decode_attn_kernel<BITS, GS, DIRECT, LIST>, grid, DA_THREADS, smem, st, d);                      \
     } while (0)
 #define PIKV_DA_LAUNCH2(BITS, GS)                                                                                         \
     do {                                                                                                                  \
-        if (direct) PIKV_DA_LAUNCH(BITS, GS, true);                                                                       \
-        else PIKV_DA_LAUNCH(BITS, GS, false);                                                                             \
+        if (lists && direct) PIKV_DA_LAUNCH(BITS, GS, true, true);                                                        \
+        else if (lists) PIKV_DA_LAUNCH(BITS, GS, false, true);                                                            \
+        else if (direct) PIKV_DA_LAUNCH(BITS, GS, true, false);                                                           \
+        else PIKV_DA_LAUNCH(BITS, GS, false, false);                                                                      \
     } while (0)
     if (bits == 8 && gs) PIKV_DA_LAUNCH2(8, true);
     else if (bits == 8) PIKV_DA_LAUNCH2(8, false);

@@ -14,6 +14,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/cuda/CUDAStream.h>
@@ -166,6 +167,20 @@ struct Cache {
         if (!PyDict_Check(buffers)) fail("a cache is passed as its buffer dict");
     }
     void* at(PyObject* key) const { return ptr(buffer(buffers, key)); }
+    // the cache as one block, for calls whose tensors lie on the device of `like`
+    pikv_paged_cache view(const at::Tensor& like) const {
+        const at::Tensor& table = buffer(buffers, s_page_table);
+        if (!table.defined() || table.scalar_type() != at::kInt) fail("the cache's page_table must be int32");
+        if (table.device() != like.device()) fail("the cache is on %s, the call's tensors are on %s", table.device().str().c_str(), like.device().str().c_str());
+        holds(table, (int64_t)num_seqs * max_pages, "the cache's page_table");
+        pikv_paged_cache c = {};
+        c.page_table = ptr<int32_t>(table);
+        c.num_seqs = num_seqs; c.max_pages = max_pages; c.num_pages = num_pages; c.n_kv = n_kv; c.bits = bits; c.symmetric = symmetric;
+        c.k_codes = at(s_k_codes); c.v_codes = at(s_v_codes); c.k_scale = at(s_k_scale); c.v_scale = at(s_v_scale);
+        c.k_zp = at(s_k_zp); c.v_zp = at(s_v_zp);
+        c.status = static_cast<uint32_t*>(at(s_status));
+        return c;
+    }
     void fill(pikv_append_params& p) const {
         p.page_table = static_cast<const int32_t*>(at(s_page_table));
         p.num_seqs = num_seqs; p.max_pages = max_pages; p.num_pages = num_pages;
@@ -482,6 +497,167 @@ PyObject* decode(PyObject* const* a, Py_ssize_t n) {
         return wrap(out);
     }
     return want_lse ? tuple(out, lse) : wrap(out);
+}
+
+// ---- speculative and sparse decoding -------------------------------------------------------------------------
+void together(const at::Tensor& like, std::initializer_list<at::Tensor> rest) {
+    for (const at::Tensor& t : rest)
+        if (t.defined() && t.device() != like.device()) fail("the call's tensors lie on different devices");
+}
+// the kernels read rows in 16-byte pieces
+at::Tensor rows16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone() : t; }
+
+// Lengths of the streams of a call: seq_ids, and one int32 each or the cache's own (None).  Checked when it is made, before
+// anything touches a device.
+struct Streams {
+    const Cache& c;
+    at::Tensor ids;
+    PyObject* given;
+    at::Tensor len;
+    Streams(const Cache& cache, const at::Tensor& like, const at::Tensor& seq_ids, PyObject* lens, int64_t B, const char* name) : c(cache), ids(seq_ids), given(lens) {
+        if (!ids.defined() && B > c.num_seqs) fail("%lld streams, the cache has %d", (long long)B, c.num_seqs);
+        holds(ids, B, "seq_ids");
+        if (given != Py_None) {
+            len = holds(req(given, name, at::kInt), B, name);
+        } else {
+            len = buffer(c.buffers, s_length);
+            if (!len.defined() || len.scalar_type() != at::kInt) fail("the cache's length must be one int32 per sequence");
+            holds(len, c.num_seqs, "the cache's length");
+        }
+        together(like, {ids, len});
+    }
+    const at::Tensor& get() {             // with the device of the call current
+        if (given == Py_None && ids.defined()) len = lengths(c, ids, given);
+        return len;
+    }
+};
+
+// tree(cache..., q, mask, seq_ids, ctx_len, nodes, want_lse)
+PyObject* tree(PyObject* const* a, Py_ssize_t) {
+    const Cache c(a);
+    a += Cache::ARGS;
+    const at::Tensor q0 = req(a[0], "q", at::kBFloat16);
+    if (q0.dim() != 4 || q0.size(3) != PIKV_HEAD_DIM) fail("q must be [B, N, n_q, %d]", PIKV_HEAD_DIM);
+    const int64_t B = q0.size(0), N = q0.size(1), n_q = q0.size(2);
+    const at::Tensor mask = req(a[1], "mask", at::kBool);
+    const bool each = mask.dim() == 3;
+    if (!(each || mask.dim() == 2) || mask.size(-1) != N || mask.size(-2) != N || (each && mask.size(0) != B)) fail("mask must be [N, N] or [B, N, N] with q's B and N");
+    const at::Tensor ids = opt(a[2], "seq_ids", at::kInt), nodes = opt(a[4], "nodes", at::kInt);
+    together(q0, {mask, nodes});
+    holds(nodes, B, "nodes");
+    Streams streams(c, q0, ids, a[3], B, "ctx_len");
+    const c10::cuda::OptionalCUDAGuard guard(q0.device());
+    const pikv_paged_cache cache = c.view(q0);
+    const at::Tensor ctx = streams.get();
+    const bool want_lse = truth(a[5]);
+    at::Tensor out = at::empty(q0.sizes(), q0.options()), lse;
+    if (want_lse) lse = at::empty({B, N, n_q}, on(q0, at::kFloat));
+    if (q0.numel()) {
+        const at::Tensor q = rows16(q0);
+        const size_t bytes = pikv_tree_attn_workspace_bytes((int32_t)B, (int32_t)N, (int32_t)n_q, c.n_kv);
+        const at::Tensor ws = workspace(q, bytes);
+        pikv_tree_params p = {};
+        p.q = ptr(q); p.out = ptr(out); p.lse = ptr<float>(lse);
+        p.B = (int32_t)B; p.N = (int32_t)N; p.n_q = (int32_t)n_q;
+        p.seq_ids = ptr<int32_t>(ids); p.ctx_len = ptr<int32_t>(ctx); p.nodes = ptr<int32_t>(nodes);
+        p.mask = ptr<uint8_t>(mask); p.mask_per_stream = each;
+        p.workspace = ptr(ws); p.workspace_bytes = bytes;
+        check(pikv_tree_attn(&cache, &p, stream()), "pikv_tree_attn");
+    }
+    return want_lse ? tuple(out, lse) : wrap(out);
+}
+
+// accept(cache..., path, path_len, seq_ids, ctx_len) -> new lengths, the cache's own among them
+PyObject* accept(PyObject* const* a, Py_ssize_t) {
+    const Cache c(a);
+    a += Cache::ARGS;
+    const at::Tensor path = req(a[0], "path", at::kInt);
+    if (path.dim() != 2) fail("path must be [B, depth]");
+    const int64_t B = path.size(0), depth = path.size(1);
+    const at::Tensor count = opt(a[1], "path_len", at::kInt), ids = opt(a[2], "seq_ids", at::kInt);
+    together(path, {count});
+    holds(count, B, "path_len");
+    Streams streams(c, path, ids, a[3], B, "ctx_len");
+    const at::Tensor& length = buffer(c.buffers, s_length);
+    if (!length.defined() || length.scalar_type() != at::kInt) fail("the cache's length must be one int32 per sequence");
+    holds(length, c.num_seqs, "the cache's length");
+    const c10::cuda::OptionalCUDAGuard guard(path.device());
+    const pikv_paged_cache cache = c.view(path);
+    const at::Tensor ctx = streams.get();
+    if (ids.defined() && ptr(ctx) == ptr(length)) fail("ctx_len must have an entry per stream of the call, not per sequence of the cache");
+    at::Tensor fresh = at::empty({B}, on(path, at::kInt));
+    if (B)
+        check(pikv_tree_accept(&cache, ptr<int32_t>(path), ptr<int32_t>(count), ptr<int32_t>(ids), ptr<int32_t>(ctx), (int32_t)B, (int32_t)depth,
+                               ptr<int32_t>(length), ptr<int32_t>(fresh), stream()), "pikv_tree_accept");
+    return wrap(fresh);
+}
+
+// a cache's bounds, as pikv_page_bounds_update writes them
+struct Bounds {
+    at::Tensor codes, scale;
+    Bounds(PyObject* o_codes, PyObject* o_scale, const Cache& c) : codes(written(o_codes, "bounds.codes", at::kChar)), scale(written(o_scale, "bounds.scale", at::kFloat)) {
+        if (!codes.defined() || !scale.defined()) fail("bounds must hold CUDA tensors");
+        holds(codes, (int64_t)c.num_pages * c.n_kv * 2 * PIKV_HEAD_DIM, "bounds.codes");
+        holds(scale, (int64_t)c.num_pages * c.n_kv, "bounds.scale");
+    }
+};
+
+// bounds(cache..., codes, scale, seq_ids, start, seq_len); without ids: as many streams as seq_len has, or all
+PyObject* bounds(PyObject* const* a, Py_ssize_t) {
+    const Cache c(a);
+    a += Cache::ARGS;
+    const Bounds to(a[0], a[1], c);
+    const at::Tensor ids = opt(a[2], "seq_ids", at::kInt), start = opt(a[3], "start", at::kInt);
+    together(to.codes, {to.scale, start});
+    const int64_t B = ids.defined() ? ids.numel() : a[4] != Py_None ? req(a[4], "seq_len", at::kInt).numel() : c.num_seqs;
+    holds(start, B, "start");
+    Streams streams(c, to.codes, ids, a[4], B, "seq_len");
+    const c10::cuda::OptionalCUDAGuard guard(to.codes.device());
+    const pikv_paged_cache cache = c.view(to.codes);
+    const at::Tensor len = streams.get();
+    if (B)
+        check(pikv_page_bounds_update(&cache, ptr(to.codes), ptr<float>(to.scale), ptr<int32_t>(ids), ptr<int32_t>(start), ptr<int32_t>(len), (int32_t)B, stream()),
+              "pikv_page_bounds_update");
+    Py_RETURN_NONE;
+}
+
+// sparse(cache..., q, codes, scale, pages, seq_ids, seq_len, first, recent, want_lse, want_pages)
+PyObject* sparse(PyObject* const* a, Py_ssize_t) {
+    const Cache c(a);
+    a += Cache::ARGS;
+    const at::Tensor q0 = req(a[0], "q", at::kBFloat16);
+    if (q0.dim() != 3 || q0.size(2) != PIKV_HEAD_DIM) fail("q must be [B, n_q, %d]", PIKV_HEAD_DIM);
+    const Bounds by(a[1], a[2], c);
+    const int64_t B = q0.size(0), n_q = q0.size(1), pages = num(a[3]);
+    if (pages < 1 || pages > PIKV_SPARSE_MAX_PAGES) fail("pages must be 1 to %d", PIKV_SPARSE_MAX_PAGES);
+    const at::Tensor ids = opt(a[4], "seq_ids", at::kInt);
+    together(q0, {by.codes, by.scale});
+    Streams streams(c, q0, ids, a[5], B, "seq_len");
+    const bool want_lse = truth(a[8]), want_pages = truth(a[9]);
+    pikv_sparse_params p = {};
+    const long first = num(a[6]), recent = num(a[7]);
+    if (first < 0 || recent < 1 || first + recent > pages) fail("first %ld + recent %ld (at least 1) must fit in %lld pages", first, recent, (long long)pages);
+    p.first = (int32_t)first; p.recent = (int32_t)recent;
+    const c10::cuda::OptionalCUDAGuard guard(q0.device());
+    const pikv_paged_cache cache = c.view(q0);
+    const at::Tensor len = streams.get();
+    at::Tensor out = at::empty(q0.sizes(), q0.options()), lse, chosen;
+    if (want_lse) lse = at::empty({B, n_q}, on(q0, at::kFloat));
+    if (want_pages) chosen = at::empty({B, c.n_kv, pages}, on(q0, at::kInt));
+    if (q0.numel()) {
+        const at::Tensor q = rows16(q0);
+        const size_t bytes = pikv_sparse_attn_workspace_bytes((int32_t)B, (int32_t)n_q, c.n_kv, c.max_pages, (int32_t)pages);
+        const at::Tensor ws = workspace(q, bytes);
+        p.q = ptr(q); p.out = ptr(out); p.lse = ptr<float>(lse);
+        p.B = (int32_t)B; p.n_q = (int32_t)n_q; p.pages = (int32_t)pages;
+        p.seq_ids = ptr<int32_t>(ids); p.seq_len = ptr<int32_t>(len);
+        p.bound_codes = ptr(by.codes); p.bound_scale = ptr<float>(by.scale);
+        p.chosen = ptr<int32_t>(chosen);
+        p.workspace = ptr(ws); p.workspace_bytes = bytes;
+        check(pikv_sparse_attn(&cache, &p, stream()), "pikv_sparse_attn");
+    }
+    if (!want_lse && !want_pages) return wrap(out);
+    return want_lse && want_pages ? tuple(out, lse, chosen) : want_lse ? tuple(out, lse) : tuple(out, chosen);
 }
 
 // ---- eviction ----------------------------------------------------------------------------------------------
@@ -930,6 +1106,10 @@ PyMethodDef methods[] = {
     method<dispatch_loss, 10>("dispatch_loss"),
     method<route_append, C + 5 + G + 1>("route_append"),
     method<decode, C + 5, C + 6>("decode"),
+    method<tree, C + 6>("tree"),
+    method<accept, C + 4>("accept"),
+    method<bounds, C + 5>("bounds"),
+    method<sparse, C + 10>("sparse"),
     method<select, 8>("select"),
     method<compact, 2 * C + 7>("compact"),
     method<quant_pair, 9>("quant_pair"),

@@ -30,8 +30,10 @@ struct ShardPlan {
     int* q_rows;
 };
 
+// lists: the page table holds a list of physical pages per (request, KV head), [B][n_kv][max_pages], in place of one row per
+// sequence
 int decode_attn_run(const pikv_decode_params* p, cudaStream_t st, int bits, const int* q_rows, const ShardReturn* ret,
-                    const ShardPlan* plan);
+                    const ShardPlan* plan, bool lists = false);
 
 constexpr unsigned SD_FAILED = 0x80000000u;      // top bit of a rank's step number: a wait of that rank ran out
 

@@ -16,6 +16,7 @@ _quantize_tensor (core/single/module/pikv_compression.py:945-1012) per
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -23,6 +24,14 @@ import torch
 from . import _lib, ops
 from ._lib import PikvError, check, host, lib
 from .ops import _p, _req, _stream, PAGE_TOKENS, HEAD_DIM
+
+
+@dataclass
+class PageBounds:
+    """Bounds of the keys of every page and head: codes int8 [num_pages, n_kv, 2, 128] (largest, smallest key of each
+    channel) in whole steps of scale fp32 [num_pages, n_kv], a power of two.  See PagedKVCache.update_bounds."""
+    codes: torch.Tensor
+    scale: torch.Tensor
 
 
 class PagedKVCache(torch.nn.Module):
@@ -156,6 +165,55 @@ class PagedKVCache(torch.nn.Module):
         probs, step_max = self.h2o_workspace(q.shape[0], q.shape[1]) if workspace is None else workspace
         return host().decode(self._buffers, self.num_seqs, self.n_kv, self.bits, self.symmetric, self.max_pages, self.num_pages,
                              q, seq_ids, seq_len, acc, probs, step_max)
+
+    # -- speculative decoding --------------------------------------------------------
+    def decode_attention_tree(self, q: torch.Tensor, mask: torch.Tensor, seq_ids: Optional[torch.Tensor] = None,
+                              ctx_len: Optional[torch.Tensor] = None, nodes: Optional[torch.Tensor] = None, want_lse: bool = False):
+        """Attention of the N drafted tokens of every stream; q [B, N, n_q, 128] bf16, N up to 64.  The drafted rows have been
+        appended behind the context: node i of stream b is position ctx_len[b] + i (ctx_len int32 [B], default: `length`, which
+        append() leaves alone).  Node i sees the whole context and the nodes j with mask[i, j] (bool [N, N], or [B, N, N] for a
+        tree per stream), its own diagonal entry included in that.  nodes int32 [B]: the nodes of each stream, those behind them are
+        neither seen nor computed (zero rows, log-sum-exp -inf, as for a node that sees nothing).  Returns out [B, N, n_q, 128],
+        with want_lse (out, lse [B, N, n_q]).  int8 symmetric and 4-bit asymmetric caches.  See pikv_tree_attn."""
+        return host().tree(self._buffers, self.num_seqs, self.n_kv, self.bits, self.symmetric, self.max_pages, self.num_pages,
+                           q, mask, seq_ids, ctx_len, nodes, want_lse)
+
+    def accept_tree(self, path: torch.Tensor, path_len: Optional[torch.Tensor] = None, seq_ids: Optional[torch.Tensor] = None,
+                    ctx_len: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The accepted path of every stream's tree becomes context, in place: its nodes' rows move up to positions ctx_len[b],
+        ctx_len[b] + 1, ... and `length` of the stream becomes ctx_len[b] + path_len[b].  path int32 [B, depth]: node numbers,
+        ascending (a node comes after its parent); path_len int32 [B] (default: depth).  Returns the new lengths int32 [B].  A path
+        that is not ascending or leaves the cache moves nothing and shows in check_status(), as does a stream named twice (the
+        later entry is not carried out and returns 0).  Every cache format.  See pikv_tree_accept."""
+        return host().accept(self._buffers, self.num_seqs, self.n_kv, self.bits, self.symmetric, self.max_pages, self.num_pages,
+                             path, path_len, seq_ids, ctx_len)
+
+    # -- sparse attention --------------------------------------------------------------
+    def page_bounds(self) -> PageBounds:
+        """Bounds for this cache's pages, to be filled by update_bounds."""
+        dev = self.k_codes.device
+        return PageBounds(torch.zeros(self.num_pages, self.n_kv, 2, HEAD_DIM, dtype=torch.int8, device=dev),
+                          torch.zeros(self.num_pages, self.n_kv, dtype=torch.float32, device=dev))
+
+    def update_bounds(self, bounds: PageBounds, seq_ids: Optional[torch.Tensor] = None, start: Optional[torch.Tensor] = None,
+                      seq_len: Optional[torch.Tensor] = None) -> None:
+        """In place: the bounds of the pages that hold positions start[b] .. seq_len[b] - 1 (int32 [B]; default: 0 and `length`),
+        computed from the rows below seq_len[b].  After rows were appended, moved or evicted, call it for what changed: a decode
+        step passes the length before its append as start.  A stream named twice needs the same seq_len both times.  int8 symmetric
+        and 4-bit asymmetric caches.  See pikv_page_bounds_update."""
+        host().bounds(self._buffers, self.num_seqs, self.n_kv, self.bits, self.symmetric, self.max_pages, self.num_pages,
+                      bounds.codes, bounds.scale, seq_ids, start, seq_len)
+
+    def decode_attention_sparse(self, q: torch.Tensor, bounds: PageBounds, pages: int, seq_ids: Optional[torch.Tensor] = None,
+                                seq_len: Optional[torch.Tensor] = None, first: int = 0, recent: int = 1, want_lse: bool = False,
+                                want_pages: bool = False):
+        """decode_attention over at most `pages` pages (of 16 rows) of each stream and KV head: its `first` pages, its `recent` last
+        ones, and of those between them the ones on which a query head of the group can reach the largest logit, by the bounds
+        (ties: the lower page).  q [B, n_q, 128] bf16, up to 8 query heads per KV head.  Returns out [B, n_q, 128]; behind it with
+        want_lse the log-sum-exp [B, n_q] over the chosen pages, with want_pages the page numbers int32 [B, n_kv, pages],
+        ascending, -1 behind them.  The bounds must be up to date (update_bounds).  See pikv_sparse_attn."""
+        return host().sparse(self._buffers, self.num_seqs, self.n_kv, self.bits, self.symmetric, self.max_pages, self.num_pages,
+                             q, bounds.codes, bounds.scale, pages, seq_ids, seq_len, first, recent, want_lse, want_pages)
 
     # -- eviction ------------------------------------------------------------------
     def compact_into(self, dst: "PagedKVCache", keep_idx: torch.Tensor, kept_count: torch.Tensor, per_head: bool,
