@@ -3,6 +3,7 @@
 // Node i of a stream is the cache row at position ctx + i.  Its query sees the ctx rows before the tree and the nodes its
 // mask row names: out = sum_t w_t V_t, w = softmax(q . K_t / sqrt(128)) over the seen rows t.
 #include "stream_list.cuh"
+#include "tc_common.cuh"
 
 #include <type_traits>
 
@@ -34,71 +35,717 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
     return ctx;
 }
 
-constexpr int TS_THREADS = 128;
+// ---- attention --------------------------------------------------------------------------------------------------
+// The nodes of a stream times the query heads of one KV head are the rows of one product: S = Q K^T for 128 rows and 64 keys
+// at a time, O += P V, both by tcgen05 with the accumulators in tensor memory.  The keys of all (stream, head, 128 rows)
+// units form one list of tiles that a persistent grid cuts into equal runs, two CTAs per SM; a unit that one CTA holds
+// whole is finished there, the pieces of others go to the workspace and a second kernel joins them.
+//
+// A CTA's ten warps:
+//   0-3  softmax: thread = row.  S comes out of tensor memory, the weights go back into it as the A operand of the second
+//        product; a row's maximum, denominator and the rescaling of its O live in its thread
+//   4-7  one page of the tile each: codes to f16 (exact integers), into the swizzled layout that both products read
+//   8    bulk copies of pages into a ring, up to TR_STAGES pages ahead
+//   9    issues the MMAs: Q K^T of tile n before P V of tile n - 1, so that the products of one tile run while the softmax
+//        of another does
+// Nothing but exact integers enters the tensor cores on the cache side, and the query enters exactly: bf16 times a power of
+// two per row that brings its largest entry to 2^14 is f16 down to 2^-38 of that entry.
+//   logit = kscale (q . code - zp sum(q))        (zp = 0 for the 8-bit cache)
+//   O     = sum w code - sum w zp,  w = f16(2^(logit - R) vscale)
+// R is a row's reference: the largest logit (log2 domain) plus the exponent of the largest vscale seen with it, so that the
+// weights sit at the top of f16's range whatever the size of V; it moves only when a tile exceeds it by 2^TR_SLACK.  The
+// denominator is the fp32 sum of 2^(logit - R).
+constexpr int TR_THREADS = 320;
+constexpr int TR_ROWS = 128;             // rows of a unit
+constexpr int TR_KEYS = 64;              // keys of a tile
+constexpr int TR_PAGES = TR_KEYS / PIKV_PAGE_TOKENS;
+constexpr int TR_CTAS = 2;               // per SM
+constexpr int TR_MIN_TILES = 1;          // per CTA
+constexpr float TR_SLACK = 8.f;
+constexpr unsigned TR_WAIT_LIMIT = 1u << 24;
+constexpr uint32_t TR_COL_O = 0, TR_COL_S = 128, TR_COL_P = 192, TR_COLS = 256;
 
-// One warp per (stream, node, query head).  Scores: lane = (row of the page, half of the channels); output: lane = 4 channels.
+template <int BITS> struct TRGeom;
+template <> struct TRGeom<8> { static constexpr int STAGES = 10, ROW = 128, PAGE = 2048, STAGE = 2 * 2048 + 64, SIDES = 2; };
+template <> struct TRGeom<4> { static constexpr int STAGES = 18, ROW = 64, PAGE = 1024, STAGE = 2 * 1024 + 64 + 128, SIDES = 4; };
+
+// shared memory behind a 1024-byte boundary
+template <int BITS> struct TRSmem {
+    static constexpr int Q = 0, K = Q + 2 * TR_ROWS * 128, V = K + 2 * TR_KEYS * 128, RING = V + 2 * TR_KEYS * 128,
+                         SIDE = RING + TRGeom<BITS>::STAGES * TRGeom<BITS>::STAGE,             // [2][SIDES][64] fp32: ks, vs, kz, vz
+                         VEXP = SIDE + 2 * TRGeom<BITS>::SIDES * TR_KEYS * 4,                  // [2][4] exponents
+                         BARS = VEXP + 32, PRE = BARS + (2 * TRGeom<BITS>::STAGES + 17) * 8, MISC = PRE + (PIKV_STREAMS_PER_LAUNCH + 1) * 4,
+                         END = MISC + 16;
+    static constexpr int BYTES = END + 1024;
+};
+
+struct TreeParts {
+    float* o;                            // [2 C][rows][128]
+    float2* ml;                          // [2 C][rows] reference and denominator
+    int* plan;                           // [0] tiles per CTA, [1 ..] prefix of the streams' tiles
+    int rows;                            // rows of a slot
+};
+
+__device__ __forceinline__ int tree_tiles(int ctx, int nodes) { return (ctx + nodes + TR_KEYS - 1) / TR_KEYS; }
+__device__ __forceinline__ int tree_row_tiles(int nodes, int G) { return (nodes * G + TR_ROWS - 1) / TR_ROWS; }
+
+// a place in the list of tiles: stream b, unit (head, 128 rows) of it, tile of the unit
+struct TreeCursor {
+    int b, unit, tile;
+    int tiles, row_tiles;                // of the stream
+    int row, ctx, nodes;
+    __device__ __forceinline__ void load(const TreeDev& d) {
+        ctx = tree_lengths(d, b, row, nodes);
+        tiles = tree_tiles(ctx, nodes);
+        row_tiles = tree_row_tiles(nodes, d.G);
+    }
+    __device__ __forceinline__ void start(const TreeDev& d, const int* pre, int f) {
+        b = stream_of(pre, d.B, f);
+        load(d);
+        unit = (f - pre[b]) / tiles;
+        tile = (f - pre[b]) % tiles;
+    }
+    __device__ __forceinline__ void next(const TreeDev& d, const int* pre, int f) {      // f: the place after this one
+        if (++tile < tiles) return;
+        tile = 0;
+        if (++unit < d.c.n_kv * row_tiles) return;
+        unit = 0;
+        do ++b; while (pre[b + 1] <= f);
+        load(d);
+    }
+    __device__ __forceinline__ int head() const { return unit / row_tiles; }
+    __device__ __forceinline__ int row_tile() const { return unit % row_tiles; }
+};
+
+__device__ __forceinline__ bool tr_wait(uint32_t bar, uint32_t parity) {
+    for (unsigned i = 0; i < TR_WAIT_LIMIT; ++i) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void tr_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// A from tensor memory (f16, two to a column), B from shared memory
+__device__ __forceinline__ void tr_mma_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void tr_tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// loads done; ties their 32 registers to the wait, so that nothing of theirs is used before it
+__device__ __forceinline__ void tr_tmem_ld_wait(float* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
+                   "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
+                   "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :: "memory");
+}
+__device__ __forceinline__ void tr_tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tr_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tr_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tr_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tr_fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float tr_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// two fp32 operations per instruction
+__device__ __forceinline__ float2 tr_mul2(float2 a, float2 b) {
+    float2 c;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 tr_fma2(float2 a, float2 b, float2 c) {
+    float2 e;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(e.x), "=f"(e.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return e;
+}
+__device__ __forceinline__ float2 tr_add2(float2 a, float2 b) {
+    float2 c;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ uint32_t tr_pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// exponent of a scale, for the reference; what is not finite has no say in it
+__device__ __forceinline__ int tr_exponent(uint32_t bits) {
+    const int e = (int)((bits >> 23) & 0xffu);
+    return e == 255 ? -100 : min(100, max(-100, e - 126));
+}
+// position of a channel inside its group of eight in the 4-bit tiles: nibbles leave a word as (0, 4), (1, 5), (2, 6), (3, 7)
+template <int BITS> __device__ __forceinline__ constexpr int tr_channel(int at) { return BITS == 8 ? at : (at & ~7) | ((at & 7) >> 1) | ((at & 1) << 2); }
+
+// 16 codes (8 bit) of a row's chunk, or 16 of a 4-bit row's unit, as f16: eight to each of two 16-byte pieces
 template <int BITS>
-__global__ void __launch_bounds__(TS_THREADS) tree_attn_simple_kernel(TreeDev d) {
-    __shared__ float qs[TS_THREADS / 32][128];
+__device__ __forceinline__ void tr_codes(const unsigned char* p, uint4& first, uint4& second) {
+    auto bytes = [](uint32_t w, uint32_t sel) {
+        uint32_t x = __byte_perm(w, 0x64646464u, sel);                 // 1024 + (code + 128), exact in f16
+        __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+        return *reinterpret_cast<uint32_t*>(&h);
+    };
+    auto nibbles = [](uint32_t w) {
+        uint32_t x = (w & 0x000f000fu) | 0x64006400u;                  // 1024 + n, centred: n - 8
+        __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6408)));
+        return *reinterpret_cast<uint32_t*>(&h);
+    };
+    if constexpr (BITS == 8) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u, c = w.z ^ 0x80808080u, e = w.w ^ 0x80808080u;
+        first = make_uint4(bytes(a, 0x4140), bytes(a, 0x4342), bytes(b, 0x4140), bytes(b, 0x4342));
+        second = make_uint4(bytes(c, 0x4140), bytes(c, 0x4342), bytes(e, 0x4140), bytes(e, 0x4342));
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        first = make_uint4(nibbles(w.x), nibbles(w.x >> 4), nibbles(w.x >> 8), nibbles(w.x >> 12));
+        second = make_uint4(nibbles(w.y), nibbles(w.y >> 4), nibbles(w.y >> 8), nibbles(w.y >> 12));
+    }
+}
+// one page of codes into its 16 rows of a [2 halves][64 keys][128 bytes] tile, by one warp.  Eight lanes read a row where the
+// cache's swizzle has put it; of the two pieces of a chunk, lanes of the upper half of the channels store the second one first:
+// eight lanes then fill eight different 16-byte columns.
+template <int BITS>
+__device__ __forceinline__ void tr_convert(const unsigned char* raw, unsigned char* tile, int page, int lane) {
+    const int at = lane & 7;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        const int c = BITS == 8 ? at ^ (r & 7) : at ^ (r & 4);         // logical chunk: channels 16 c ..
+        uint4 x, y;
+        tr_codes<BITS>(raw + r * TRGeom<BITS>::ROW + at * (TRGeom<BITS>::ROW / 8), x, y);
+        const bool upper = c >= 4;
+        unsigned char* row = tile + (upper ? TR_KEYS * 128 : 0) + (page * PIKV_PAGE_TOKENS + r) * 128;
+        const int d0 = (2 * (c & 3)) ^ (r & 7), d1 = (2 * (c & 3) + 1) ^ (r & 7);
+        *reinterpret_cast<uint4*>(row + 16 * (upper ? d1 : d0)) = upper ? y : x;
+        *reinterpret_cast<uint4*>(row + 16 * (upper ? d0 : d1)) = upper ? x : y;
+    }
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev d, TreeParts parts) {
+    using GEO = TRGeom<BITS>;
+    using SM = TRSmem<BITS>;
+    constexpr int STAGES = GEO::STAGES;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (lr_smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = lr_smem_u32(smem);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int* pre = reinterpret_cast<int*>(smem + SM::PRE);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::MISC);
+    const uint32_t bars = sbase + SM::BARS;
+    const uint32_t raw_full = bars, raw_empty = bars + 8 * STAGES, b0 = bars + 16 * STAGES;
+    const uint32_t k_full = b0, k_empty = b0 + 8, v_full = b0 + 16, v_empty = b0 + 24, s_full = b0 + 32, s_empty = b0 + 40, p_full = b0 + 48,
+                   pv_done = b0 + 64, side_full = b0 + 80, side_empty = b0 + 96, q_full = b0 + 112;
+    dependency_release();
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; ++i) lr_mbar_init(raw_full + 8 * i, 1), lr_mbar_init(raw_empty + 8 * i, 1);
+        lr_mbar_init(k_full, 4); lr_mbar_init(k_empty, 1);
+        lr_mbar_init(v_full, 4); lr_mbar_init(v_empty, 1);
+        lr_mbar_init(s_full, 1); lr_mbar_init(s_empty, 4);
+        lr_mbar_init(q_full, 4);
+        for (int i = 0; i < 2; ++i) {
+            lr_mbar_init(p_full + 8 * i, 4); lr_mbar_init(pv_done + 8 * i, 1);
+            lr_mbar_init(side_full + 8 * i, 4); lr_mbar_init(side_empty + 8 * i, 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // keys behind a stream's last page keep what was in the tile: weights of 0 times something finite
+    for (int i = tid; i < 4 * TR_KEYS * 128 / 16; i += TR_THREADS) reinterpret_cast<uint4*>(smem + SM::K)[i] = make_uint4(0u, 0u, 0u, 0u);
+    tr_fence_smem();
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lr_smem_u32(tmem_slot)), "r"(TR_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    dependency_wait();
+    const int total = stream_prefix<TR_THREADS>(d.B, pre, [&](int i) {
+        int row, nodes;
+        const int ctx = tree_lengths(d, i, row, nodes);
+        if (row < 0 && blockIdx.x == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_SEQ);
+        return nodes > 0 ? d.c.n_kv * tree_row_tiles(nodes, d.G) * tree_tiles(ctx, nodes) : 0;
+    });
+    const int per = max(TR_MIN_TILES, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    if (blockIdx.x == 0) {
+        if (tid == 0) parts.plan[0] = per;
+        for (int i = tid; i <= d.B; i += TR_THREADS) parts.plan[1 + i] = pre[i];
+    }
+    tr_fence_before();
+    __syncthreads();
+    tr_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int f0 = (int)min((long long)total, (long long)blockIdx.x * per), f1 = min(total, f0 + per);
+    bool failed = false;
+
+    if (f0 < f1) {
+        TreeCursor cur;
+        cur.start(d, pre, f0);
+        if (warp == 8) {
+            // ---- pages into the ring ----
+            int issued = 0, ids = -1, ids_row = -2, ids_at = 0;
+            for (int f = f0; f < f1 && !failed; ++f) {
+                const int h = cur.head(), p0 = cur.tile * TR_PAGES;
+                const int np = min(TR_PAGES, (cur.ctx + cur.nodes + PIKV_PAGE_TOKENS - 1) / PIKV_PAGE_TOKENS - p0);
+                if (cur.row != ids_row || p0 < ids_at || p0 >= ids_at + 32) {
+                    ids_row = cur.row;
+                    ids_at = p0;
+                    ids = p0 + lane < d.c.max_pages ? __ldg(d.c.page_table + (size_t)cur.row * d.c.max_pages + p0 + lane) : -1;
+                }
+                for (int i = 0; i < np; ++i) {
+                    const int s = issued % STAGES;
+                    int page = __shfl_sync(0xffffffffu, ids, p0 + i - ids_at);
+                    if (page < 0 || page >= d.c.num_pages) {
+                        if (lane == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_PAGE);
+                        page = 0;
+                    }
+                    if (!tr_wait(raw_empty + 8 * s, ((uint32_t)(issued / STAGES) & 1u) ^ 1u)) { failed = true; break; }
+                    const uint32_t bar = raw_full + 8 * s, dst = sbase + SM::RING + s * GEO::STAGE;
+                    if (lane == 0) lr_mbar_expect_tx(bar, GEO::STAGE);
+                    __syncwarp();
+                    const size_t prow = ((size_t)page * d.c.n_kv + h) * PIKV_PAGE_TOKENS;
+                    if (lane == 0) tr_bulk(dst, d.c.k_codes + prow * GEO::ROW, GEO::PAGE, bar);
+                    if (lane == 1) tr_bulk(dst + GEO::PAGE, d.c.v_codes + prow * GEO::ROW, GEO::PAGE, bar);
+                    if (lane == 2) tr_bulk(dst + 2 * GEO::PAGE, d.c.k_scale + prow, 32, bar);
+                    if (lane == 3) tr_bulk(dst + 2 * GEO::PAGE + 32, d.c.v_scale + prow, 32, bar);
+                    if (BITS == 4 && lane == 4) tr_bulk(dst + 2 * GEO::PAGE + 64, d.c.k_zp + prow, 64, bar);
+                    if (BITS == 4 && lane == 5) tr_bulk(dst + 2 * GEO::PAGE + 128, d.c.v_zp + prow, 64, bar);
+                    ++issued;
+                }
+                if (f + 1 < f1) cur.next(d, pre, f + 1);
+            }
+            // a consumer that gave up leaves copies behind: they land before this CTA's shared memory goes to another
+            for (int i = max(0, issued - STAGES); i < issued; ++i) failed |= !tr_wait(raw_full + 8 * (i % STAGES), (uint32_t)(i / STAGES) & 1u);
+        } else if (warp == 9) {
+            // ---- the products ----
+            const uint32_t idesc_qk = (1u << 4) | ((uint32_t)(TR_KEYS >> 3) << 17) | ((uint32_t)(TR_ROWS >> 4) << 24);
+            const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(TR_ROWS >> 4) << 24);
+            const uint32_t q_lo = lr_desc_lo(sbase + SM::Q), k_lo = lr_desc_lo(sbase + SM::K);
+            // V: [64 channels][keys], channels contiguous: 64-channel halves 8192 bytes apart (leading), 8-key groups 1024 (stride)
+            const uint32_t v_lo = (((sbase + SM::V) & 0x3FFFFu) >> 4) | ((uint32_t)(TR_KEYS * 128 >> 4) << 16);
+            const int count = f1 - f0;
+            int seg = 0;
+            bool first_before = true;                                // whether tile n - 1 opened its unit here
+            auto pv = [&](int m, bool first) {
+                if (!tr_wait(p_full + 8 * (m & 1), (uint32_t)(m >> 1) & 1u) || !tr_wait(v_full, (uint32_t)m & 1u)) return false;
+                tr_fence_after();
+                if (lr_elect()) {
+#pragma unroll
+                    for (int k = 0; k < TR_KEYS / 16; ++k)
+                        tr_mma_ta(tmem + TR_COL_O, tmem + TR_COL_P + 32 * (m & 1) + 8 * k, lr_desc(v_lo + 128 * k), idesc_pv, !first || k ? 1u : 0u);
+                    lr_commit(v_empty);
+                    lr_commit(pv_done + 8 * (m & 1));
+                }
+                __syncwarp();
+                return true;
+            };
+            for (int n = 0; n < count && !failed; ++n) {
+                const bool first = n == 0 || cur.tile == 0;
+                if (first) {
+                    // the next unit's Q takes the place of this one's after its last product
+                    if (n > 0 && !pv(n - 1, first_before)) { failed = true; break; }
+                    if (!tr_wait(q_full, (uint32_t)seg & 1u)) { failed = true; break; }
+                    ++seg;
+                }
+                if (!tr_wait(k_full, (uint32_t)n & 1u) || !tr_wait(s_empty, ((uint32_t)n & 1u) ^ 1u)) { failed = true; break; }
+                tr_fence_after();
+                if (lr_elect()) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        lr_mma(tmem + TR_COL_S, lr_desc(q_lo + (k >> 2) * (TR_ROWS * 128 >> 4) + 2 * (k & 3)),
+                               lr_desc(k_lo + (k >> 2) * (TR_KEYS * 128 >> 4) + 2 * (k & 3)), idesc_qk, k ? 1u : 0u);
+                    lr_commit(s_full);
+                    lr_commit(k_empty);
+                }
+                __syncwarp();
+                if (!first && !pv(n - 1, first_before)) { failed = true; break; }
+                first_before = first;
+                if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
+            }
+            if (!failed) failed = !pv(count - 1, first_before);
+            // nothing of this CTA's is in flight when its tensor memory goes back
+            if (!failed) failed = !tr_wait(pv_done + 8 * ((count - 1) & 1), (uint32_t)((count - 1) >> 1) & 1u);
+        } else if (warp >= 4) {
+            // ---- codes to f16 ----
+            const int w = warp - 4;
+            int page0 = 0;                                            // pages of the tiles before this one
+            for (int n = 0, f = f0; f < f1; ++f, ++n) {
+                const int end = cur.ctx + cur.nodes, p0 = cur.tile * TR_PAGES;
+                const int np = min(TR_PAGES, (end + PIKV_PAGE_TOKENS - 1) / PIKV_PAGE_TOKENS - p0);
+                const int i = page0 + w, s = i % STAGES;
+                const unsigned char* raw = smem + SM::RING + s * GEO::STAGE;
+                const bool mine = w < np;
+                if (mine && !tr_wait(raw_full + 8 * s, (uint32_t)(i / STAGES) & 1u)) { failed = true; break; }
+                if (!tr_wait(side_empty + 8 * (n & 1), ((uint32_t)(n >> 1) & 1u) ^ 1u)) { failed = true; break; }
+                {
+                    // lanes 0-15: scales (and zero points) of K, 16-31: of V; rows behind the end have none
+                    const int r = lane & 15, side = lane >> 4;
+                    const bool there = mine && (p0 + w) * PIKV_PAGE_TOKENS + r < end;
+                    const uint32_t bits16 = there ? reinterpret_cast<const uint16_t*>(raw + 2 * GEO::PAGE)[lane] : 0u;
+                    float* to = reinterpret_cast<float*>(smem + SM::SIDE) + (n & 1) * GEO::SIDES * TR_KEYS + side * TR_KEYS + w * PIKV_PAGE_TOKENS + r;
+                    // a key of infinities has a logit that is not a number, whatever the sign of the whole product
+                    *to = side == 0 && (bits16 & 0x7f80u) == 0x7f80u ? __uint_as_float(0x7fffffffu) : __uint_as_float(bits16 << 16);
+                    if (BITS == 4) to[2 * TR_KEYS] = there ? reinterpret_cast<const float*>(raw + 2 * GEO::PAGE + 64)[lane] - 8.f : 0.f;
+                    int e = side ? tr_exponent(bits16 << 16) : -100;
+                    e = __reduce_max_sync(0xffffffffu, e);
+                    if (lane == 0) reinterpret_cast<int*>(smem + SM::VEXP)[(n & 1) * 4 + w] = e;
+                }
+                __syncwarp();
+                if (lane == 0) lr_mbar_arrive(side_full + 8 * (n & 1));
+                if (!tr_wait(k_empty, ((uint32_t)n & 1u) ^ 1u)) { failed = true; break; }
+                if (mine) tr_convert<BITS>(raw, smem + SM::K, w, lane);
+                tr_fence_smem();
+                __syncwarp();
+                if (lane == 0) lr_mbar_arrive(k_full);
+                if (!tr_wait(v_empty, ((uint32_t)n & 1u) ^ 1u)) { failed = true; break; }
+                if (mine) tr_convert<BITS>(raw + GEO::PAGE, smem + SM::V, w, lane);
+                tr_fence_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    lr_mbar_arrive(v_full);
+                    if (mine) lr_mbar_arrive(raw_empty + 8 * s);
+                }
+                page0 += np;
+                if (f + 1 < f1) cur.next(d, pre, f + 1);
+            }
+        } else {
+            // ---- softmax: thread = row ----
+            const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+            float qmul = 0.f, qsum = 0.f, ref = -INFINITY, den = 0.f, corr = 0.f;
+            uint64_t tree = 0;
+            int node = 0;
+            bool live = false, warp_live = false;
+            size_t out_row = 0;
+            for (int n = 0, f = f0; f < f1; ++f, ++n) {
+                const bool first = n == 0 || cur.tile == 0;
+                if (first) {
+                    // ---- this row's query ----
+                    const int row = cur.row_tile() * TR_ROWS + tid, h = cur.head();
+                    node = row / d.G;
+                    live = node < cur.nodes;
+                    warp_live = __any_sync(0xffffffffu, live);
+                    ref = -INFINITY;
+                    den = corr = 0.f;
+                    if (warp_live) {
+                        out_row = ((size_t)cur.b * d.N + (live ? node : 0)) * d.n_q + (size_t)h * d.G + row % d.G;
+                        const uint4* src = reinterpret_cast<const uint4*>(d.q + out_row * 128);
+                        float amax = 0.f, odd = 0.f;
+#pragma unroll 4
+                        for (int i = 0; i < 16; ++i) {
+                            const uint4 w4 = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+                            const uint32_t ww[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                float x, y;
+                                bf16x2_to_f32(ww[k], x, y);
+                                amax = fmaxf(amax, fmaxf(fabsf(x), fabsf(y)));
+                                odd += x * 0.f + y * 0.f;             // NaN where the row is not finite
+                            }
+                        }
+                        const int sh = amax > 0.f && amax < INFINITY ? min(126, 14 - ((int)(__float_as_uint(amax) >> 23) - 127)) : 0;
+                        const float up = exp2_int(max(sh, -126));
+                        qsum = 0.f;
+#pragma unroll 4
+                        for (int i = 0; i < 16; ++i) {
+                            const uint4 w4 = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+                            float x[8];
+                            bf16x2_to_f32(w4.x, x[0], x[1]);
+                            bf16x2_to_f32(w4.y, x[2], x[3]);
+                            bf16x2_to_f32(w4.z, x[4], x[5]);
+                            bf16x2_to_f32(w4.w, x[6], x[7]);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                x[k] *= up;
+                                qsum += x[k];
+                            }
+                            uint4 y;
+                            y.x = tr_pack(x[tr_channel<BITS>(0)], x[tr_channel<BITS>(1)]);
+                            y.y = tr_pack(x[tr_channel<BITS>(2)], x[tr_channel<BITS>(3)]);
+                            y.z = tr_pack(x[tr_channel<BITS>(4)], x[tr_channel<BITS>(5)]);
+                            y.w = tr_pack(x[tr_channel<BITS>(6)], x[tr_channel<BITS>(7)]);
+                            *reinterpret_cast<uint4*>(smem + SM::Q + (i >> 3) * TR_ROWS * 128 + tid * 128 + 16 * ((i & 7) ^ (tid & 7))) = y;
+                        }
+                        qmul = exp2_int(-max(sh, -126)) * (0.08838834764831845f * 1.4426950408889634f) + odd;
+                        // what this node sees of the tree, a bit per node
+                        tree = 0;
+                        if (live) {
+                            const uint8_t* m = d.mask + (size_t)cur.b * d.mask_stride + (size_t)node * d.N;
+                            for (int i = 0; i < cur.nodes; ++i) tree |= (uint64_t)(__ldg(m + i) != 0) << i;
+                        }
+                        tr_fence_smem();
+                    }
+                    __syncwarp();
+                    if (lane == 0) lr_mbar_arrive(q_full);
+                }
+                if (!tr_wait(s_full, (uint32_t)n & 1u) || !tr_wait(side_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u)) { failed = true; break; }
+                const bool last = f + 1 == f1 || cur.tile + 1 == cur.tiles;
+                if (warp_live) {
+                    tr_fence_after();
+                    float x[TR_KEYS];
+                    tr_tmem_ld32(tmem + lanes + TR_COL_S, x);
+                    tr_tmem_ld32(tmem + lanes + TR_COL_S + 32, x + 32);
+                    tr_tmem_ld_wait(x);
+                    tr_tmem_ld_wait(x + 32);
+                    tr_fence_before();
+                    __syncwarp();
+                    if (lane == 0) lr_mbar_arrive(s_empty);
+                    const float* ks = reinterpret_cast<const float*>(smem + SM::SIDE) + (n & 1) * GEO::SIDES * TR_KEYS;
+                    const float* vs = ks + TR_KEYS;
+                    const float* kz = ks + 2 * TR_KEYS;
+                    const float* vz = ks + 3 * TR_KEYS;
+                    const int4 ve = *reinterpret_cast<const int4*>(smem + SM::VEXP + (n & 1) * 16);
+                    const int pos0 = cur.tile * TR_KEYS;
+                    // scaled scores; the positions behind the context show only where the mask opens them
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < TR_KEYS; j += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4*>(ks + j);
+                        float2 a = make_float2(x[j], x[j + 1]), c = make_float2(x[j + 2], x[j + 3]);
+                        if (BITS == 4) {
+                            const float4 z4 = *reinterpret_cast<const float4*>(kz + j);
+                            a = tr_fma2(make_float2(z4.x, z4.y), make_float2(-qsum, -qsum), a);
+                            c = tr_fma2(make_float2(z4.z, z4.w), make_float2(-qsum, -qsum), c);
+                        }
+                        a = tr_mul2(a, make_float2(s4.x, s4.y));
+                        c = tr_mul2(c, make_float2(s4.z, s4.w));
+                        x[j] = a.x; x[j + 1] = a.y; x[j + 2] = c.x; x[j + 3] = c.y;
+                    }
+                    uint64_t seen = ~0ull;
+                    int vexp = max(max(ve.x, ve.y), max(ve.z, ve.w));
+                    const bool edge = pos0 + TR_KEYS > cur.ctx;          // the same for the whole CTA
+                    if (edge) {
+                        const int sh = cur.ctx - pos0;                   // the tree's first bit
+                        seen = sh >= 0 ? (sh < 64 ? tree << sh : 0ull) | ((1ull << sh) - 1) : (sh > -64 ? tree >> -sh : 0ull);
+                        vexp = -100;                                     // of the rows that this one sees
+#pragma unroll
+                        for (int j = 0; j < TR_KEYS; ++j) {
+                            if ((seen >> j) & 1) vexp = max(vexp, tr_exponent(__float_as_uint(vs[j])));
+                            else x[j] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < TR_KEYS; ++j) mx = fmaxf(mx, x[j]);
+                    // does the reference hold?  (-inf while nothing has been seen)
+                    const float want = mx * qmul + (float)vexp;
+                    const bool move = mx > -INFINITY && want > ref + TR_SLACK;
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float next = move ? want : ref;
+                        const float fac = move ? tr_ex2(ref - next) : 1.f;     // 0 from -inf
+                        ref = next;
+                        den *= fac;
+                        corr *= fac;
+                        if (!first) {
+                            if (!tr_wait(pv_done + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u)) { failed = true; break; }
+                            tr_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < 128; c += 32) {
+                                float o[32];
+                                tr_tmem_ld32(tmem + lanes + TR_COL_O + c, o);
+                                tr_tmem_ld_wait(o);
+                                uint32_t r[32];
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(o[i] * fac);
+                                tr_tmem_st32(tmem + lanes + TR_COL_O + c, r);
+                            }
+                            tr_tmem_st_wait();
+                        }
+                    }
+                    const float off = ref == -INFINITY ? 0.f : -ref;
+                    float2 sum = make_float2(0.f, 0.f);
+                    uint32_t wgt[TR_KEYS / 2];
+#pragma unroll
+                    for (int j = 0; j < TR_KEYS; j += 4) {
+                        const float4 v4 = *reinterpret_cast<const float4*>(vs + j);
+                        float2 a = tr_fma2(make_float2(x[j], x[j + 1]), make_float2(qmul, qmul), make_float2(off, off));
+                        float2 c = tr_fma2(make_float2(x[j + 2], x[j + 3]), make_float2(qmul, qmul), make_float2(off, off));
+                        a = make_float2(tr_ex2(a.x), tr_ex2(a.y));
+                        c = make_float2(tr_ex2(c.x), tr_ex2(c.y));
+                        sum = tr_add2(sum, tr_add2(a, c));
+                        a = tr_mul2(a, make_float2(v4.x, v4.y));
+                        c = tr_mul2(c, make_float2(v4.z, v4.w));
+                        if (edge) {                                      // 0 times a scale that is not finite
+                            if (!((seen >> j) & 1)) a.x = 0.f;
+                            if (!((seen >> (j + 1)) & 1)) a.y = 0.f;
+                            if (!((seen >> (j + 2)) & 1)) c.x = 0.f;
+                            if (!((seen >> (j + 3)) & 1)) c.y = 0.f;
+                        }
+                        wgt[j / 2] = tr_pack(a.x, a.y);
+                        wgt[j / 2 + 1] = tr_pack(c.x, c.y);
+                        if (BITS == 4) {
+                            const float4 z4 = *reinterpret_cast<const float4*>(vz + j);
+                            const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2]));
+                            const float2 rc = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2 + 1]));
+                            if (edge) {
+                                corr += (ra.x ? ra.x * z4.x : 0.f) + (ra.y ? ra.y * z4.y : 0.f) + (rc.x ? rc.x * z4.z : 0.f) + (rc.y ? rc.y * z4.w : 0.f);
+                            } else {
+                                const float2 t = tr_fma2(ra, make_float2(z4.x, z4.y), tr_mul2(rc, make_float2(z4.z, z4.w)));
+                                corr += t.x + t.y;
+                            }
+                        }
+                    }
+                    den += sum.x + sum.y;
+                    __syncwarp();
+                    if (lane == 0) lr_mbar_arrive(side_empty + 8 * (n & 1));
+                    if (n >= 2 && !tr_wait(pv_done + 8 * (n & 1), (uint32_t)((n - 2) >> 1) & 1u)) { failed = true; break; }
+                    tr_fence_after();
+                    tr_tmem_st32(tmem + lanes + TR_COL_P + 32 * (n & 1), wgt);
+                    tr_tmem_st_wait();
+                    tr_fence_before();
+                    __syncwarp();
+                    if (lane == 0) lr_mbar_arrive(p_full + 8 * (n & 1));
+                } else if (lane == 0) {
+                    lr_mbar_arrive(s_empty);
+                    lr_mbar_arrive(side_empty + 8 * (n & 1));
+                    lr_mbar_arrive(p_full + 8 * (n & 1));
+                }
+                if (last) {
+                    // ---- this CTA's share of the unit is done ----
+                    if (!tr_wait(pv_done + 8 * (n & 1), (uint32_t)(n >> 1) & 1u)) { failed = true; break; }
+                    if (warp_live) {
+                        tr_fence_after();
+                        const int begun = f - cur.tile;                  // place of the unit's first tile
+                        const bool whole = begun >= f0 && cur.tile + 1 == cur.tiles;
+                        const float inv = den == 0.f ? 0.f : 1.f / den;
+                        const size_t slot = (size_t)(2 * blockIdx.x + (begun >= f0 ? 1 : 0)) * parts.rows + tid;
+#pragma unroll 1
+                        for (int c = 0; c < 128; c += 32) {
+                            float o[32];
+                            tr_tmem_ld32(tmem + lanes + TR_COL_O + c, o);
+                            tr_tmem_ld_wait(o);
+                            if (BITS == 4) {
+                                float t[32];
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) t[tr_channel<BITS>(i)] = o[i] - corr;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = t[i];
+                            }
+                            if (live && whole) {
+                                uint4* to = reinterpret_cast<uint4*>(d.out + out_row * 128 + c);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    uint32_t r[4];
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) {
+                                        const __nv_bfloat162 h2 = __floats2bfloat162_rn(den == 0.f ? 0.f : o[8 * i + 2 * k] * inv, den == 0.f ? 0.f : o[8 * i + 2 * k + 1] * inv);
+                                        r[k] = *reinterpret_cast<const uint32_t*>(&h2);
+                                    }
+                                    to[i] = make_uint4(r[0], r[1], r[2], r[3]);
+                                }
+                            } else if (live) {
+                                float4* to = reinterpret_cast<float4*>(parts.o + slot * 128 + c);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            }
+                            __syncwarp();
+                        }
+                        if (live && whole && d.lse) d.lse[out_row] = den == 0.f ? -INFINITY : ref * 0.6931471805599453f + logf(den);
+                        if (live && !whole) parts.ml[slot] = make_float2(ref, den);
+                        tr_fence_before();
+                    }
+                }
+                if (f + 1 < f1) cur.next(d, pre, f + 1);
+            }
+        }
+        if (failed && lane == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_WAIT_TIMEOUT);
+    }
+    tr_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tr_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TR_COLS) : "memory");
+    }
+}
+
+constexpr int TM_THREADS = 128;
+
+// Joins the pieces of units that were cut, and answers for the rows that no unit has.  One warp per (stream, node, query head),
+// lane = 4 channels: O = sum_i O_i 2^(R_i - R), the denominator likewise.
+__global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeParts parts) {
     dependency_release();
     dependency_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long unit = (long long)blockIdx.x * (TS_THREADS / 32) + warp;
-    if (unit >= (long long)d.B * d.N * d.n_q) return;
-    const int qh = (int)(unit % d.n_q), node = (int)(unit / d.n_q % d.N), b = (int)(unit / d.n_q / d.N);
-    const int h = qh / d.G;
+    const int lane = threadIdx.x & 31;
+    const long long at = (long long)blockIdx.x * (TM_THREADS / 32) + (threadIdx.x >> 5);
+    if (at >= (long long)d.B * d.N * d.n_q) return;
+    const int qh = (int)(at % d.n_q), node = (int)(at / d.n_q % d.N), b = (int)(at / d.n_q / d.N);
+    const int per = parts.plan[0], pre0 = parts.plan[1 + b];
     int row, nodes;
     const int ctx = tree_lengths(d, b, row, nodes);
-    if (row < 0 && lane == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_SEQ);
-    const int total = node < nodes ? ctx + nodes : 0;
-    for (int i = lane; i < 128; i += 32) qs[warp][i] = __bfloat162float(d.q[unit * 128 + i]);
-    __syncwarp();
-    const uint8_t* mask = d.mask + (size_t)b * d.mask_stride + (size_t)node * d.N;
-    const int r = lane & 15, half = lane >> 4;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 < total; p0 += PIKV_PAGE_TOKENS) {
-        const int page = stream_page(d.c, row, p0 / PIKV_PAGE_TOKENS);
-        const size_t base = ((size_t)page * d.c.n_kv + h) * PIKV_PAGE_TOKENS;
-        const int pos = p0 + r;
-        const bool open = pos < ctx || (pos < total && mask[pos - ctx] != 0);
-        float s = 0.f;
-        if (open) {
-            const float ks = bf16_bits_to_f32(d.c.k_scale[base + r]), kz = BITS == 4 ? d.c.k_zp[base + r] : 0.f;
-            for (int i = 0; i < 64; ++i) {
-                const int c = 64 * half + i;
-                float code;
-                if (BITS == 8) code = (float)(int8_t)d.c.k_codes[(base + r) * 128 + 16 * ((c >> 4) ^ (r & 7)) + (c & 15)];
-                else code = (float)((d.c.k_codes[(base + r) * 64 + 8 * ((c >> 4) ^ (r & 4)) + ((c & 15) >> 1)] >> (4 * (c & 1))) & 15) - kz;
-                s += qs[warp][c] * code;
-            }
-            s *= ks * 0.08838834764831845f;
-        }
-        s += __shfl_xor_sync(0xffffffffu, s, 16);
-        if (!open) s = -INFINITY;
-        const float mn = fmaxf(m, warp_max(s)), mu = mn == -INFINITY ? 0.f : mn;
-        const float p = expf(s - mu), al = expf(m - mu);
-        l = l * al + warp_sum(half ? 0.f : p);
-        m = mn;
+    uint2* out = reinterpret_cast<uint2*>(d.out + at * 128) + lane;
+    if (node >= nodes) {
+        *out = make_uint2(0u, 0u);
+        if (lane == 0 && d.lse) d.lse[at] = -INFINITY;
+        return;
+    }
+    const int tiles = tree_tiles(ctx, nodes), row_tiles = tree_row_tiles(nodes, d.G);
+    const int r = node * d.G + qh % d.G;
+    const int f0 = pre0 + ((qh / d.G) * row_tiles + r / TR_ROWS) * tiles, f1 = f0 + tiles;
+    const int c0 = f0 / per, c1 = (f1 - 1) / per;
+    if (c0 == c1) return;                                               // whole: written by its CTA
+    auto slot = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * parts.rows + r % TR_ROWS; };
+    float M = -INFINITY, den = 0.f;
+    for (int g = c0; g <= c1; g += 32) M = fmaxf(M, warp_max(g + lane <= c1 ? parts.ml[slot(g + lane)].x : -INFINITY));
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g = c0; g <= c1; g += 32) {
+        const int cnt = min(32, c1 - g + 1);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < cnt) ml = parts.ml[slot(g + lane)];
+        // a piece that saw nothing has no weight; one that is not a number keeps it
+        const float w_l = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - (M == -INFINITY ? 0.f : M));
+        for (int i = 0; i < cnt; i += 4) {
+            float4 o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= al;
-        for (int t = 0; t < PIKV_PAGE_TOKENS; ++t) {
-            const float w = __shfl_sync(0xffffffffu, p, t);
-            if (!__shfl_sync(0xffffffffu, (int)open, t)) continue;
-            const float vs = bf16_bits_to_f32(d.c.v_scale[base + t]), vz = BITS == 4 ? d.c.v_zp[base + t] : 0.f;
+            for (int u = 0; u < 4; ++u)
+                if (i + u < cnt) o[u] = reinterpret_cast<const float4*>(parts.o + slot(g + i + u) * 128)[lane];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = 4 * lane + i;
-                float code;
-                if (BITS == 8) code = (float)(int8_t)d.c.v_codes[(base + t) * 128 + 16 * ((c >> 4) ^ (t & 7)) + (c & 15)];
-                else code = (float)((d.c.v_codes[(base + t) * 64 + 8 * ((c >> 4) ^ (t & 4)) + ((c & 15) >> 1)] >> (4 * (c & 1))) & 15) - vz;
-                o[i] += w * (code * vs);
+            for (int u = 0; u < 4; ++u) {
+                if (i + u >= cnt) break;
+                const float w = __shfl_sync(0xffffffffu, w_l, i + u), l = __shfl_sync(0xffffffffu, ml.y, i + u);
+                acc.x += o[u].x * w; acc.y += o[u].y * w; acc.z += o[u].z * w; acc.w += o[u].w * w;
+                den += l * w;
             }
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;                 // nothing seen: zero; NaN stays NaN
-#pragma unroll
-    for (int i = 0; i < 4; ++i) d.out[unit * 128 + 4 * lane + i] = __float2bfloat16_rn(o[i] * inv);
-    if (lane == 0 && d.lse) d.lse[unit] = l == 0.f ? -INFINITY : m + logf(l);
+    const bool any = den != 0.f;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(any ? acc.x / den : 0.f, any ? acc.y / den : 0.f);
+    const __nv_bfloat162 hi = __floats2bfloat162_rn(any ? acc.z / den : 0.f, any ? acc.w / den : 0.f);
+    *out = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    if (lane == 0 && d.lse) d.lse[at] = any ? (M == -INFINITY ? 0.f : M) * 0.6931471805599453f + logf(den) : -INFINITY;
+}
+
+static int tree_slot_rows(int N, int G) { return std::min(TR_ROWS, N * G); }
+struct TreeLayout {
+    size_t ml, o, total;
+};
+static TreeLayout tree_layout(int N, int G) {
+    const size_t slots = (size_t)2 * sm_count() * TR_CTAS, rows = tree_slot_rows(N, G);
+    TreeLayout l;
+    l.ml = ((size_t)(PIKV_STREAMS_PER_LAUNCH + 2) * sizeof(int) + 255) & ~(size_t)255;
+    l.o = l.ml + slots * rows * sizeof(float2);
+    l.total = l.o + slots * rows * 128 * sizeof(float);
+    return l;
 }
 
 // ---- acceptance -------------------------------------------------------------------------------------------------
@@ -209,7 +856,7 @@ using namespace pikv;
 
 extern "C" size_t pikv_tree_attn_workspace_bytes(int32_t B, int32_t N, int32_t n_q, int32_t n_kv) {
     if (B <= 0 || N <= 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv != 0) return 0;
-    return 16;
+    return tree_layout(N, n_q / n_kv).total;
 }
 
 extern "C" int pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params* p, pikv_stream_t stream) {
@@ -224,6 +871,17 @@ extern "C" int pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params*
     PIKV_REQUIRE(((reinterpret_cast<uintptr_t>(p->workspace) | reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->out)) & 15) == 0, PIKV_EINVAL,
                  "tree_attn: q, out and workspace must be 16-byte aligned");
     d.N = p->N; d.n_q = p->n_q; d.G = p->n_q / c->n_kv;
+    const TreeLayout lay = tree_layout(d.N, d.G);
+    PIKV_REQUIRE(p->workspace_bytes >= lay.total, PIKV_EINVAL, "tree_attn: workspace too small (%zu bytes, %zu needed)", p->workspace_bytes, lay.total);
+    const int64_t most = (int64_t)std::min(p->B, PIKV_STREAMS_PER_LAUNCH) * c->n_kv * ceil_div(d.N * d.G, TR_ROWS) * ceil_div(c->max_pages, TR_PAGES);
+    PIKV_REQUIRE(most < (1ll << 31), PIKV_ELIMIT, "tree_attn: streams * heads * pages must stay below 2^33");
+    unsigned char* ws = static_cast<unsigned char*>(p->workspace);
+    TreeParts parts;
+    parts.plan = reinterpret_cast<int*>(ws);
+    parts.ml = reinterpret_cast<float2*>(ws + lay.ml);
+    parts.o = reinterpret_cast<float*>(ws + lay.o);
+    parts.rows = tree_slot_rows(d.N, d.G);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     d.mask_stride = p->mask_per_stream ? p->N * p->N : 0;
     const size_t rows = (size_t)p->N * p->n_q;
     for (int b0 = 0; b0 < p->B; b0 += PIKV_STREAMS_PER_LAUNCH) {
@@ -237,10 +895,16 @@ extern "C" int pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params*
         d.q = static_cast<const __nv_bfloat16*>(p->q) + b0 * rows * 128;
         d.out = static_cast<__nv_bfloat16*>(p->out) + b0 * rows * 128;
         d.lse = p->lse ? p->lse + b0 * rows : nullptr;
-        const int grid = (int)((d.B * rows + TS_THREADS / 32 - 1) / (TS_THREADS / 32));
-        if (c->bits == 8) launch_dependent(tree_attn_simple_kernel<8>, grid, TS_THREADS, 0, static_cast<cudaStream_t>(stream), d);
-        else launch_dependent(tree_attn_simple_kernel<4>, grid, TS_THREADS, 0, static_cast<cudaStream_t>(stream), d);
-        count_launch(1);
+        const int grid = (int)std::min<int64_t>(sm_count() * TR_CTAS, (int64_t)d.B * c->n_kv * ceil_div(d.N * d.G, TR_ROWS) * ceil_div(c->max_pages, TR_PAGES));
+        if (c->bits == 8) {
+            if (!allow_smem<tree_attn_kernel<8>>(TRSmem<8>::BYTES)) return check_launch("tree_attn smem attribute");
+            launch_dependent(tree_attn_kernel<8>, grid, TR_THREADS, TRSmem<8>::BYTES, st, d, parts);
+        } else {
+            if (!allow_smem<tree_attn_kernel<4>>(TRSmem<4>::BYTES)) return check_launch("tree_attn smem attribute");
+            launch_dependent(tree_attn_kernel<4>, grid, TR_THREADS, TRSmem<4>::BYTES, st, d, parts);
+        }
+        launch_dependent(tree_merge_kernel, (int)((d.B * rows + TM_THREADS / 32 - 1) / (TM_THREADS / 32)), TM_THREADS, 0, st, d, parts);
+        count_launch(2);
     }
     return check_launch("tree_attn_kernel");
 }
