@@ -41,12 +41,12 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // units form one list of tiles that a persistent grid cuts into equal runs, two CTAs per SM; a unit that one CTA holds
 // whole is finished there, the pieces of others go to the workspace and a second kernel joins them.
 //
-// A CTA's ten warps:
+// A CTA's warps:
 //   0-3  softmax: thread = row.  S comes out of tensor memory, the weights go back into it as the A operand of the second
 //        product; a row's maximum, denominator and the rescaling of its O live in its thread
-//   4-7  one page of the tile each: codes to f16 (exact integers), into the swizzled layout that both products read
-//   8    bulk copies of pages into a ring, up to TR_STAGES pages ahead
-//   9    issues the MMAs: Q K^T of tile n before P V of tile n - 1, so that the products of one tile run while the softmax
+//   4-7  one page of the tile each: codes from global memory to registers a tile ahead, to f16 (exact integers), into the
+//        swizzled layout that both products read, two tiles of K and of V deep
+//   8    issues the MMAs: Q K^T of tile n + 1 before P V of tile n, so that the products of one tile run while the softmax
 //        of another does
 // Nothing but exact integers enters the tensor cores on the cache side, and the query enters exactly: bf16 times a power of
 // two per row that brings its largest entry to 2^14 is f16 down to 2^-38 of that entry.
@@ -55,7 +55,7 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // R is a row's reference: the largest logit (log2 domain) plus the exponent of the largest vscale seen with it, so that the
 // weights sit at the top of f16's range whatever the size of V; it moves only when a tile exceeds it by 2^TR_SLACK.  The
 // denominator is the fp32 sum of 2^(logit - R).
-constexpr int TR_THREADS = 320;
+constexpr int TR_THREADS = 384;          // three warpgroups: warps 9 to 11 only complete the third
 constexpr int TR_ROWS = 128;             // rows of a unit
 constexpr int TR_KEYS = 64;              // keys of a tile
 constexpr int TR_PAGES = TR_KEYS / PIKV_PAGE_TOKENS;
@@ -63,19 +63,18 @@ constexpr int TR_CTAS = 2;               // per SM
 constexpr int TR_MIN_TILES = 1;          // per CTA
 constexpr float TR_SLACK = 8.f;
 constexpr unsigned TR_WAIT_LIMIT = 1u << 24;
-constexpr uint32_t TR_COL_O = 0, TR_COL_S = 128, TR_COL_P = 192, TR_COLS = 256;
+constexpr uint32_t TR_COL_O = 0, TR_COL_S = 128, TR_COLS = 256;      // S of even and odd tiles, the weights in its first columns
 
-template <int BITS> struct TRGeom;
-template <> struct TRGeom<8> { static constexpr int STAGES = 10, ROW = 128, PAGE = 2048, STAGE = 2 * 2048 + 64, SIDES = 2; };
-template <> struct TRGeom<4> { static constexpr int STAGES = 18, ROW = 64, PAGE = 1024, STAGE = 2 * 1024 + 64 + 128, SIDES = 4; };
+constexpr int TR_TILE = 2 * TR_KEYS * 128;                                     // bytes of a tile of f16: [2 halves of the channels][64 keys][128 bytes]
 
 // shared memory behind a 1024-byte boundary
 template <int BITS> struct TRSmem {
-    static constexpr int Q = 0, K = Q + 2 * TR_ROWS * 128, V = K + 2 * TR_KEYS * 128, RING = V + 2 * TR_KEYS * 128,
-                         SIDE = RING + TRGeom<BITS>::STAGES * TRGeom<BITS>::STAGE,             // [2][SIDES][64] fp32: ks, vs, kz, vz
-                         VEXP = SIDE + 2 * TRGeom<BITS>::SIDES * TR_KEYS * 4,                  // [2][4] exponents
-                         BARS = VEXP + 32, PRE = BARS + (2 * TRGeom<BITS>::STAGES + 17) * 8, MISC = PRE + (PIKV_STREAMS_PER_LAUNCH + 1) * 4,
-                         END = MISC + 16;
+    static constexpr int SIDES = BITS == 8 ? 2 : 4;
+    static constexpr int Q = 0, K = Q + 2 * TR_ROWS * 128, V = K + 2 * TR_TILE,
+                         SIDE = V + 2 * TR_TILE,                               // [4][SIDES][64] fp32: ks, vs, kz, vz of four tiles
+                         VEXP = SIDE + 4 * SIDES * TR_KEYS * 4,                // [4][4] exponents
+                         BARS = VEXP + 64, NBARS = 16,
+                         PRE = BARS + NBARS * 8, MISC = PRE + (PIKV_STREAMS_PER_LAUNCH + 1) * 4, END = MISC + 16;
     static constexpr int BYTES = END + 1024;
 };
 
@@ -91,7 +90,7 @@ __device__ __forceinline__ int tree_row_tiles(int nodes, int G) { return (nodes 
 
 // a place in the list of tiles: stream b, unit (head, 128 rows) of it, tile of the unit
 struct TreeCursor {
-    int b, unit, tile;
+    int b, head, row_tile, tile;
     int tiles, row_tiles;                // of the stream
     int row, ctx, nodes;
     __device__ __forceinline__ void load(const TreeDev& d) {
@@ -102,22 +101,27 @@ struct TreeCursor {
     __device__ __forceinline__ void start(const TreeDev& d, const int* pre, int f) {
         b = stream_of(pre, d.B, f);
         load(d);
-        unit = (f - pre[b]) / tiles;
+        const int unit = (f - pre[b]) / tiles;
         tile = (f - pre[b]) % tiles;
+        head = unit / row_tiles;
+        row_tile = unit % row_tiles;
     }
     __device__ __forceinline__ void next(const TreeDev& d, const int* pre, int f) {      // f: the place after this one
         if (++tile < tiles) return;
         tile = 0;
-        if (++unit < d.c.n_kv * row_tiles) return;
-        unit = 0;
+        if (++row_tile < row_tiles) return;
+        row_tile = 0;
+        if (++head < d.c.n_kv) return;
+        head = 0;
         do ++b; while (pre[b + 1] <= f);
         load(d);
     }
-    __device__ __forceinline__ int head() const { return unit / row_tiles; }
-    __device__ __forceinline__ int row_tile() const { return unit % row_tiles; }
+    __device__ __forceinline__ int end() const { return ctx + nodes; }
+    __device__ __forceinline__ int pages() const { return min(TR_PAGES, (end() + PIKV_PAGE_TOKENS - 1) / PIKV_PAGE_TOKENS - tile * TR_PAGES); }
 };
 
 __device__ __forceinline__ bool tr_wait(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
     for (unsigned i = 0; i < TR_WAIT_LIMIT; ++i) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -125,10 +129,6 @@ __device__ __forceinline__ bool tr_wait(uint32_t bar, uint32_t parity) {
         if (ok) return true;
     }
     return false;
-}
-__device__ __forceinline__ void tr_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 // A from tensor memory (f16, two to a column), B from shared memory
 __device__ __forceinline__ void tr_mma_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
@@ -162,6 +162,11 @@ __device__ __forceinline__ void tr_tmem_st32(uint32_t taddr, const uint32_t* r) 
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
           "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tr_tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                 "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void tr_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tr_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -203,55 +208,127 @@ __device__ __forceinline__ int tr_exponent(uint32_t bits) {
 // position of a channel inside its group of eight in the 4-bit tiles: nibbles leave a word as (0, 4), (1, 5), (2, 6), (3, 7)
 template <int BITS> __device__ __forceinline__ constexpr int tr_channel(int at) { return BITS == 8 ? at : (at & ~7) | ((at & 7) >> 1) | ((at & 1) << 2); }
 
-// 16 codes (8 bit) of a row's chunk, or 16 of a 4-bit row's unit, as f16: eight to each of two 16-byte pieces
+// A page of codes on its way into the 16 rows of a [2 halves][64 keys][128 bytes] tile of f16, in the registers of a warp.
+// Lane l holds, of rows base and base + 8 (base = 2 (l >> 3), with 5 added exclusively for l & 4), the logical chunks l & 3 and
+// (l & 3) + 4 of 16 codes: eight neighbouring lanes then touch eight different 16-byte columns both where the cache's swizzle has
+// put the codes and where the products' swizzle wants them.
+__device__ __forceinline__ int tr_row(int lane) { return (2 * (lane >> 3)) ^ (lane & 4 ? 5 : 0); }
+// byte of a lane's first piece in a page
 template <int BITS>
-__device__ __forceinline__ void tr_codes(const unsigned char* p, uint4& first, uint4& second) {
-    auto bytes = [](uint32_t w, uint32_t sel) {
-        uint32_t x = __byte_perm(w, 0x64646464u, sel);                 // 1024 + (code + 128), exact in f16
-        __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
-        return *reinterpret_cast<uint32_t*>(&h);
-    };
-    auto nibbles = [](uint32_t w) {
-        uint32_t x = (w & 0x000f000fu) | 0x64006400u;                  // 1024 + n, centred: n - 8
-        __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6408)));
-        return *reinterpret_cast<uint32_t*>(&h);
-    };
-    if constexpr (BITS == 8) {
-        const uint4 w = *reinterpret_cast<const uint4*>(p);
-        const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u, c = w.z ^ 0x80808080u, e = w.w ^ 0x80808080u;
-        first = make_uint4(bytes(a, 0x4140), bytes(a, 0x4342), bytes(b, 0x4140), bytes(b, 0x4342));
-        second = make_uint4(bytes(c, 0x4140), bytes(c, 0x4342), bytes(e, 0x4140), bytes(e, 0x4342));
-    } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-        first = make_uint4(nibbles(w.x), nibbles(w.x >> 4), nibbles(w.x >> 8), nibbles(w.x >> 12));
-        second = make_uint4(nibbles(w.y), nibbles(w.y >> 4), nibbles(w.y >> 8), nibbles(w.y >> 12));
-    }
+__device__ __forceinline__ int tr_place(int lane) {
+    const int r = tr_row(lane);
+    return BITS == 8 ? r * 128 + 16 * ((lane & 3) ^ (r & 7)) : r * 64 + 8 * ((lane & 3) ^ (r & 4));
 }
-// one page of codes into its 16 rows of a [2 halves][64 keys][128 bytes] tile, by one warp.  Eight lanes read a row where the
-// cache's swizzle has put it; of the two pieces of a chunk, lanes of the upper half of the channels store the second one first:
-// eight lanes then fill eight different 16-byte columns.
-template <int BITS>
-__device__ __forceinline__ void tr_convert(const unsigned char* raw, unsigned char* tile, int page, int lane) {
-    const int at = lane & 7;
+template <int BITS> struct TRPage {
+    uint32_t w[4][BITS / 2];             // [row + 8][upper half]
+    __device__ __forceinline__ void load(const unsigned char* page, int at) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = 4 * i + (lane >> 3);
-        const int c = BITS == 8 ? at ^ (r & 7) : at ^ (r & 4);         // logical chunk: channels 16 c ..
-        uint4 x, y;
-        tr_codes<BITS>(raw + r * TRGeom<BITS>::ROW + at * (TRGeom<BITS>::ROW / 8), x, y);
-        const bool upper = c >= 4;
-        unsigned char* row = tile + (upper ? TR_KEYS * 128 : 0) + (page * PIKV_PAGE_TOKENS + r) * 128;
-        const int d0 = (2 * (c & 3)) ^ (r & 7), d1 = (2 * (c & 3) + 1) ^ (r & 7);
-        *reinterpret_cast<uint4*>(row + 16 * (upper ? d1 : d0)) = upper ? y : x;
-        *reinterpret_cast<uint4*>(row + 16 * (upper ? d0 : d1)) = upper ? x : y;
+        for (int i = 0; i < 4; ++i) {
+            // the chunk of the upper half: 4 chunks on, exclusively
+            const unsigned char* p = page + ((i & 1) ? at ^ (BITS == 8 ? 64 : 32) : at) + (i >> 1) * 8 * (16 * BITS);
+            if constexpr (BITS == 8) {
+                const uint4 x = ld_stream_16(p);
+                w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
+            } else {
+                const uint2 x = ld_stream_8(p);
+                w[i][0] = x.x; w[i][1] = x.y;
+            }
+        }
     }
-}
+    static __device__ __forceinline__ uint32_t bytes(uint32_t x, uint32_t sel) {
+        x = __byte_perm(x, 0x64646464u, sel);                          // 1024 + (code + 128), exact in f16
+        const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint32_t nibbles(uint32_t x) {
+        x = (x & 0x000f000fu) | 0x64006400u;                           // 1024 + n, centred: n - 8
+        const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6408)));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    __device__ __forceinline__ void store(unsigned char* tile, int page, int lane) const {
+        const int r = tr_row(lane), c = lane & 3;
+        unsigned char* row = tile + (page * PIKV_PAGE_TOKENS + r) * 128;
+        const int d0 = 16 * ((2 * c) ^ (r & 7)), d1 = 16 * ((2 * c + 1) ^ (r & 7));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            unsigned char* to = row + (i & 1) * TR_KEYS * 128 + (i >> 1) * 8 * 128;
+            if constexpr (BITS == 8) {
+                const uint32_t a = w[i][0] ^ 0x80808080u, b = w[i][1] ^ 0x80808080u, e = w[i][2] ^ 0x80808080u, f = w[i][3] ^ 0x80808080u;
+                *reinterpret_cast<uint4*>(to + d0) = make_uint4(bytes(a, 0x4140), bytes(a, 0x4342), bytes(b, 0x4140), bytes(b, 0x4342));
+                *reinterpret_cast<uint4*>(to + d1) = make_uint4(bytes(e, 0x4140), bytes(e, 0x4342), bytes(f, 0x4140), bytes(f, 0x4342));
+            } else {
+                const uint32_t a = w[i][0], b = w[i][1];
+                *reinterpret_cast<uint4*>(to + d0) = make_uint4(nibbles(a), nibbles(a >> 4), nibbles(a >> 8), nibbles(a >> 12));
+                *reinterpret_cast<uint4*>(to + d1) = make_uint4(nibbles(b), nibbles(b >> 4), nibbles(b >> 8), nibbles(b >> 12));
+            }
+        }
+    }
+};
 
+// 32 products of a row with codes to scores, in place (not yet times the query's own factor); returns the largest.  ks: scales,
+// and 2 TR_KEYS behind them the zero points less 8; what `open` has no bit for shows as -infinity
+template <int BITS, bool EDGE>
+__device__ __forceinline__ float tr_scale(float (&x)[32], const float* ks, float qsum, uint32_t open) {
+    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+        const float4 s4 = *reinterpret_cast<const float4*>(ks + j);
+        float2 a = make_float2(x[j], x[j + 1]), c = make_float2(x[j + 2], x[j + 3]);
+        if (BITS == 4) {
+            const float4 z4 = *reinterpret_cast<const float4*>(ks + 2 * TR_KEYS + j);
+            a = tr_fma2(make_float2(z4.x, z4.y), make_float2(-qsum, -qsum), a);
+            c = tr_fma2(make_float2(z4.z, z4.w), make_float2(-qsum, -qsum), c);
+        }
+        a = tr_mul2(a, make_float2(s4.x, s4.y));
+        c = tr_mul2(c, make_float2(s4.z, s4.w));
+        x[j] = a.x; x[j + 1] = a.y; x[j + 2] = c.x; x[j + 3] = c.y;
+        if (EDGE) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!((open >> (j + i)) & 1u)) x[j + i] = -INFINITY;
+        }
+        m0 = fmaxf(m0, fmaxf(x[j], x[j + 1]));
+        m1 = fmaxf(m1, fmaxf(x[j + 2], x[j + 3]));
+    }
+    return fmaxf(m0, m1);
+}
+// 32 scores to weights f16(2^(score qmul + off) vscale), their share of the denominator and (4 bit) of the zero points' sum
+template <int BITS, bool EDGE>
+__device__ __forceinline__ void tr_weights(float (&x)[32], uint32_t (&wgt)[16], const float* vs, float qmul, float off, uint32_t open, float& den, float& corr) {
+    float2 sum = make_float2(0.f, 0.f), zsum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+        const float4 v4 = *reinterpret_cast<const float4*>(vs + j);
+        float2 a = tr_fma2(make_float2(x[j], x[j + 1]), make_float2(qmul, qmul), make_float2(off, off));
+        float2 c = tr_fma2(make_float2(x[j + 2], x[j + 3]), make_float2(qmul, qmul), make_float2(off, off));
+        a = make_float2(tr_ex2(a.x), tr_ex2(a.y));
+        c = make_float2(tr_ex2(c.x), tr_ex2(c.y));
+        sum = tr_add2(sum, tr_add2(a, c));
+        a = tr_mul2(a, make_float2(v4.x, v4.y));
+        c = tr_mul2(c, make_float2(v4.z, v4.w));
+        float4 z4 = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (BITS == 4) z4 = *reinterpret_cast<const float4*>(vs + 2 * TR_KEYS + j);
+        if (EDGE) {                                                      // 0 times something that need not be finite
+            if (!((open >> j) & 1u)) a.x = z4.x = 0.f;
+            if (!((open >> (j + 1)) & 1u)) a.y = z4.y = 0.f;
+            if (!((open >> (j + 2)) & 1u)) c.x = z4.z = 0.f;
+            if (!((open >> (j + 3)) & 1u)) c.y = z4.w = 0.f;
+        }
+        wgt[j / 2] = tr_pack(a.x, a.y);
+        wgt[j / 2 + 1] = tr_pack(c.x, c.y);
+        if (BITS == 4) {
+            const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2]));
+            const float2 rc = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2 + 1]));
+            zsum = tr_fma2(ra, make_float2(z4.x, z4.y), zsum);
+            zsum = tr_fma2(rc, make_float2(z4.z, z4.w), zsum);
+        }
+    }
+    den += sum.x + sum.y;
+    if (BITS == 4) corr += zsum.x + zsum.y;
+}
 template <int BITS>
 __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev d, TreeParts parts) {
-    using GEO = TRGeom<BITS>;
     using SM = TRSmem<BITS>;
-    constexpr int STAGES = GEO::STAGES;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (lr_smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = lr_smem_u32(smem);
@@ -259,26 +336,21 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
     int* pre = reinterpret_cast<int*>(smem + SM::PRE);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::MISC);
     const uint32_t bars = sbase + SM::BARS;
-    const uint32_t raw_full = bars, raw_empty = bars + 8 * STAGES, b0 = bars + 16 * STAGES;
-    const uint32_t k_full = b0, k_empty = b0 + 8, v_full = b0 + 16, v_empty = b0 + 24, s_full = b0 + 32, s_empty = b0 + 40, p_full = b0 + 48,
-                   pv_done = b0 + 64, side_full = b0 + 80, side_empty = b0 + 96, q_full = b0 + 112;
+    const uint32_t k_full = bars, v_full = bars + 16, s_full = bars + 32, p_full = bars + 48, pv_done = bars + 64, side_full = bars + 80, q_full = bars + 112;
     dependency_release();
     if (tid == 0) {
-        for (int i = 0; i < STAGES; ++i) lr_mbar_init(raw_full + 8 * i, 1), lr_mbar_init(raw_empty + 8 * i, 1);
-        lr_mbar_init(k_full, 4); lr_mbar_init(k_empty, 1);
-        lr_mbar_init(v_full, 4); lr_mbar_init(v_empty, 1);
-        lr_mbar_init(s_full, 1); lr_mbar_init(s_empty, 4);
-        lr_mbar_init(q_full, 4);
         for (int i = 0; i < 2; ++i) {
-            lr_mbar_init(p_full + 8 * i, 4); lr_mbar_init(pv_done + 8 * i, 1);
-            lr_mbar_init(side_full + 8 * i, 4); lr_mbar_init(side_empty + 8 * i, 4);
+            lr_mbar_init(k_full + 8 * i, 4); lr_mbar_init(v_full + 8 * i, 4); lr_mbar_init(p_full + 8 * i, 4);
+            lr_mbar_init(s_full + 8 * i, 1); lr_mbar_init(pv_done + 8 * i, 1);
         }
+        for (int i = 0; i < 4; ++i) lr_mbar_init(side_full + 8 * i, 4);
+        lr_mbar_init(q_full, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // keys behind a stream's last page keep what was in the tile: weights of 0 times something finite
-    for (int i = tid; i < 4 * TR_KEYS * 128 / 16; i += TR_THREADS) reinterpret_cast<uint4*>(smem + SM::K)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < 4 * TR_TILE / 16; i += TR_THREADS) reinterpret_cast<uint4*>(smem + SM::K)[i] = make_uint4(0u, 0u, 0u, 0u);
     tr_fence_smem();
-    if (warp == 9) {
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lr_smem_u32(tmem_slot)), "r"(TR_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -300,46 +372,13 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
     const uint32_t tmem = *tmem_slot;
     const int f0 = (int)min((long long)total, (long long)blockIdx.x * per), f1 = min(total, f0 + per);
     bool failed = false;
-
     if (f0 < f1) {
+        // registers go where the scores are: 120 + 72 + 48 of the 3 x 80 a thread that the block was launched with
         TreeCursor cur;
-        cur.start(d, pre, f0);
-        if (warp == 8) {
-            // ---- pages into the ring ----
-            int issued = 0, ids = -1, ids_row = -2, ids_at = 0;
-            for (int f = f0; f < f1 && !failed; ++f) {
-                const int h = cur.head(), p0 = cur.tile * TR_PAGES;
-                const int np = min(TR_PAGES, (cur.ctx + cur.nodes + PIKV_PAGE_TOKENS - 1) / PIKV_PAGE_TOKENS - p0);
-                if (cur.row != ids_row || p0 < ids_at || p0 >= ids_at + 32) {
-                    ids_row = cur.row;
-                    ids_at = p0;
-                    ids = p0 + lane < d.c.max_pages ? __ldg(d.c.page_table + (size_t)cur.row * d.c.max_pages + p0 + lane) : -1;
-                }
-                for (int i = 0; i < np; ++i) {
-                    const int s = issued % STAGES;
-                    int page = __shfl_sync(0xffffffffu, ids, p0 + i - ids_at);
-                    if (page < 0 || page >= d.c.num_pages) {
-                        if (lane == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_PAGE);
-                        page = 0;
-                    }
-                    if (!tr_wait(raw_empty + 8 * s, ((uint32_t)(issued / STAGES) & 1u) ^ 1u)) { failed = true; break; }
-                    const uint32_t bar = raw_full + 8 * s, dst = sbase + SM::RING + s * GEO::STAGE;
-                    if (lane == 0) lr_mbar_expect_tx(bar, GEO::STAGE);
-                    __syncwarp();
-                    const size_t prow = ((size_t)page * d.c.n_kv + h) * PIKV_PAGE_TOKENS;
-                    if (lane == 0) tr_bulk(dst, d.c.k_codes + prow * GEO::ROW, GEO::PAGE, bar);
-                    if (lane == 1) tr_bulk(dst + GEO::PAGE, d.c.v_codes + prow * GEO::ROW, GEO::PAGE, bar);
-                    if (lane == 2) tr_bulk(dst + 2 * GEO::PAGE, d.c.k_scale + prow, 32, bar);
-                    if (lane == 3) tr_bulk(dst + 2 * GEO::PAGE + 32, d.c.v_scale + prow, 32, bar);
-                    if (BITS == 4 && lane == 4) tr_bulk(dst + 2 * GEO::PAGE + 64, d.c.k_zp + prow, 64, bar);
-                    if (BITS == 4 && lane == 5) tr_bulk(dst + 2 * GEO::PAGE + 128, d.c.v_zp + prow, 64, bar);
-                    ++issued;
-                }
-                if (f + 1 < f1) cur.next(d, pre, f + 1);
-            }
-            // a consumer that gave up leaves copies behind: they land before this CTA's shared memory goes to another
-            for (int i = max(0, issued - STAGES); i < issued; ++i) failed |= !tr_wait(raw_full + 8 * (i % STAGES), (uint32_t)(i / STAGES) & 1u);
-        } else if (warp == 9) {
+        if (warp >= 8) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+            if (warp == 8) {
+            cur.start(d, pre, f0);
             // ---- the products ----
             const uint32_t idesc_qk = (1u << 4) | ((uint32_t)(TR_KEYS >> 3) << 17) | ((uint32_t)(TR_ROWS >> 4) << 24);
             const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(TR_ROWS >> 4) << 24);
@@ -347,38 +386,39 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             // V: [64 channels][keys], channels contiguous: 64-channel halves 8192 bytes apart (leading), 8-key groups 1024 (stride)
             const uint32_t v_lo = (((sbase + SM::V) & 0x3FFFFu) >> 4) | ((uint32_t)(TR_KEYS * 128 >> 4) << 16);
             const int count = f1 - f0;
-            int seg = 0;
+            uint32_t seg = 0;
             bool first_before = true;                                // whether tile n - 1 opened its unit here
             auto pv = [&](int m, bool first) {
-                if (!tr_wait(p_full + 8 * (m & 1), (uint32_t)(m >> 1) & 1u) || !tr_wait(v_full, (uint32_t)m & 1u)) return false;
+                const uint32_t b = m & 1, ph = (uint32_t)(m >> 1) & 1u;
+                if (!tr_wait(v_full + 8 * b, ph) || !tr_wait(p_full + 8 * b, ph)) return false;
                 tr_fence_after();
                 if (lr_elect()) {
 #pragma unroll
                     for (int k = 0; k < TR_KEYS / 16; ++k)
-                        tr_mma_ta(tmem + TR_COL_O, tmem + TR_COL_P + 32 * (m & 1) + 8 * k, lr_desc(v_lo + 128 * k), idesc_pv, !first || k ? 1u : 0u);
-                    lr_commit(v_empty);
-                    lr_commit(pv_done + 8 * (m & 1));
+                        tr_mma_ta(tmem + TR_COL_O, tmem + TR_COL_S + TR_KEYS * b + 8 * k, lr_desc(v_lo + (TR_TILE >> 4) * b + 128 * k), idesc_pv, !first || k ? 1u : 0u);
+                    lr_commit(pv_done + 8 * b);
                 }
                 __syncwarp();
                 return true;
             };
-            for (int n = 0; n < count && !failed; ++n) {
+            for (int n = 0; n < count; ++n) {
                 const bool first = n == 0 || cur.tile == 0;
+                const uint32_t b = n & 1;
                 if (first) {
                     // the next unit's Q takes the place of this one's after its last product
                     if (n > 0 && !pv(n - 1, first_before)) { failed = true; break; }
-                    if (!tr_wait(q_full, (uint32_t)seg & 1u)) { failed = true; break; }
+                    if (!tr_wait(q_full, seg & 1u)) { failed = true; break; }
                     ++seg;
                 }
-                if (!tr_wait(k_full, (uint32_t)n & 1u) || !tr_wait(s_empty, ((uint32_t)n & 1u) ^ 1u)) { failed = true; break; }
+                // (S of tile n lies where the weights of tile n - 2 were: their product has been issued before this one)
+                if (!tr_wait(k_full + 8 * b, (uint32_t)(n >> 1) & 1u)) { failed = true; break; }
                 tr_fence_after();
                 if (lr_elect()) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        lr_mma(tmem + TR_COL_S, lr_desc(q_lo + (k >> 2) * (TR_ROWS * 128 >> 4) + 2 * (k & 3)),
-                               lr_desc(k_lo + (k >> 2) * (TR_KEYS * 128 >> 4) + 2 * (k & 3)), idesc_qk, k ? 1u : 0u);
-                    lr_commit(s_full);
-                    lr_commit(k_empty);
+                        lr_mma(tmem + TR_COL_S + TR_KEYS * b, lr_desc(q_lo + (k >> 2) * (TR_ROWS * 128 >> 4) + 2 * (k & 3)),
+                               lr_desc(k_lo + (TR_TILE >> 4) * b + (k >> 2) * (TR_KEYS * 128 >> 4) + 2 * (k & 3)), idesc_qk, k ? 1u : 0u);
+                    lr_commit(s_full + 8 * b);
                 }
                 __syncwarp();
                 if (!first && !pv(n - 1, first_before)) { failed = true; break; }
@@ -388,50 +428,79 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             if (!failed) failed = !pv(count - 1, first_before);
             // nothing of this CTA's is in flight when its tensor memory goes back
             if (!failed) failed = !tr_wait(pv_done + 8 * ((count - 1) & 1), (uint32_t)((count - 1) >> 1) & 1u);
+        }
         } else if (warp >= 4) {
-            // ---- codes to f16 ----
-            const int w = warp - 4;
-            int page0 = 0;                                            // pages of the tiles before this one
-            for (int n = 0, f = f0; f < f1; ++f, ++n) {
-                const int end = cur.ctx + cur.nodes, p0 = cur.tile * TR_PAGES;
-                const int np = min(TR_PAGES, (end + PIKV_PAGE_TOKENS - 1) / PIKV_PAGE_TOKENS - p0);
-                const int i = page0 + w, s = i % STAGES;
-                const unsigned char* raw = smem + SM::RING + s * GEO::STAGE;
-                const bool mine = w < np;
-                if (mine && !tr_wait(raw_full + 8 * s, (uint32_t)(i / STAGES) & 1u)) { failed = true; break; }
-                if (!tr_wait(side_empty + 8 * (n & 1), ((uint32_t)(n >> 1) & 1u) ^ 1u)) { failed = true; break; }
-                {
-                    // lanes 0-15: scales (and zero points) of K, 16-31: of V; rows behind the end have none
-                    const int r = lane & 15, side = lane >> 4;
-                    const bool there = mine && (p0 + w) * PIKV_PAGE_TOKENS + r < end;
-                    const uint32_t bits16 = there ? reinterpret_cast<const uint16_t*>(raw + 2 * GEO::PAGE)[lane] : 0u;
-                    float* to = reinterpret_cast<float*>(smem + SM::SIDE) + (n & 1) * GEO::SIDES * TR_KEYS + side * TR_KEYS + w * PIKV_PAGE_TOKENS + r;
-                    // a key of infinities has a logit that is not a number, whatever the sign of the whole product
-                    *to = side == 0 && (bits16 & 0x7f80u) == 0x7f80u ? __uint_as_float(0x7fffffffu) : __uint_as_float(bits16 << 16);
-                    if (BITS == 4) to[2 * TR_KEYS] = there ? reinterpret_cast<const float*>(raw + 2 * GEO::PAGE + 64)[lane] - 8.f : 0.f;
-                    int e = side ? tr_exponent(bits16 << 16) : -100;
-                    e = __reduce_max_sync(0xffffffffu, e);
-                    if (lane == 0) reinterpret_cast<int*>(smem + SM::VEXP)[(n & 1) * 4 + w] = e;
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+            cur.start(d, pre, f0);
+            // ---- codes to f16: warp w takes page w of every tile ----
+            const int w = warp - 4, count = f1 - f0;
+            const int at = tr_place<BITS>(lane);
+            const int side = lane >> 4;                               // lanes 0-15: scales (and zero points) of K, 16-31: of V
+            const uint16_t* scales = side ? d.c.v_scale : d.c.k_scale;
+            const float* zps = side ? d.c.v_zp : d.c.k_zp;
+            // page numbers of this stream, 32 at a time: eight tiles
+            int ids = -1, ids_row = -2, ids_at = 0;
+            TRPage<BITS> xk, xv;
+            uint32_t scale = 0;
+            float zp = 0.f;
+            bool mine = false;
+            size_t prow = 0;
+            // what this warp needs of the tile at the cursor: page, scales, K
+            auto fetch = [&]() {
+                const int p = cur.tile * TR_PAGES + w;
+                if (cur.row != ids_row || p < ids_at || p >= ids_at + 32) {
+                    ids_row = cur.row;
+                    ids_at = p;
+                    ids = p + lane < d.c.max_pages ? __ldg(d.c.page_table + (size_t)cur.row * d.c.max_pages + p + lane) : -1;
                 }
-                __syncwarp();
-                if (lane == 0) lr_mbar_arrive(side_full + 8 * (n & 1));
-                if (!tr_wait(k_empty, ((uint32_t)n & 1u) ^ 1u)) { failed = true; break; }
-                if (mine) tr_convert<BITS>(raw, smem + SM::K, w, lane);
-                tr_fence_smem();
-                __syncwarp();
-                if (lane == 0) lr_mbar_arrive(k_full);
-                if (!tr_wait(v_empty, ((uint32_t)n & 1u) ^ 1u)) { failed = true; break; }
-                if (mine) tr_convert<BITS>(raw + GEO::PAGE, smem + SM::V, w, lane);
+                mine = w < cur.pages();
+                int page = __shfl_sync(0xffffffffu, ids, p - ids_at);
+                if (mine && (page < 0 || page >= d.c.num_pages)) {
+                    if (lane == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_PAGE);
+                    page = 0;
+                }
+                prow = ((size_t)max(page, 0) * d.c.n_kv + cur.head) * PIKV_PAGE_TOKENS;
+                const bool there = mine && p * PIKV_PAGE_TOKENS + (lane & 15) < cur.end();      // rows behind the end have no scale
+                scale = there ? (uint32_t)__ldg(scales + prow + (lane & 15)) << 16 : 0u;
+                if (BITS == 4) zp = there ? __ldg(zps + prow + (lane & 15)) - 8.f : 0.f;
+                if (mine) xk.load(d.c.k_codes + prow * (16 * BITS), at);
+            };
+            auto fetch_v = [&]() { if (mine) xv.load(d.c.v_codes + prow * (16 * BITS), at); };
+            fetch();
+            fetch_v();
+            for (int m = 0; m < count; ++m) {
+                const uint32_t b = m & 1, ph = ((uint32_t)(m >> 1) & 1u) ^ 1u;
+                const bool now = mine;
+                // Q K^T of tile m - 2 has read this buffer.  The four sets of scales need no wait of their own: the one written here
+                // served tile m - 4, whose second product was issued before that Q K^T
+                if (!tr_wait(s_full + 8 * b, ph)) { failed = true; break; }
+                float* to = reinterpret_cast<float*>(smem + SM::SIDE) + (m & 3) * SM::SIDES * TR_KEYS + side * TR_KEYS + w * PIKV_PAGE_TOKENS + (lane & 15);
+                // a key of infinities has a logit that is not a number, whatever the sign of the whole product
+                *to = side == 0 && (scale & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(scale);
+                if (BITS == 4) to[2 * TR_KEYS] = zp;
+                const int e = __reduce_max_sync(0xffffffffu, side ? tr_exponent(scale) : -100);
+                if (lane == 0) reinterpret_cast<int*>(smem + SM::VEXP)[(m & 3) * 4 + w] = e;
+                if (now) xk.store(smem + SM::K + TR_TILE * b, w, lane);
                 tr_fence_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    lr_mbar_arrive(v_full);
-                    if (mine) lr_mbar_arrive(raw_empty + 8 * s);
+                    lr_mbar_arrive(side_full + 8 * (m & 3));
+                    lr_mbar_arrive(k_full + 8 * b);
                 }
-                page0 += np;
-                if (f + 1 < f1) cur.next(d, pre, f + 1);
+                if (m + 1 < count) {
+                    cur.next(d, pre, f0 + m + 1);
+                    fetch();
+                }
+                if (!tr_wait(pv_done + 8 * b, ph)) { failed = true; break; }             // P V of tile m - 2
+                if (now) xv.store(smem + SM::V + TR_TILE * b, w, lane);
+                tr_fence_smem();
+                __syncwarp();
+                if (lane == 0) lr_mbar_arrive(v_full + 8 * b);
+                if (m + 1 < count) fetch_v();
             }
         } else {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+            cur.start(d, pre, f0);
             // ---- softmax: thread = row ----
             const uint32_t lanes = (uint32_t)(warp * 32) << 16;
             float qmul = 0.f, qsum = 0.f, ref = -INFINITY, den = 0.f, corr = 0.f;
@@ -443,7 +512,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 const bool first = n == 0 || cur.tile == 0;
                 if (first) {
                     // ---- this row's query ----
-                    const int row = cur.row_tile() * TR_ROWS + tid, h = cur.head();
+                    const int row = cur.row_tile * TR_ROWS + tid, h = cur.head;
                     node = row / d.G;
                     live = node < cur.nodes;
                     warp_live = __any_sync(0xffffffffu, live);
@@ -500,54 +569,34 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     __syncwarp();
                     if (lane == 0) lr_mbar_arrive(q_full);
                 }
-                if (!tr_wait(s_full, (uint32_t)n & 1u) || !tr_wait(side_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u)) { failed = true; break; }
+                if (!tr_wait(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u) || !tr_wait(side_full + 8 * (n & 3), (uint32_t)(n >> 2) & 1u)) { failed = true; break; }
                 const bool last = f + 1 == f1 || cur.tile + 1 == cur.tiles;
                 if (warp_live) {
                     tr_fence_after();
-                    float x[TR_KEYS];
-                    tr_tmem_ld32(tmem + lanes + TR_COL_S, x);
-                    tr_tmem_ld32(tmem + lanes + TR_COL_S + 32, x + 32);
-                    tr_tmem_ld_wait(x);
-                    tr_tmem_ld_wait(x + 32);
-                    tr_fence_before();
-                    __syncwarp();
-                    if (lane == 0) lr_mbar_arrive(s_empty);
-                    const float* ks = reinterpret_cast<const float*>(smem + SM::SIDE) + (n & 1) * GEO::SIDES * TR_KEYS;
-                    const float* vs = ks + TR_KEYS;
-                    const float* kz = ks + 2 * TR_KEYS;
-                    const float* vz = ks + 3 * TR_KEYS;
-                    const int4 ve = *reinterpret_cast<const int4*>(smem + SM::VEXP + (n & 1) * 16);
-                    const int pos0 = cur.tile * TR_KEYS;
-                    // scaled scores; the positions behind the context show only where the mask opens them
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < TR_KEYS; j += 4) {
-                        const float4 s4 = *reinterpret_cast<const float4*>(ks + j);
-                        float2 a = make_float2(x[j], x[j + 1]), c = make_float2(x[j + 2], x[j + 3]);
-                        if (BITS == 4) {
-                            const float4 z4 = *reinterpret_cast<const float4*>(kz + j);
-                            a = tr_fma2(make_float2(z4.x, z4.y), make_float2(-qsum, -qsum), a);
-                            c = tr_fma2(make_float2(z4.z, z4.w), make_float2(-qsum, -qsum), c);
-                        }
-                        a = tr_mul2(a, make_float2(s4.x, s4.y));
-                        c = tr_mul2(c, make_float2(s4.z, s4.w));
-                        x[j] = a.x; x[j + 1] = a.y; x[j + 2] = c.x; x[j + 3] = c.y;
-                    }
-                    uint64_t seen = ~0ull;
+                    const uint32_t scores = tmem + lanes + TR_COL_S + TR_KEYS * (n & 1);
+                    const float* ks = reinterpret_cast<const float*>(smem + SM::SIDE) + (n & 3) * SM::SIDES * TR_KEYS;
+                    const int4 ve = *reinterpret_cast<const int4*>(smem + SM::VEXP + (n & 3) * 16);
                     int vexp = max(max(ve.x, ve.y), max(ve.z, ve.w));
+                    const int pos0 = cur.tile * TR_KEYS;
+                    uint64_t seen = ~0ull;
                     const bool edge = pos0 + TR_KEYS > cur.ctx;          // the same for the whole CTA
                     if (edge) {
+                        // the positions behind the context show only where the mask opens them
                         const int sh = cur.ctx - pos0;                   // the tree's first bit
                         seen = sh >= 0 ? (sh < 64 ? tree << sh : 0ull) | ((1ull << sh) - 1) : (sh > -64 ? tree >> -sh : 0ull);
                         vexp = -100;                                     // of the rows that this one sees
-#pragma unroll
-                        for (int j = 0; j < TR_KEYS; ++j) {
-                            if ((seen >> j) & 1) vexp = max(vexp, tr_exponent(__float_as_uint(vs[j])));
-                            else x[j] = -INFINITY;
-                        }
+#pragma unroll 4
+                        for (int j = 0; j < TR_KEYS; ++j)
+                            if ((seen >> j) & 1) vexp = max(vexp, tr_exponent(__float_as_uint(ks[TR_KEYS + j])));
                     }
-#pragma unroll
-                    for (int j = 0; j < TR_KEYS; ++j) mx = fmaxf(mx, x[j]);
+                    float x0[32], x1[32];
+                    tr_tmem_ld32(scores, x0);
+                    tr_tmem_ld32(scores + 32, x1);
+                    tr_tmem_ld_wait(x0);
+                    tr_tmem_ld_wait(x1);
+                    float mx;
+                    if (edge) mx = fmaxf(tr_scale<BITS, true>(x0, ks, qsum, (uint32_t)seen), tr_scale<BITS, true>(x1, ks + 32, qsum, (uint32_t)(seen >> 32)));
+                    else mx = fmaxf(tr_scale<BITS, false>(x0, ks, qsum, ~0u), tr_scale<BITS, false>(x1, ks + 32, qsum, ~0u));
                     // does the reference hold?  (-inf while nothing has been seen)
                     const float want = mx * qmul + (float)vexp;
                     const bool move = mx > -INFINITY && want > ref + TR_SLACK;
@@ -561,64 +610,36 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                             if (!tr_wait(pv_done + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u)) { failed = true; break; }
                             tr_fence_after();
 #pragma unroll 1
-                            for (int c = 0; c < 128; c += 32) {
-                                float o[32];
-                                tr_tmem_ld32(tmem + lanes + TR_COL_O + c, o);
-                                tr_tmem_ld_wait(o);
-                                uint32_t r[32];
+                            for (int c = 0; c < 128; c += 16) {             // few registers: the scores are in the others
+                                float o[16];
+                                lr_tmem_ld16(tmem + lanes + TR_COL_O + c, o);
+                                uint32_t r[16];
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(o[i] * fac);
-                                tr_tmem_st32(tmem + lanes + TR_COL_O + c, r);
+                                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(o[i] * fac);
+                                tr_tmem_st16(tmem + lanes + TR_COL_O + c, r);
                             }
                             tr_tmem_st_wait();
                         }
                     }
                     const float off = ref == -INFINITY ? 0.f : -ref;
-                    float2 sum = make_float2(0.f, 0.f);
-                    uint32_t wgt[TR_KEYS / 2];
-#pragma unroll
-                    for (int j = 0; j < TR_KEYS; j += 4) {
-                        const float4 v4 = *reinterpret_cast<const float4*>(vs + j);
-                        float2 a = tr_fma2(make_float2(x[j], x[j + 1]), make_float2(qmul, qmul), make_float2(off, off));
-                        float2 c = tr_fma2(make_float2(x[j + 2], x[j + 3]), make_float2(qmul, qmul), make_float2(off, off));
-                        a = make_float2(tr_ex2(a.x), tr_ex2(a.y));
-                        c = make_float2(tr_ex2(c.x), tr_ex2(c.y));
-                        sum = tr_add2(sum, tr_add2(a, c));
-                        a = tr_mul2(a, make_float2(v4.x, v4.y));
-                        c = tr_mul2(c, make_float2(v4.z, v4.w));
-                        if (edge) {                                      // 0 times a scale that is not finite
-                            if (!((seen >> j) & 1)) a.x = 0.f;
-                            if (!((seen >> (j + 1)) & 1)) a.y = 0.f;
-                            if (!((seen >> (j + 2)) & 1)) c.x = 0.f;
-                            if (!((seen >> (j + 3)) & 1)) c.y = 0.f;
-                        }
-                        wgt[j / 2] = tr_pack(a.x, a.y);
-                        wgt[j / 2 + 1] = tr_pack(c.x, c.y);
-                        if (BITS == 4) {
-                            const float4 z4 = *reinterpret_cast<const float4*>(vz + j);
-                            const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2]));
-                            const float2 rc = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2 + 1]));
-                            if (edge) {
-                                corr += (ra.x ? ra.x * z4.x : 0.f) + (ra.y ? ra.y * z4.y : 0.f) + (rc.x ? rc.x * z4.z : 0.f) + (rc.y ? rc.y * z4.w : 0.f);
-                            } else {
-                                const float2 t = tr_fma2(ra, make_float2(z4.x, z4.y), tr_mul2(rc, make_float2(z4.z, z4.w)));
-                                corr += t.x + t.y;
-                            }
-                        }
+                    // the weights take the place of the scores that they come from, two to a column
+                    {
+                        uint32_t wgt[16];
+                        if (edge) tr_weights<BITS, true>(x0, wgt, ks + TR_KEYS, qmul, off, (uint32_t)seen, den, corr);
+                        else tr_weights<BITS, false>(x0, wgt, ks + TR_KEYS, qmul, off, ~0u, den, corr);
+                        tr_tmem_st16(scores, wgt);
                     }
-                    den += sum.x + sum.y;
-                    __syncwarp();
-                    if (lane == 0) lr_mbar_arrive(side_empty + 8 * (n & 1));
-                    if (n >= 2 && !tr_wait(pv_done + 8 * (n & 1), (uint32_t)((n - 2) >> 1) & 1u)) { failed = true; break; }
-                    tr_fence_after();
-                    tr_tmem_st32(tmem + lanes + TR_COL_P + 32 * (n & 1), wgt);
+                    {
+                        uint32_t wgt[16];
+                        if (edge) tr_weights<BITS, true>(x1, wgt, ks + TR_KEYS + 32, qmul, off, (uint32_t)(seen >> 32), den, corr);
+                        else tr_weights<BITS, false>(x1, wgt, ks + TR_KEYS + 32, qmul, off, ~0u, den, corr);
+                        tr_tmem_st16(scores + 16, wgt);
+                    }
                     tr_tmem_st_wait();
                     tr_fence_before();
                     __syncwarp();
                     if (lane == 0) lr_mbar_arrive(p_full + 8 * (n & 1));
                 } else if (lane == 0) {
-                    lr_mbar_arrive(s_empty);
-                    lr_mbar_arrive(side_empty + 8 * (n & 1));
                     lr_mbar_arrive(p_full + 8 * (n & 1));
                 }
                 if (last) {
@@ -673,7 +694,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
     }
     tr_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 8) {
         tr_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TR_COLS) : "memory");
     }
