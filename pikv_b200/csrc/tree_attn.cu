@@ -44,18 +44,23 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // A CTA's warps:
 //   0-3  softmax: thread = row.  S comes out of tensor memory, the weights go back into it as the A operand of the second
 //        product; a row's maximum, denominator and the rescaling of its O live in its thread
-//   4-7  one page of the tile each: codes from global memory to registers a tile ahead, to f16 (exact integers), into the
-//        swizzled layout that both products read, two tiles of K and of V deep
+//   4-7  one page of every tile each: codes to f16 (exact integers), into the swizzled layout that both products read
 //   8    issues the MMAs: Q K^T of tile n + 1 before P V of tile n, so that the products of one tile run while the softmax
 //        of another does
-// Nothing but exact integers enters the tensor cores on the cache side, and the query enters exactly: bf16 times a power of
-// two per row that brings its largest entry to 2^14 is f16 down to 2^-38 of that entry.
-//   logit = kscale (q . code - zp sum(q))        (zp = 0 for the 8-bit cache)
-//   O     = sum w code - sum w zp,  w = f16(2^(logit - R) vscale)
-// R is a row's reference: the largest logit (log2 domain) plus the exponent of the largest vscale seen with it, so that the
-// weights sit at the top of f16's range whatever the size of V; it moves only when a tile exceeds it by 2^TR_SLACK.  The
-// denominator is the fp32 sum of 2^(logit - R).
-constexpr int TR_THREADS = 384;          // three warpgroups: warps 9 to 11 only complete the third
+//   9    bulk copies of pages into two rings, K three tiles ahead and V two
+// The query enters exactly: bf16 times a power of two per row that brings its largest entry to 2^14 is f16 down to 2^-38 of
+// that entry.  Keys and values enter as f16 of code * scale, in units of a power of two per tile (2^(e - 9), 2^e above the tile's
+// largest scale): one rounding, 2^-11 of the entry, the size of the weights' own; in return the softmax neither loads nor
+// multiplies by the scales (shared-memory reads of the scales by every row were the busiest pipe of the kernel that applied
+// them to exact integer products: 58 % busy, 248 us for 16 x 16384 x 32 nodes against XXX).
+//   logit = 2^(e_k + 9) / sqrt(128) (q . K16 - z)      z: the zero points' part, (zp - 8) scale sum(q), 4 bit only
+//   O     = sum w V16 - sum w z_v,  w = f16(2^(logit - R + e_v + 9))
+// R is a row's reference: the largest logit (log2 domain) plus e_v + 9 of the tile it was seen in, so that the weights sit at
+// the top of f16's range whatever the size of V; it moves only when a tile exceeds it by 2^TR_SLACK.  The denominator is
+// the fp32 sum of 2^(logit - R).  A row of V that is not finite enters as zeros and makes the result of the rows that see it
+// not a number; one that a row does not see does not reach it.
+constexpr int TR_THREADS = 384;          // three warpgroups: warps 10 and 11 only complete the last
+constexpr int TR_CONVERT = 4, TR_MMA = 8, TR_COPY = 9;      // first converting warp, and the two single ones
 constexpr int TR_ROWS = 128;             // rows of a unit
 constexpr int TR_KEYS = 64;              // keys of a tile
 constexpr int TR_PAGES = TR_KEYS / PIKV_PAGE_TOKENS;
@@ -66,14 +71,19 @@ constexpr unsigned TR_WAIT_LIMIT = 1u << 24;
 constexpr uint32_t TR_COL_O = 0, TR_COL_S = 128, TR_COLS = 256;      // S of even and odd tiles, the weights in its first columns
 
 constexpr int TR_TILE = 2 * TR_KEYS * 128;                                     // bytes of a tile of f16: [2 halves of the channels][64 keys][128 bytes]
+constexpr int TR_K_AHEAD = 3, TR_V_AHEAD = 2;                                   // tiles whose copies are on their way
 
 // shared memory behind a 1024-byte boundary
 template <int BITS> struct TRSmem {
-    static constexpr int SIDES = BITS == 8 ? 2 : 4;
-    static constexpr int Q = 0, K = Q + 2 * TR_ROWS * 128, V = K + 2 * TR_TILE,
-                         SIDE = V + 2 * TR_TILE,                               // [4][SIDES][64] fp32: ks, vs, kz, vz of four tiles
-                         VEXP = SIDE + 4 * SIDES * TR_KEYS * 4,                // [4][4] exponents
-                         BARS = VEXP + 64, NBARS = 16,
+    static constexpr int SIDES = BITS == 8 ? 0 : 2;
+    static constexpr int PAGE = 256 * BITS, META = BITS == 8 ? 64 : 192;       // codes of a page of one head; scales (and zero points) of K and V
+    static constexpr int Q = 0, K = Q + 2 * TR_ROWS * 128, V = K + TR_TILE,
+                         KRING = V + TR_TILE,                                  // [ahead][page of the tile] codes of K
+                         VRING = KRING + TR_K_AHEAD * TR_PAGES * PAGE,
+                         MRING = VRING + TR_V_AHEAD * TR_PAGES * PAGE,         // [ahead of K][page] scales, zero points
+                         SIDE = MRING + TR_K_AHEAD * TR_PAGES * META,          // 4 bit: [4][2][64] fp32: z of K, of V, of four tiles
+                         VEXP = SIDE + 4 * SIDES * TR_KEYS * 4,                // [4] of four tiles: e_k + 9, e_v + 9, rows of V that are not finite (a bit each)
+                         BARS = VEXP + 64, NBARS = 14 + 2 * (TR_K_AHEAD + TR_V_AHEAD),
                          PRE = BARS + NBARS * 8, MISC = PRE + (PIKV_STREAMS_PER_LAUNCH + 1) * 4, END = MISC + 16;
     static constexpr int BYTES = END + 1024;
 };
@@ -219,69 +229,85 @@ __device__ __forceinline__ int tr_place(int lane) {
     const int r = tr_row(lane);
     return BITS == 8 ? r * 128 + 16 * ((lane & 3) ^ (r & 7)) : r * 64 + 8 * ((lane & 3) ^ (r & 4));
 }
+// two phases of which both are wanted: their polls overlap
+__device__ __forceinline__ bool tr_wait2(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1) {
+#pragma unroll 1
+    for (unsigned i = 0; i < TR_WAIT_LIMIT; ++i) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p, q;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tmbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+                     "and.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void tr_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 template <int BITS> struct TRPage {
-    uint32_t w[4][BITS / 2];             // [row + 8][upper half]
+    uint32_t w[4][BITS / 2];
     __device__ __forceinline__ void load(const unsigned char* page, int at) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             // the chunk of the upper half: 4 chunks on, exclusively
-            const unsigned char* p = page + ((i & 1) ? at ^ (BITS == 8 ? 64 : 32) : at) + (i >> 1) * 8 * (16 * BITS);
+            const unsigned char* p = page + ((i & 1) ? at ^ (8 * BITS) : at) + (i >> 1) * 8 * (16 * BITS);
             if constexpr (BITS == 8) {
-                const uint4 x = ld_stream_16(p);
+                const uint4 x = *reinterpret_cast<const uint4*>(p);
                 w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
             } else {
-                const uint2 x = ld_stream_8(p);
+                const uint2 x = *reinterpret_cast<const uint2*>(p);
                 w[i][0] = x.x; w[i][1] = x.y;
             }
         }
     }
-    static __device__ __forceinline__ uint32_t bytes(uint32_t x, uint32_t sel) {
-        x = __byte_perm(x, 0x64646464u, sel);                          // 1024 + (code + 128), exact in f16
-        const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+    // A byte or nibble n in the low bits of an f16 is n 2^-24, exactly (a subnormal).  With a = scale 2^(15 - e) and b the offset's
+    // part, the fused a n 2^-24 + b is (n - offset) scale 2^(-9 - e), rounded once.
+    static __device__ __forceinline__ uint32_t fma2(uint32_t x, __half2 a, __half2 b) {
+        const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
-    static __device__ __forceinline__ uint32_t nibbles(uint32_t x) {
-        x = (x & 0x000f000fu) | 0x64006400u;                           // 1024 + n, centred: n - 8
-        const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6408)));
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    __device__ __forceinline__ void store(unsigned char* tile, int page, int lane) const {
+    // a0, a1: of rows base and base + 8
+    __device__ __forceinline__ void store(unsigned char* tile, int page, int lane, float a0, float a1) const {
         const int r = tr_row(lane), c = lane & 3;
         unsigned char* row = tile + (page * PIKV_PAGE_TOKENS + r) * 128;
         const int d0 = 16 * ((2 * c) ^ (r & 7)), d1 = 16 * ((2 * c + 1) ^ (r & 7));
+        constexpr float OFFSET = (BITS == 8 ? -128.f : -8.f) / 16777216.f;
+        const __half2 a[2] = {__float2half2_rn(a0), __float2half2_rn(a1)}, b[2] = {__float2half2_rn(a0 * OFFSET), __float2half2_rn(a1 * OFFSET)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             unsigned char* to = row + (i & 1) * TR_KEYS * 128 + (i >> 1) * 8 * 128;
+            const __half2 s = a[i >> 1], o = b[i >> 1];
             if constexpr (BITS == 8) {
-                const uint32_t a = w[i][0] ^ 0x80808080u, b = w[i][1] ^ 0x80808080u, e = w[i][2] ^ 0x80808080u, f = w[i][3] ^ 0x80808080u;
-                *reinterpret_cast<uint4*>(to + d0) = make_uint4(bytes(a, 0x4140), bytes(a, 0x4342), bytes(b, 0x4140), bytes(b, 0x4342));
-                *reinterpret_cast<uint4*>(to + d1) = make_uint4(bytes(e, 0x4140), bytes(e, 0x4342), bytes(f, 0x4140), bytes(f, 0x4342));
+                uint32_t x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = w[i][k] ^ 0x80808080u;             // code + 128
+                auto pair = [&](int k, uint32_t sel) { return fma2(__byte_perm(x[k], 0u, sel), s, o); };
+                *reinterpret_cast<uint4*>(to + d0) = make_uint4(pair(0, 0x4140), pair(0, 0x4342), pair(1, 0x4140), pair(1, 0x4342));
+                *reinterpret_cast<uint4*>(to + d1) = make_uint4(pair(2, 0x4140), pair(2, 0x4342), pair(3, 0x4140), pair(3, 0x4342));
             } else {
-                const uint32_t a = w[i][0], b = w[i][1];
-                *reinterpret_cast<uint4*>(to + d0) = make_uint4(nibbles(a), nibbles(a >> 4), nibbles(a >> 8), nibbles(a >> 12));
-                *reinterpret_cast<uint4*>(to + d1) = make_uint4(nibbles(b), nibbles(b >> 4), nibbles(b >> 8), nibbles(b >> 12));
+                auto pair = [&](uint32_t x) { return fma2(x & 0x000f000fu, s, o); };
+                const uint32_t x = w[i][0], y = w[i][1];
+                *reinterpret_cast<uint4*>(to + d0) = make_uint4(pair(x), pair(x >> 4), pair(x >> 8), pair(x >> 12));
+                *reinterpret_cast<uint4*>(to + d1) = make_uint4(pair(y), pair(y >> 4), pair(y >> 8), pair(y >> 12));
             }
         }
     }
 };
 
-// 32 products of a row with codes to scores, in place (not yet times the query's own factor); returns the largest.  ks: scales,
-// and 2 TR_KEYS behind them the zero points less 8; what `open` has no bit for shows as -infinity
+// 32 products of a row to scores, in place: the zero points' part off (4 bit), what `open` has no bit for to -infinity; returns the
+// largest.  kz: z of K of these keys
 template <int BITS, bool EDGE>
-__device__ __forceinline__ float tr_scale(float (&x)[32], const float* ks, float qsum, uint32_t open) {
+__device__ __forceinline__ float tr_scores(float (&x)[32], const float* kz, float qsum, uint32_t open) {
     float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-        const float4 s4 = *reinterpret_cast<const float4*>(ks + j);
-        float2 a = make_float2(x[j], x[j + 1]), c = make_float2(x[j + 2], x[j + 3]);
         if (BITS == 4) {
-            const float4 z4 = *reinterpret_cast<const float4*>(ks + 2 * TR_KEYS + j);
-            a = tr_fma2(make_float2(z4.x, z4.y), make_float2(-qsum, -qsum), a);
-            c = tr_fma2(make_float2(z4.z, z4.w), make_float2(-qsum, -qsum), c);
+            const float4 z4 = *reinterpret_cast<const float4*>(kz + j);
+            const float2 a = tr_fma2(make_float2(z4.x, z4.y), make_float2(-qsum, -qsum), make_float2(x[j], x[j + 1]));
+            const float2 c = tr_fma2(make_float2(z4.z, z4.w), make_float2(-qsum, -qsum), make_float2(x[j + 2], x[j + 3]));
+            x[j] = a.x; x[j + 1] = a.y; x[j + 2] = c.x; x[j + 3] = c.y;
         }
-        a = tr_mul2(a, make_float2(s4.x, s4.y));
-        c = tr_mul2(c, make_float2(s4.z, s4.w));
-        x[j] = a.x; x[j + 1] = a.y; x[j + 2] = c.x; x[j + 3] = c.y;
         if (EDGE) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -292,40 +318,39 @@ __device__ __forceinline__ float tr_scale(float (&x)[32], const float* ks, float
     }
     return fmaxf(m0, m1);
 }
-// 32 scores to weights f16(2^(score qmul + off) vscale), their share of the denominator and (4 bit) of the zero points' sum
+// 32 scores to weights f16(2^(score mul + off)), their sum and (4 bit) the sum of their zero points' parts; vz: z of V
 template <int BITS, bool EDGE>
-__device__ __forceinline__ void tr_weights(float (&x)[32], uint32_t (&wgt)[16], const float* vs, float qmul, float off, uint32_t open, float& den, float& corr) {
-    float2 sum = make_float2(0.f, 0.f), zsum = make_float2(0.f, 0.f);
+__device__ __forceinline__ void tr_weights(const float (&x)[32], uint32_t (&wgt)[16], const float* vz, float mul, float off, uint32_t open, float& total, float& corr) {
+    float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f), zsum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-        const float4 v4 = *reinterpret_cast<const float4*>(vs + j);
-        float2 a = tr_fma2(make_float2(x[j], x[j + 1]), make_float2(qmul, qmul), make_float2(off, off));
-        float2 c = tr_fma2(make_float2(x[j + 2], x[j + 3]), make_float2(qmul, qmul), make_float2(off, off));
+        float2 a = tr_fma2(make_float2(x[j], x[j + 1]), make_float2(mul, mul), make_float2(off, off));
+        float2 c = tr_fma2(make_float2(x[j + 2], x[j + 3]), make_float2(mul, mul), make_float2(off, off));
         a = make_float2(tr_ex2(a.x), tr_ex2(a.y));
         c = make_float2(tr_ex2(c.x), tr_ex2(c.y));
-        sum = tr_add2(sum, tr_add2(a, c));
-        a = tr_mul2(a, make_float2(v4.x, v4.y));
-        c = tr_mul2(c, make_float2(v4.z, v4.w));
-        float4 z4 = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (BITS == 4) z4 = *reinterpret_cast<const float4*>(vs + 2 * TR_KEYS + j);
-        if (EDGE) {                                                      // 0 times something that need not be finite
-            if (!((open >> j) & 1u)) a.x = z4.x = 0.f;
-            if (!((open >> (j + 1)) & 1u)) a.y = z4.y = 0.f;
-            if (!((open >> (j + 2)) & 1u)) c.x = z4.z = 0.f;
-            if (!((open >> (j + 3)) & 1u)) c.y = z4.w = 0.f;
-        }
+        s0 = tr_add2(s0, a);
+        s1 = tr_add2(s1, c);
         wgt[j / 2] = tr_pack(a.x, a.y);
         wgt[j / 2 + 1] = tr_pack(c.x, c.y);
         if (BITS == 4) {
+            float4 z4 = *reinterpret_cast<const float4*>(vz + j);
+            if (EDGE) {                                                  // 0 times something that need not be finite
+                if (!((open >> j) & 1u)) z4.x = 0.f;
+                if (!((open >> (j + 1)) & 1u)) z4.y = 0.f;
+                if (!((open >> (j + 2)) & 1u)) z4.z = 0.f;
+                if (!((open >> (j + 3)) & 1u)) z4.w = 0.f;
+            }
             const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2]));
             const float2 rc = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2 + 1]));
             zsum = tr_fma2(ra, make_float2(z4.x, z4.y), zsum);
             zsum = tr_fma2(rc, make_float2(z4.z, z4.w), zsum);
         }
     }
-    den += sum.x + sum.y;
+    s0 = tr_add2(s0, s1);
+    total += s0.x + s0.y;
     if (BITS == 4) corr += zsum.x + zsum.y;
 }
+
 template <int BITS>
 __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev d, TreeParts parts) {
     using SM = TRSmem<BITS>;
@@ -336,21 +361,23 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
     int* pre = reinterpret_cast<int*>(smem + SM::PRE);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::MISC);
     const uint32_t bars = sbase + SM::BARS;
-    const uint32_t k_full = bars, v_full = bars + 16, s_full = bars + 32, p_full = bars + 48, pv_done = bars + 64, side_full = bars + 80, q_full = bars + 112;
+    const uint32_t k_full = bars, v_full = bars + 8, q_full = bars + 16, s_full = bars + 24, p_full = bars + 40, pv_done = bars + 56, side_full = bars + 72,
+                   kr_full = bars + 112, kr_empty = kr_full + 8 * TR_K_AHEAD, vr_full = kr_empty + 8 * TR_K_AHEAD, vr_empty = vr_full + 8 * TR_V_AHEAD;
     dependency_release();
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            lr_mbar_init(k_full + 8 * i, 4); lr_mbar_init(v_full + 8 * i, 4); lr_mbar_init(p_full + 8 * i, 4);
-            lr_mbar_init(s_full + 8 * i, 1); lr_mbar_init(pv_done + 8 * i, 1);
-        }
-        for (int i = 0; i < 4; ++i) lr_mbar_init(side_full + 8 * i, 4);
+        lr_mbar_init(k_full, 4);
+        lr_mbar_init(v_full, 4);
         lr_mbar_init(q_full, 4);
+        for (int i = 0; i < 2; ++i) lr_mbar_init(s_full + 8 * i, 1), lr_mbar_init(p_full + 8 * i, 4), lr_mbar_init(pv_done + 8 * i, 1);
+        for (int i = 0; i < 4; ++i) lr_mbar_init(side_full + 8 * i, 4);
+        for (int i = 0; i < TR_K_AHEAD; ++i) lr_mbar_init(kr_full + 8 * i, 1), lr_mbar_init(kr_empty + 8 * i, 4);
+        for (int i = 0; i < TR_V_AHEAD; ++i) lr_mbar_init(vr_full + 8 * i, 1), lr_mbar_init(vr_empty + 8 * i, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // keys behind a stream's last page keep what was in the tile: weights of 0 times something finite
-    for (int i = tid; i < 4 * TR_TILE / 16; i += TR_THREADS) reinterpret_cast<uint4*>(smem + SM::K)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < 2 * TR_TILE / 16; i += TR_THREADS) reinterpret_cast<uint4*>(smem + SM::K)[i] = make_uint4(0u, 0u, 0u, 0u);
     tr_fence_smem();
-    if (warp == 8) {
+    if (warp == TR_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lr_smem_u32(tmem_slot)), "r"(TR_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -375,9 +402,9 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
     if (f0 < f1) {
         // registers go where the scores are: 120 + 72 + 48 of the 3 x 80 a thread that the block was launched with
         TreeCursor cur;
-        if (warp >= 8) {
+        if (warp >= TR_MMA) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-            if (warp == 8) {
+            if (warp == TR_MMA) {
             cur.start(d, pre, f0);
             // ---- the products ----
             const uint32_t idesc_qk = (1u << 4) | ((uint32_t)(TR_KEYS >> 3) << 17) | ((uint32_t)(TR_ROWS >> 4) << 24);
@@ -390,12 +417,12 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             bool first_before = true;                                // whether tile n - 1 opened its unit here
             auto pv = [&](int m, bool first) {
                 const uint32_t b = m & 1, ph = (uint32_t)(m >> 1) & 1u;
-                if (!tr_wait(v_full + 8 * b, ph) || !tr_wait(p_full + 8 * b, ph)) return false;
+                if (!tr_wait2(v_full, b, p_full + 8 * b, ph)) return false;
                 tr_fence_after();
                 if (lr_elect()) {
 #pragma unroll
                     for (int k = 0; k < TR_KEYS / 16; ++k)
-                        tr_mma_ta(tmem + TR_COL_O, tmem + TR_COL_S + TR_KEYS * b + 8 * k, lr_desc(v_lo + (TR_TILE >> 4) * b + 128 * k), idesc_pv, !first || k ? 1u : 0u);
+                        tr_mma_ta(tmem + TR_COL_O, tmem + TR_COL_S + TR_KEYS * b + 8 * k, lr_desc(v_lo + 128 * k), idesc_pv, !first || k ? 1u : 0u);
                     lr_commit(pv_done + 8 * b);
                 }
                 __syncwarp();
@@ -411,13 +438,13 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     ++seg;
                 }
                 // (S of tile n lies where the weights of tile n - 2 were: their product has been issued before this one)
-                if (!tr_wait(k_full + 8 * b, (uint32_t)(n >> 1) & 1u)) { failed = true; break; }
+                if (!tr_wait(k_full, b)) { failed = true; break; }
                 tr_fence_after();
                 if (lr_elect()) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         lr_mma(tmem + TR_COL_S + TR_KEYS * b, lr_desc(q_lo + (k >> 2) * (TR_ROWS * 128 >> 4) + 2 * (k & 3)),
-                               lr_desc(k_lo + (TR_TILE >> 4) * b + (k >> 2) * (TR_KEYS * 128 >> 4) + 2 * (k & 3)), idesc_qk, k ? 1u : 0u);
+                               lr_desc(k_lo + (k >> 2) * (TR_KEYS * 128 >> 4) + 2 * (k & 3)), idesc_qk, k ? 1u : 0u);
                     lr_commit(s_full + 8 * b);
                 }
                 __syncwarp();
@@ -428,75 +455,131 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             if (!failed) failed = !pv(count - 1, first_before);
             // nothing of this CTA's is in flight when its tensor memory goes back
             if (!failed) failed = !tr_wait(pv_done + 8 * ((count - 1) & 1), (uint32_t)((count - 1) >> 1) & 1u);
-        }
-        } else if (warp >= 4) {
+            } else if (warp == TR_COPY) {
+                // ---- pages into the rings: lanes 0-3 the K and the scales of a tile's pages, lanes 4-7 the V of the tile before ----
+                cur.start(d, pre, f0);
+                const int count = f1 - f0, i = lane & 3;
+                int ids = -1, ids_row = -2, ids_at = 0;              // page numbers of this stream, 32 at a time: eight tiles
+                int ks = 0, vs = 0, np = 0;                          // stages; pages of the tile whose K went last
+                uint32_t kph = 1, vph = 1, unit = 0;                 // unit: place of page i in the pools
+                for (int n = 0; n <= count; ++n) {
+                    const uint32_t v_unit = unit;
+                    const int v_np = np;
+                    if (n < count) {
+                        const int p = cur.tile * TR_PAGES;
+                        np = cur.pages();
+                        if (cur.row != ids_row || p < ids_at || p >= ids_at + 32) {
+                            ids_row = cur.row;
+                            ids_at = p;
+                            ids = p + lane < d.c.max_pages ? __ldg(d.c.page_table + (size_t)cur.row * d.c.max_pages + p + lane) : -1;
+                        }
+                        int page = __shfl_sync(0xffffffffu, ids, (p + i - ids_at) & 31);
+                        if (i < np && (page < 0 || page >= d.c.num_pages)) {
+                            if (lane < 4 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_PAGE);
+                            page = 0;
+                        }
+                        unit = (uint32_t)page * (uint32_t)d.c.n_kv + (uint32_t)cur.head;
+                        if (!tr_wait(kr_empty + 8 * ks, kph)) { failed = true; break; }
+                        const uint32_t bar = kr_full + 8 * ks;
+                        if (lane == 0) lr_mbar_expect_tx(bar, (uint32_t)np * (SM::PAGE + SM::META));
+                        __syncwarp();
+                        if (lane < np) {
+                            const uint32_t dst = sbase + SM::MRING + (ks * TR_PAGES + i) * SM::META;
+                            tr_bulk(sbase + SM::KRING + (ks * TR_PAGES + i) * SM::PAGE, d.c.k_codes + (size_t)unit * SM::PAGE, SM::PAGE, bar);
+                            tr_bulk(dst, d.c.k_scale + (size_t)unit * 16, 32, bar);
+                            tr_bulk(dst + 32, d.c.v_scale + (size_t)unit * 16, 32, bar);
+                            if (BITS == 4) {
+                                tr_bulk(dst + 64, d.c.k_zp + (size_t)unit * 16, 64, bar);
+                                tr_bulk(dst + 128, d.c.v_zp + (size_t)unit * 16, 64, bar);
+                            }
+                        }
+                        if (++ks == TR_K_AHEAD) ks = 0, kph ^= 1u;
+                        if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
+                    }
+                    if (n == 0) continue;
+                    if (!tr_wait(vr_empty + 8 * vs, vph)) { failed = true; break; }
+                    if (lane == 4) lr_mbar_expect_tx(vr_full + 8 * vs, (uint32_t)v_np * SM::PAGE);
+                    __syncwarp();
+                    if (lane >= 4 && lane < 4 + v_np)
+                        tr_bulk(sbase + SM::VRING + (vs * TR_PAGES + i) * SM::PAGE, d.c.v_codes + (size_t)v_unit * SM::PAGE, SM::PAGE, vr_full + 8 * vs);
+                    if (++vs == TR_V_AHEAD) vs = 0, vph ^= 1u;
+                }
+                // copies that a warp which gave up no longer waits for land before this CTA's shared memory goes to another
+                for (int k = 0; k < TR_K_AHEAD; ++k) (void)tr_wait(kr_full + 8 * k, k < ks ? kph ^ 1u : kph);
+                for (int k = 0; k < TR_V_AHEAD; ++k) (void)tr_wait(vr_full + 8 * k, k < vs ? vph ^ 1u : vph);
+            }
+        } else if (warp >= TR_CONVERT) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
             cur.start(d, pre, f0);
-            // ---- codes to f16: warp w takes page w of every tile ----
-            const int w = warp - 4, count = f1 - f0;
+            // ---- codes to f16: warp w takes page w of every tile, the K of tile m + 1 before the V of tile m ----
+            const int w = warp - TR_CONVERT, count = f1 - f0;
             const int at = tr_place<BITS>(lane);
-            const int side = lane >> 4;                               // lanes 0-15: scales (and zero points) of K, 16-31: of V
-            const uint16_t* scales = side ? d.c.v_scale : d.c.k_scale;
-            const float* zps = side ? d.c.v_zp : d.c.k_zp;
-            // page numbers of this stream, 32 at a time: eight tiles
-            int ids = -1, ids_row = -2, ids_at = 0;
-            TRPage<BITS> xk, xv;
-            uint32_t scale = 0;
-            float zp = 0.f;
-            bool mine = false;
-            size_t prow = 0;
-            // what this warp needs of the tile at the cursor: page, scales, K
-            auto fetch = [&]() {
-                const int p = cur.tile * TR_PAGES + w;
-                if (cur.row != ids_row || p < ids_at || p >= ids_at + 32) {
-                    ids_row = cur.row;
-                    ids_at = p;
-                    ids = p + lane < d.c.max_pages ? __ldg(d.c.page_table + (size_t)cur.row * d.c.max_pages + p + lane) : -1;
+            int ks = 0, vs = 0, rows = 0;                             // stages; rows of page w that are inside the stream, of the tile whose K went last
+            uint32_t kph = 0, vph = 0;
+            float va0_next = 0.f, va1_next = 0.f;                     // factors of the V of the tile whose K went last
+            for (int m = -1; m < count; ++m) {
+                const int j = m + 1, v_rows = rows;
+                const float va0 = va0_next, va1 = va1_next;
+                if (j < count) {
+                    if (j > 0) cur.next(d, pre, f0 + j);
+                    rows = max(0, min(PIKV_PAGE_TOKENS, cur.end() - (cur.tile * TR_PAGES + w) * PIKV_PAGE_TOKENS));
+                    if (!tr_wait(kr_full + 8 * ks, kph)) { failed = true; break; }
+                    TRPage<BITS> x;
+                    if (rows > 0) x.load(smem + SM::KRING + (ks * TR_PAGES + w) * SM::PAGE, at);
+                    // the tile's exponents: lane = two neighbouring rows of page lane / 8, scales of K in one word, of V in another; rows
+                    // behind the end have none
+                    const unsigned char* metas = smem + SM::MRING + ks * TR_PAGES * SM::META;
+                    const unsigned char* pair = metas + (lane >> 3) * SM::META + (lane & 7) * 4;
+                    const int left = cur.end() - cur.tile * TR_KEYS - 2 * lane;       // rows from the pair's first on
+                    uint32_t k2 = left > 0 ? *reinterpret_cast<const uint32_t*>(pair) : 0u, v2 = left > 0 ? *reinterpret_cast<const uint32_t*>(pair + 32) : 0u;
+                    if (left == 1) k2 &= 0xffffu, v2 &= 0xffffu;
+                    const int ke = __reduce_max_sync(0xffffffffu, max(tr_exponent(k2 << 16), tr_exponent(k2 & 0xffff0000u)));
+                    const int ve = __reduce_max_sync(0xffffffffu, max(tr_exponent(v2 << 16), tr_exponent(v2 & 0xffff0000u)));
+                    // rows of V that are not finite
+                    const uint32_t odd0 = __ballot_sync(0xffffffffu, (v2 & 0x7f80u) == 0x7f80u), odd1 = __ballot_sync(0xffffffffu, (v2 & 0x7f800000u) == 0x7f800000u);
+                    // this warp's rows: tr_row(lane) and 8 on
+                    const unsigned char* meta = metas + w * SM::META;
+                    const int r0 = tr_row(lane);
+                    auto scale = [&](int r, int side) { return r < rows ? (uint32_t)reinterpret_cast<const uint16_t*>(meta + 32 * side)[r] << 16 : 0u; };
+                    const float up_k = exp2_int(15 - ke), up_v = exp2_int(15 - ve);
+                    const float ka0 = __uint_as_float(scale(r0, 0)) * up_k, ka1 = __uint_as_float(scale(r0 + 8, 0)) * up_k;
+                    auto finite = [](uint32_t s) { return (s & 0x7f800000u) == 0x7f800000u ? 0u : s; };
+                    va0_next = __uint_as_float(finite(scale(r0, 1))) * up_v;
+                    va1_next = __uint_as_float(finite(scale(r0 + 8, 1))) * up_v;
+                    // The four sets need no wait of their own: the one written here served tile j - 4, whose second product was
+                    // issued before the Q K^T of tile j - 2, and this warp has seen that one done
+                    if (w == 0 && lane == 0) *reinterpret_cast<int4*>(smem + SM::VEXP + (j & 3) * 16) = make_int4(ke + 9, ve + 9, (int)odd0, (int)odd1);
+                    if (BITS == 4) {
+                        // lanes 0-15: z of K, 16-31: of V
+                        const int side = lane >> 4, r = lane & 15;
+                        const float z = r < rows ? (reinterpret_cast<const float*>(meta + 64)[lane] - 8.f) * (__uint_as_float(scale(r, side)) * exp2_int(-9 - (side ? ve : ke))) : 0.f;
+                        reinterpret_cast<float*>(smem + SM::SIDE)[((j & 3) * 2 + side) * TR_KEYS + w * PIKV_PAGE_TOKENS + r] = z;
+                    }
+                    // Q K^T of the tile before has read the buffer
+                    if (j > 0 && !tr_wait(s_full + 8 * ((j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u)) { failed = true; break; }
+                    if (rows > 0) x.store(smem + SM::K, w, lane, ka0, ka1);
+                    tr_fence_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        lr_mbar_arrive(side_full + 8 * (j & 3));
+                        lr_mbar_arrive(k_full);
+                        lr_mbar_arrive(kr_empty + 8 * ks);
+                    }
+                    if (++ks == TR_K_AHEAD) ks = 0, kph ^= 1u;
                 }
-                mine = w < cur.pages();
-                int page = __shfl_sync(0xffffffffu, ids, p - ids_at);
-                if (mine && (page < 0 || page >= d.c.num_pages)) {
-                    if (lane == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_PAGE);
-                    page = 0;
-                }
-                prow = ((size_t)max(page, 0) * d.c.n_kv + cur.head) * PIKV_PAGE_TOKENS;
-                const bool there = mine && p * PIKV_PAGE_TOKENS + (lane & 15) < cur.end();      // rows behind the end have no scale
-                scale = there ? (uint32_t)__ldg(scales + prow + (lane & 15)) << 16 : 0u;
-                if (BITS == 4) zp = there ? __ldg(zps + prow + (lane & 15)) - 8.f : 0.f;
-                if (mine) xk.load(d.c.k_codes + prow * (16 * BITS), at);
-            };
-            auto fetch_v = [&]() { if (mine) xv.load(d.c.v_codes + prow * (16 * BITS), at); };
-            fetch();
-            fetch_v();
-            for (int m = 0; m < count; ++m) {
-                const uint32_t b = m & 1, ph = ((uint32_t)(m >> 1) & 1u) ^ 1u;
-                const bool now = mine;
-                // Q K^T of tile m - 2 has read this buffer.  The four sets of scales need no wait of their own: the one written here
-                // served tile m - 4, whose second product was issued before that Q K^T
-                if (!tr_wait(s_full + 8 * b, ph)) { failed = true; break; }
-                float* to = reinterpret_cast<float*>(smem + SM::SIDE) + (m & 3) * SM::SIDES * TR_KEYS + side * TR_KEYS + w * PIKV_PAGE_TOKENS + (lane & 15);
-                // a key of infinities has a logit that is not a number, whatever the sign of the whole product
-                *to = side == 0 && (scale & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(scale);
-                if (BITS == 4) to[2 * TR_KEYS] = zp;
-                const int e = __reduce_max_sync(0xffffffffu, side ? tr_exponent(scale) : -100);
-                if (lane == 0) reinterpret_cast<int*>(smem + SM::VEXP)[(m & 3) * 4 + w] = e;
-                if (now) xk.store(smem + SM::K + TR_TILE * b, w, lane);
+                if (m < 0) continue;
+                if (!tr_wait(vr_full + 8 * vs, vph)) { failed = true; break; }
+                TRPage<BITS> x;
+                if (v_rows > 0) x.load(smem + SM::VRING + (vs * TR_PAGES + w) * SM::PAGE, at);
+                if (m > 0 && !tr_wait(pv_done + 8 * ((m - 1) & 1), (uint32_t)((m - 1) >> 1) & 1u)) { failed = true; break; }
+                if (v_rows > 0) x.store(smem + SM::V, w, lane, va0, va1);
                 tr_fence_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    lr_mbar_arrive(side_full + 8 * (m & 3));
-                    lr_mbar_arrive(k_full + 8 * b);
+                    lr_mbar_arrive(v_full);
+                    lr_mbar_arrive(vr_empty + 8 * vs);
                 }
-                if (m + 1 < count) {
-                    cur.next(d, pre, f0 + m + 1);
-                    fetch();
-                }
-                if (!tr_wait(pv_done + 8 * b, ph)) { failed = true; break; }             // P V of tile m - 2
-                if (now) xv.store(smem + SM::V + TR_TILE * b, w, lane);
-                tr_fence_smem();
-                __syncwarp();
-                if (lane == 0) lr_mbar_arrive(v_full + 8 * b);
-                if (m + 1 < count) fetch_v();
+                if (++vs == TR_V_AHEAD) vs = 0, vph ^= 1u;
             }
         } else {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
@@ -504,6 +587,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             // ---- softmax: thread = row ----
             const uint32_t lanes = (uint32_t)(warp * 32) << 16;
             float qmul = 0.f, qsum = 0.f, ref = -INFINITY, den = 0.f, corr = 0.f;
+            float odd_v = 0.f;                                        // not a number once the row has seen a V that is not finite
             uint64_t tree = 0;
             int node = 0;
             bool live = false, warp_live = false;
@@ -517,7 +601,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     live = node < cur.nodes;
                     warp_live = __any_sync(0xffffffffu, live);
                     ref = -INFINITY;
-                    den = corr = 0.f;
+                    den = corr = odd_v = 0.f;
                     if (warp_live) {
                         out_row = ((size_t)cur.b * d.N + (live ? node : 0)) * d.n_q + (size_t)h * d.G + row % d.G;
                         const uint4* src = reinterpret_cast<const uint4*>(d.q + out_row * 128);
@@ -569,14 +653,19 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     __syncwarp();
                     if (lane == 0) lr_mbar_arrive(q_full);
                 }
-                if (!tr_wait(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u) || !tr_wait(side_full + 8 * (n & 3), (uint32_t)(n >> 2) & 1u)) { failed = true; break; }
+                if (!tr_wait2(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u, side_full + 8 * (n & 3), (uint32_t)(n >> 2) & 1u)) { failed = true; break; }
                 const bool last = f + 1 == f1 || cur.tile + 1 == cur.tiles;
                 if (warp_live) {
                     tr_fence_after();
                     const uint32_t scores = tmem + lanes + TR_COL_S + TR_KEYS * (n & 1);
-                    const float* ks = reinterpret_cast<const float*>(smem + SM::SIDE) + (n & 3) * SM::SIDES * TR_KEYS;
-                    const int4 ve = *reinterpret_cast<const int4*>(smem + SM::VEXP + (n & 3) * 16);
-                    int vexp = max(max(ve.x, ve.y), max(ve.z, ve.w));
+                    float x0[32], x1[32];
+                    tr_tmem_ld32(scores, x0);
+                    tr_tmem_ld32(scores + 32, x1);
+                    const float* kz = reinterpret_cast<const float*>(smem + SM::SIDE) + (n & 3) * SM::SIDES * TR_KEYS;      // 4 bit only
+                    const float* vz = kz + TR_KEYS;
+                    const int4 of = *reinterpret_cast<const int4*>(smem + SM::VEXP + (n & 3) * 16);
+                    float mul = qmul * exp2_int(of.x);
+                    if (mul == 0.f) mul = 1.17549435e-38f;               // (masked scores are -infinity: times 0 they would not be a number)
                     const int pos0 = cur.tile * TR_KEYS;
                     uint64_t seen = ~0ull;
                     const bool edge = pos0 + TR_KEYS > cur.ctx;          // the same for the whole CTA
@@ -584,21 +673,18 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                         // the positions behind the context show only where the mask opens them
                         const int sh = cur.ctx - pos0;                   // the tree's first bit
                         seen = sh >= 0 ? (sh < 64 ? tree << sh : 0ull) | ((1ull << sh) - 1) : (sh > -64 ? tree >> -sh : 0ull);
-                        vexp = -100;                                     // of the rows that this one sees
-#pragma unroll 4
-                        for (int j = 0; j < TR_KEYS; ++j)
-                            if ((seen >> j) & 1) vexp = max(vexp, tr_exponent(__float_as_uint(ks[TR_KEYS + j])));
                     }
-                    float x0[32], x1[32];
-                    tr_tmem_ld32(scores, x0);
-                    tr_tmem_ld32(scores + 32, x1);
+                    if (of.z | of.w) {                                   // (their bits: even rows in one word, odd ones in the other)
+                        for (int j = 0; j < TR_KEYS; ++j)
+                            if (((j & 1 ? of.w : of.z) >> (j >> 1)) & (int)(seen >> j) & 1) odd_v = __uint_as_float(0x7fffffffu);
+                    }
                     tr_tmem_ld_wait(x0);
                     tr_tmem_ld_wait(x1);
                     float mx;
-                    if (edge) mx = fmaxf(tr_scale<BITS, true>(x0, ks, qsum, (uint32_t)seen), tr_scale<BITS, true>(x1, ks + 32, qsum, (uint32_t)(seen >> 32)));
-                    else mx = fmaxf(tr_scale<BITS, false>(x0, ks, qsum, ~0u), tr_scale<BITS, false>(x1, ks + 32, qsum, ~0u));
+                    if (edge) mx = fmaxf(tr_scores<BITS, true>(x0, kz, qsum, (uint32_t)seen), tr_scores<BITS, true>(x1, kz + 32, qsum, (uint32_t)(seen >> 32)));
+                    else mx = fmaxf(tr_scores<BITS, false>(x0, kz, qsum, ~0u), tr_scores<BITS, false>(x1, kz + 32, qsum, ~0u));
                     // does the reference hold?  (-inf while nothing has been seen)
-                    const float want = mx * qmul + (float)vexp;
+                    const float want = mx * mul + (float)of.y;
                     const bool move = mx > -INFINITY && want > ref + TR_SLACK;
                     if (__any_sync(0xffffffffu, move)) {
                         const float next = move ? want : ref;
@@ -621,20 +707,22 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                             tr_tmem_st_wait();
                         }
                     }
-                    const float off = ref == -INFINITY ? 0.f : -ref;
+                    const float off = (float)of.y - (ref == -INFINITY ? 0.f : ref);
+                    float total = 0.f;
                     // the weights take the place of the scores that they come from, two to a column
                     {
                         uint32_t wgt[16];
-                        if (edge) tr_weights<BITS, true>(x0, wgt, ks + TR_KEYS, qmul, off, (uint32_t)seen, den, corr);
-                        else tr_weights<BITS, false>(x0, wgt, ks + TR_KEYS, qmul, off, ~0u, den, corr);
+                        if (edge) tr_weights<BITS, true>(x0, wgt, vz, mul, off, (uint32_t)seen, total, corr);
+                        else tr_weights<BITS, false>(x0, wgt, vz, mul, off, ~0u, total, corr);
                         tr_tmem_st16(scores, wgt);
                     }
                     {
                         uint32_t wgt[16];
-                        if (edge) tr_weights<BITS, true>(x1, wgt, ks + TR_KEYS + 32, qmul, off, (uint32_t)(seen >> 32), den, corr);
-                        else tr_weights<BITS, false>(x1, wgt, ks + TR_KEYS + 32, qmul, off, ~0u, den, corr);
+                        if (edge) tr_weights<BITS, true>(x1, wgt, vz + 32, mul, off, (uint32_t)(seen >> 32), total, corr);
+                        else tr_weights<BITS, false>(x1, wgt, vz + 32, mul, off, ~0u, total, corr);
                         tr_tmem_st16(scores + 16, wgt);
                     }
+                    den += total * exp2_int(-of.y);
                     tr_tmem_st_wait();
                     tr_fence_before();
                     __syncwarp();
@@ -663,6 +751,8 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) o[i] = t[i];
                             }
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] += odd_v;
                             if (live && whole) {
                                 uint4* to = reinterpret_cast<uint4*>(d.out + out_row * 128 + c);
 #pragma unroll
@@ -694,7 +784,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
     }
     tr_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == TR_MMA) {
         tr_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TR_COLS) : "memory");
     }

@@ -52,16 +52,17 @@ def attend64(q, k, v, sees):
     return out.reshape(R, n_q, D), lse.reshape(R, n_q), big.expand(R, n_kv, n_q // n_kv).reshape(R, n_q), size.reshape(R, n_q)
 
 
-def attention_bound(want, big, size, logit):
+def attention_bound(want, big, size, logit, value):
     """How far a kernel's output and log-sum-exp may be off: the output's rounding to bf16 (2^-8 of itself), the weights' to
-    f16 (2^-11, and 2^-24 of the largest where they are tiny) and an error of the logits, `logit` of their terms' sum, which moves a
-    weight and the denominator by that much each; the weights add up to 1, so all but the first are relative to the largest V."""
+    f16 (2^-11, and 2^-24 of the largest where they are tiny), that of V (`value` of the largest) and an error of the logits,
+    `logit` of their terms' sum, which moves a weight and the denominator by that much each; the weights add up to 1, so all but
+    the first are relative to the largest V."""
     slip = logit * size + 2.0 ** -20
-    return 2.0 ** -8 * want.abs() + ((2.0 ** -11 + 2.0 ** -20 + 2 * slip) * big)[..., None], slip + 2.0 ** -20
+    return 2.0 ** -8 * want.abs() + ((2.0 ** -11 + value + 2.0 ** -20 + 2 * slip) * big)[..., None], slip + 2.0 ** -20
 
 
-def check_attention(out, lse, want, want_lse, big, size, logit):
-    far, far_lse = attention_bound(want, big, size, logit)
+def check_attention(out, lse, want, want_lse, big, size, logit, value=0.0):
+    far, far_lse = attention_bound(want, big, size, logit, value)
     nothing = want_lse == -math.inf
     off = (out.double() - want).abs()
     assert bool((off <= far).all()), f"output off by {float((off / far.clamp(min=1e-300)).max())} of what its roundings allow"

@@ -7,9 +7,13 @@ import torch
 from paged_reference import D, append_rows, attend64, check_attention, filled_cache, rows64
 
 pytestmark = pytest.mark.gpu
-# a logit: 128 products summed in fp32 (2^-24 each at most, of the sum of their sizes; tensor cores truncate, twice that),
-# the scalings behind them and the exponential's argument (a few times 2^-24 of a value below the same sum)
-LOGIT = (2 * 128 + 8) * 2.0 ** -24
+# K and V enter as f16 in units of 2^(e - 9), 2^e above the largest scale of 64 rows: a rounding of 2^-11 of the entry, and of
+# 2^-25 units = 2^-16 2^e, at most 2^-15 of the largest scale, where the entry is below f16's normal range.  Rows of one size have
+# entries of 40 scales in the mean (127 at most), their scales lie within a factor of two: 2^-15 / 20 < 2^-19 of a mean entry.
+# A logit: that of each of its 128 products, which are then summed in fp32 (2^-24 each at most, of the sum of their sizes; tensor
+# cores truncate, twice that), the scalings behind them and the exponential's argument (a few times 2^-24 of a value below that sum)
+VALUE = 2.0 ** -11 + 2.0 ** -19
+LOGIT = VALUE + (2 * 128 + 8) * 2.0 ** -24
 
 
 @pytest.fixture(autouse=True)
@@ -43,7 +47,7 @@ def compare(cache, q, mask, ctx, nodes, out, lse, ids=None):
         k, v = rows64(cache, s, n + t)
         m = mask[b] if mask.dim() == 3 else mask
         sees = torch.cat([torch.ones(t, n, dtype=torch.bool, device="cuda"), m[:t, :t]], 1)
-        check_attention(out[b, :t], None if lse is None else lse[b, :t], *attend64(q[b, :t], k, v, sees), LOGIT)
+        check_attention(out[b, :t], None if lse is None else lse[b, :t], *attend64(q[b, :t], k, v, sees), LOGIT, VALUE)
 
 
 # one row alone; contexts at the edges of pages and of 64-row tiles; row counts (nodes x group) of one, of a ragged tile, of two and
@@ -117,7 +121,7 @@ def test_tree_many_streams():
     for b in some.tolist():
         k, v = rows64(cache, b, rows[b])
         sees = torch.cat([torch.ones(N, rows[b] - N, dtype=torch.bool, device="cuda"), mask[b]], 1)
-        check_attention(out[b], lse[b], *attend64(q[b], k, v, sees), LOGIT)
+        check_attention(out[b], lse[b], *attend64(q[b], k, v, sees), LOGIT, VALUE)
     ids = torch.randperm(S, generator=gen, device="cuda")
     cache.length.copy_(ctx)
     again = cache.decode_attention_tree(q[ids].contiguous(), mask[ids].contiguous(), seq_ids=ids.int())
