@@ -88,6 +88,9 @@ template <int BITS> struct TRSmem {
     static constexpr int BYTES = END + 1024;
 };
 
+// what hardly ever happens goes behind the loops: a jump over it costs the instruction cache
+#define TR_RARE(x) __builtin_expect(!!(x), 0)
+
 struct TreeParts {
     float* o;                            // [2 C][rows][128]
     float2* ml;                          // [2 C][rows] reference and denominator
@@ -117,7 +120,7 @@ struct TreeCursor {
         row_tile = unit % row_tiles;
     }
     __device__ __forceinline__ void next(const TreeDev& d, const int* pre, int f) {      // f: the place after this one
-        if (++tile < tiles) return;
+        if (!TR_RARE(++tile >= tiles)) return;
         tile = 0;
         if (++row_tile < row_tiles) return;
         row_tile = 0;
@@ -417,7 +420,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             bool first_before = true;                                // whether tile n - 1 opened its unit here
             auto pv = [&](int m, bool first) {
                 const uint32_t b = m & 1, ph = (uint32_t)(m >> 1) & 1u;
-                if (!tr_wait2(v_full, b, p_full + 8 * b, ph)) return false;
+                if (TR_RARE(!tr_wait2(v_full, b, p_full + 8 * b, ph))) return false;
                 tr_fence_after();
                 if (lr_elect()) {
 #pragma unroll
@@ -431,14 +434,14 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             for (int n = 0; n < count; ++n) {
                 const bool first = n == 0 || cur.tile == 0;
                 const uint32_t b = n & 1;
-                if (first) {
+                if (TR_RARE(first)) {
                     // the next unit's Q takes the place of this one's after its last product
                     if (n > 0 && !pv(n - 1, first_before)) { failed = true; break; }
-                    if (!tr_wait(q_full, seg & 1u)) { failed = true; break; }
+                    if (TR_RARE(!tr_wait(q_full, seg & 1u))) { failed = true; break; }
                     ++seg;
                 }
                 // (S of tile n lies where the weights of tile n - 2 were: their product has been issued before this one)
-                if (!tr_wait(k_full, b)) { failed = true; break; }
+                if (TR_RARE(!tr_wait(k_full, b))) { failed = true; break; }
                 tr_fence_after();
                 if (lr_elect()) {
 #pragma unroll
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     lr_commit(s_full + 8 * b);
                 }
                 __syncwarp();
-                if (!first && !pv(n - 1, first_before)) { failed = true; break; }
+                if (!first && TR_RARE(!pv(n - 1, first_before))) { failed = true; break; }
                 first_before = first;
                 if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
             }
@@ -468,18 +471,18 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     if (n < count) {
                         const int p = cur.tile * TR_PAGES;
                         np = cur.pages();
-                        if (cur.row != ids_row || p < ids_at || p >= ids_at + 32) {
+                        if (TR_RARE(cur.row != ids_row || p < ids_at || p >= ids_at + 32)) {
                             ids_row = cur.row;
                             ids_at = p;
                             ids = p + lane < d.c.max_pages ? __ldg(d.c.page_table + (size_t)cur.row * d.c.max_pages + p + lane) : -1;
                         }
                         int page = __shfl_sync(0xffffffffu, ids, (p + i - ids_at) & 31);
-                        if (i < np && (page < 0 || page >= d.c.num_pages)) {
+                        if (TR_RARE(i < np && (page < 0 || page >= d.c.num_pages))) {
                             if (lane < 4 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_PAGE);
                             page = 0;
                         }
                         unit = (uint32_t)page * (uint32_t)d.c.n_kv + (uint32_t)cur.head;
-                        if (!tr_wait(kr_empty + 8 * ks, kph)) { failed = true; break; }
+                        if (TR_RARE(!tr_wait(kr_empty + 8 * ks, kph))) { failed = true; break; }
                         const uint32_t bar = kr_full + 8 * ks;
                         if (lane == 0) lr_mbar_expect_tx(bar, (uint32_t)np * (SM::PAGE + SM::META));
                         __syncwarp();
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                         if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
                     }
                     if (n == 0) continue;
-                    if (!tr_wait(vr_empty + 8 * vs, vph)) { failed = true; break; }
+                    if (TR_RARE(!tr_wait(vr_empty + 8 * vs, vph))) { failed = true; break; }
                     if (lane == 4) lr_mbar_expect_tx(vr_full + 8 * vs, (uint32_t)v_np * SM::PAGE);
                     __syncwarp();
                     if (lane >= 4 && lane < 4 + v_np)
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 if (j < count) {
                     if (j > 0) cur.next(d, pre, f0 + j);
                     rows = max(0, min(PIKV_PAGE_TOKENS, cur.end() - (cur.tile * TR_PAGES + w) * PIKV_PAGE_TOKENS));
-                    if (!tr_wait(kr_full + 8 * ks, kph)) { failed = true; break; }
+                    if (TR_RARE(!tr_wait(kr_full + 8 * ks, kph))) { failed = true; break; }
                     TRPage<BITS> x;
                     if (rows > 0) x.load(smem + SM::KRING + (ks * TR_PAGES + w) * SM::PAGE, at);
                     // the tile's exponents: lane = two neighbouring rows of page lane / 8, scales of K in one word, of V in another; rows
@@ -568,7 +571,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     if (++ks == TR_K_AHEAD) ks = 0, kph ^= 1u;
                 }
                 if (m < 0) continue;
-                if (!tr_wait(vr_full + 8 * vs, vph)) { failed = true; break; }
+                if (TR_RARE(!tr_wait(vr_full + 8 * vs, vph))) { failed = true; break; }
                 TRPage<BITS> x;
                 if (v_rows > 0) x.load(smem + SM::VRING + (vs * TR_PAGES + w) * SM::PAGE, at);
                 if (m > 0 && !tr_wait(pv_done + 8 * ((m - 1) & 1), (uint32_t)((m - 1) >> 1) & 1u)) { failed = true; break; }
@@ -594,7 +597,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             size_t out_row = 0;
             for (int n = 0, f = f0; f < f1; ++f, ++n) {
                 const bool first = n == 0 || cur.tile == 0;
-                if (first) {
+                if (TR_RARE(first)) {
                     // ---- this row's query ----
                     const int row = cur.row_tile * TR_ROWS + tid, h = cur.head;
                     node = row / d.G;
@@ -653,7 +656,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     __syncwarp();
                     if (lane == 0) lr_mbar_arrive(q_full);
                 }
-                if (!tr_wait2(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u, side_full + 8 * (n & 3), (uint32_t)(n >> 2) & 1u)) { failed = true; break; }
+                if (TR_RARE(!tr_wait2(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u, side_full + 8 * (n & 3), (uint32_t)(n >> 2) & 1u))) { failed = true; break; }
                 const bool last = f + 1 == f1 || cur.tile + 1 == cur.tiles;
                 if (warp_live) {
                     tr_fence_after();
@@ -669,31 +672,31 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     const int pos0 = cur.tile * TR_KEYS;
                     uint64_t seen = ~0ull;
                     const bool edge = pos0 + TR_KEYS > cur.ctx;          // the same for the whole CTA
-                    if (edge) {
+                    if (TR_RARE(edge)) {
                         // the positions behind the context show only where the mask opens them
                         const int sh = cur.ctx - pos0;                   // the tree's first bit
                         seen = sh >= 0 ? (sh < 64 ? tree << sh : 0ull) | ((1ull << sh) - 1) : (sh > -64 ? tree >> -sh : 0ull);
                     }
-                    if (of.z | of.w) {                                   // (their bits: even rows in one word, odd ones in the other)
+                    if (TR_RARE(of.z | of.w)) {                                   // (their bits: even rows in one word, odd ones in the other)
                         for (int j = 0; j < TR_KEYS; ++j)
                             if (((j & 1 ? of.w : of.z) >> (j >> 1)) & (int)(seen >> j) & 1) odd_v = __uint_as_float(0x7fffffffu);
                     }
                     tr_tmem_ld_wait(x0);
                     tr_tmem_ld_wait(x1);
                     float mx;
-                    if (edge) mx = fmaxf(tr_scores<BITS, true>(x0, kz, qsum, (uint32_t)seen), tr_scores<BITS, true>(x1, kz + 32, qsum, (uint32_t)(seen >> 32)));
+                    if (TR_RARE(edge)) mx = fmaxf(tr_scores<BITS, true>(x0, kz, qsum, (uint32_t)seen), tr_scores<BITS, true>(x1, kz + 32, qsum, (uint32_t)(seen >> 32)));
                     else mx = fmaxf(tr_scores<BITS, false>(x0, kz, qsum, ~0u), tr_scores<BITS, false>(x1, kz + 32, qsum, ~0u));
                     // does the reference hold?  (-inf while nothing has been seen)
                     const float want = mx * mul + (float)of.y;
                     const bool move = mx > -INFINITY && want > ref + TR_SLACK;
-                    if (__any_sync(0xffffffffu, move)) {
+                    if (TR_RARE(__any_sync(0xffffffffu, move))) {
                         const float next = move ? want : ref;
                         const float fac = move ? tr_ex2(ref - next) : 1.f;     // 0 from -inf
                         ref = next;
                         den *= fac;
                         corr *= fac;
                         if (!first) {
-                            if (!tr_wait(pv_done + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u)) { failed = true; break; }
+                            if (TR_RARE(!tr_wait(pv_done + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) { failed = true; break; }
                             tr_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < 128; c += 16) {             // few registers: the scores are in the others
@@ -712,13 +715,13 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     // the weights take the place of the scores that they come from, two to a column
                     {
                         uint32_t wgt[16];
-                        if (edge) tr_weights<BITS, true>(x0, wgt, vz, mul, off, (uint32_t)seen, total, corr);
+                        if (TR_RARE(edge)) tr_weights<BITS, true>(x0, wgt, vz, mul, off, (uint32_t)seen, total, corr);
                         else tr_weights<BITS, false>(x0, wgt, vz, mul, off, ~0u, total, corr);
                         tr_tmem_st16(scores, wgt);
                     }
                     {
                         uint32_t wgt[16];
-                        if (edge) tr_weights<BITS, true>(x1, wgt, vz + 32, mul, off, (uint32_t)(seen >> 32), total, corr);
+                        if (TR_RARE(edge)) tr_weights<BITS, true>(x1, wgt, vz + 32, mul, off, (uint32_t)(seen >> 32), total, corr);
                         else tr_weights<BITS, false>(x1, wgt, vz + 32, mul, off, ~0u, total, corr);
                         tr_tmem_st16(scores + 16, wgt);
                     }
@@ -730,9 +733,9 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 } else if (lane == 0) {
                     lr_mbar_arrive(p_full + 8 * (n & 1));
                 }
-                if (last) {
+                if (TR_RARE(last)) {
                     // ---- this CTA's share of the unit is done ----
-                    if (!tr_wait(pv_done + 8 * (n & 1), (uint32_t)(n >> 1) & 1u)) { failed = true; break; }
+                    if (TR_RARE(!tr_wait(pv_done + 8 * (n & 1), (uint32_t)(n >> 1) & 1u))) { failed = true; break; }
                     if (warp_live) {
                         tr_fence_after();
                         const int begun = f - cur.tile;                  // place of the unit's first tile
