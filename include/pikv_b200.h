@@ -588,7 +588,8 @@ int pikv_tree_accept(const pikv_paged_cache* c, const int32_t* path, const int32
  * the smallest key of each channel as whole steps of a power of two, rounded outwards:
  *   bound_scale[page][h] = the smallest power of two s >= 2^-126 with |K| <= 127 s on the page
  *   bound_codes[page][h][0][c] = ceil(max K_c / s),  [1][c] = floor(min K_c / s)      int8
- * A page that holds something not finite has scale +infinity and codes 0.  The pages that hold positions
+ * A page with a row whose scale (or zero point) is not below 2^112 in size, what is not finite among them, or with a key that
+ * is not finite has scale +infinity and codes 0.  The pages that hold positions
  * start[b] .. seq_len[b] - 1 (start NULL: all) are computed anew.  Decodable formats (see bits). */
 int pikv_page_bounds_update(const pikv_paged_cache* c, void* bound_codes, float* bound_scale, const int32_t* seq_ids,
                             const int32_t* start, const int32_t* seq_len, int32_t B, pikv_stream_t stream);

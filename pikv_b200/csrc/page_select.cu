@@ -8,12 +8,22 @@
 // number times exact powers of two: the choice of pages depends neither on the order of a sum nor on the type it is held in.
 #include "stream_list.cuh"
 #include "shard_decode.cuh"
+#include "tc_common.cuh"
 
 namespace pikv {
 
 // ---- bounds ---------------------------------------------------------------------------------------------------
 constexpr int PB_THREADS = 256;
 constexpr int PB_CTAS = 4;               // per SM
+constexpr int PB_STAGES = 3;             // pages that a warp has on their way or at hand
+
+// a stage of a warp's ring: codes of a page of one head, scales (and zero points), and what the warp needs to know of it
+template <int BITS> struct PBGeom {
+    static constexpr int CODES = 256 * BITS, COPY = CODES + 32 + (BITS == 4 ? 64 : 0), STAGE = COPY + 16;
+    static constexpr int SMEM = (PB_THREADS / 32) * PB_STAGES * (STAGE + 8);
+};
+constexpr float PB_HUGE = 5.192296858534828e33f;       // 2^112: 2^15 + 128 times a scale below it is finite
+constexpr uint32_t PB_HUGE_BITS = 0x7780u;            // the same as bf16
 
 struct BoundsDev {
     CacheDev c;
@@ -25,13 +35,25 @@ struct BoundsDev {
     int B;
 };
 
-__device__ __forceinline__ float unit_code(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 
-// One warp per (page, head).  Lane l holds channels 16 (l & 7) .. + 15 of rows (l >> 3) + 4 i: one 16-byte chunk (8 bit) or
-// one 8-byte unit (4 bit) of four rows, read where the cache's swizzle has put them, so that eight lanes read a whole row.
-// The four row groups are joined by two exchanges in which a lane gives away half of its channels each time.
+__device__ __forceinline__ void pb_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// One warp per (page, head); a lane has CH channels of ROWS rows (8 bit: 4 channels of all sixteen, 4 bit: 8 channels of every
+// second row, joined by one exchange), so that a load of the warp is whole rows, wherever the cache's swizzle has put their
+// chunks, and next to nothing crosses lanes.  Pages come by bulk copies into a ring of the warp's own (with plain loads a warp
+// had nothing on its way while it computed).
+// Bound by the integer pipes.  Keys are compared as whole numbers: a scale is m 2^E with m below 2^8, so code m 2^(E - least E of the
+// page) fits 32 bits where the exponents span at most 15; one byte-dot-product takes a code out of its word (and the zero point
+// off), one multiplication does the rest, and two rows go into a three-operand maximum and minimum.  (As floats, a byte-permute, half
+// a fused operation, a minimum and a maximum a key: 88 us for 8 x 32768 rows x 8 heads, now 74 = 4.1 TB/s.)  Pages that this does not fit,
+// a stream's unfilled last one among them, take floats: a byte becomes 2^15 + u exactly by one byte-permute (u = code + 128 in
+// the second byte of 0x47000000) and a key by (2^15 + u) s - (2^15 + 128) s, whose second factor has 17 bits and is exact.
 template <int BITS>
 __global__ void __launch_bounds__(PB_THREADS, PB_CTAS) page_bounds_kernel(BoundsDev d) {
+    constexpr int ROWS = BITS == 8 ? 16 : 8, CH = BITS == 8 ? 4 : 8;
     __shared__ int pre[PIKV_STREAMS_PER_LAUNCH + 1];
     const int lane = threadIdx.x & 31;
     const int n_kv = d.c.n_kv, max_len = d.c.max_pages * PIKV_PAGE_TOKENS;
@@ -50,92 +72,201 @@ __global__ void __launch_bounds__(PB_THREADS, PB_CTAS) page_bounds_kernel(Bounds
         if (d.start && __ldg(d.start + i) >= len) return 0;
         return max(0, (len + PIKV_PAGE_TOKENS - 1) / PIKV_PAGE_TOKENS - first);
     });
+    // runs of (page, head) items, heads innermost: they lie side by side in the pool
     const long long items = (long long)total * n_kv;
     const int warps = gridDim.x * (PB_THREADS / 32);
     const int self = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
-    const int ch = lane & 7, rg = lane >> 3;
-    for (long long it = self; it < items; it += warps) {
-        const int f = (int)(it / n_kv), h = (int)(it % n_kv);
-        const int b = stream_of(pre, d.B, f);
-        int first, len;
-        const int row = range(b, first, len);
-        const int lp = first + f - pre[b];
-        const int page = stream_page(d.c, row, lp);
-        const int rows = min(PIKV_PAGE_TOKENS, len - lp * PIKV_PAGE_TOKENS);
-        const size_t base = ((size_t)page * n_kv + h) * PIKV_PAGE_TOKENS;
-        float hi[16], lo[16];
+    const long long run = (items + warps - 1) / warps, it0 = min(items, self * run);
+    int left = (int)(min(items, it0 + run) - it0);
+    if (left <= 0) return;
+    extern __shared__ __align__(16) unsigned char pb_smem[];
+    using GEO = PBGeom<BITS>;
+    unsigned char* ring = pb_smem + (threadIdx.x >> 5) * PB_STAGES * GEO::STAGE;
+    const uint32_t bar0 = lr_smem_u32(pb_smem + (PB_THREADS / 32) * PB_STAGES * GEO::STAGE) + (threadIdx.x >> 5) * PB_STAGES * 8;
+    if (lane == 0) {
+        for (int i = 0; i < PB_STAGES; ++i) lr_mbar_init(bar0 + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    // the item that is copied next
+    int f = (int)(it0 / n_kv), h = (int)(it0 % n_kv);
+    int b = stream_of(pre, d.B, f), first, len;
+    int row = range(b, first, len);
+    int lp = first + f - pre[b], page = stream_page(d.c, row, lp);
+    int to_copy = left;
+    auto copy = [&](int stage) {
+        if (to_copy == 0) return;
+        const size_t unit = (size_t)page * n_kv + h;
+        unsigned char* to = ring + stage * GEO::STAGE;
+        if (lane == 0) {
+            const uint32_t dst = lr_smem_u32(to), bar = bar0 + 8 * stage;
+            *reinterpret_cast<int4*>(to + GEO::COPY) = make_int4((int)(uint32_t)unit, (int)(uint32_t)(unit >> 32), min(PIKV_PAGE_TOKENS, len - lp * PIKV_PAGE_TOKENS), 0);
+            lr_mbar_expect_tx(bar, GEO::COPY);
+            pb_bulk(dst, d.c.k_codes + unit * GEO::CODES, GEO::CODES, bar);
+            pb_bulk(dst + GEO::CODES, d.c.k_scale + unit * 16, 32, bar);
+            if (BITS == 4) pb_bulk(dst + GEO::CODES + 32, d.c.k_zp + unit * 16, 64, bar);
+        }
+        __syncwarp();
+        if (--to_copy == 0) return;
+        if (++h < n_kv) return;
+        h = 0;
+        if (++f == pre[b + 1]) {
+            do ++b; while (pre[b + 1] <= f);
+            row = range(b, first, len);
+        }
+        lp = first + f - pre[b];
+        page = stream_page(d.c, row, lp);
+    };
+    for (int i = 0; i < PB_STAGES - 1; ++i) copy(i);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool late = false;
+    for (; left > 0; --left) {
+        copy(stage == 0 ? PB_STAGES - 1 : stage - 1);            // the stage of the item before this one
+        late |= !lr_mbar_wait(bar0 + 8 * stage, phase);
+        if (late) break;
+        const unsigned char* from = ring + stage * GEO::STAGE;
+        const int4 what = *reinterpret_cast<const int4*>(from + GEO::COPY);
+        const size_t unit = (size_t)(uint32_t)what.y << 32 | (uint32_t)what.x;
+        const int rows = what.z;
+        uint32_t w[ROWS];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) hi[i] = -INFINITY, lo[i] = INFINITY;
-        bool bad = false;
+        for (int i = 0; i < ROWS; ++i) {
+            // 8 bit: chunk lane / 4 of row i; 4 bit: unit (lane % 16) / 2 of row 2 i + lane / 16
+            const int r = BITS == 8 ? i : 2 * i + (lane >> 4);
+            const int at = BITS == 8 ? i * 128 + 16 * ((lane >> 2) ^ (i & 7)) + 4 * (lane & 3) : r * 64 + 8 * (((lane & 15) >> 1) ^ (r & 4)) + 4 * (lane & 1);
+            w[i] = *reinterpret_cast<const uint32_t*>(from + at);
+        }
+        // this lane's row, lane % 16: scale as m 2^(E - 134)
+        const uint32_t mine = reinterpret_cast<const uint16_t*>(from + GEO::CODES)[lane & 15];
+        const bool inside = (lane & 15) < rows;
+        const int E = max(1, (int)((mine >> 7) & 0xffu));
+        const uint32_t m = (mine & 0x7fu) | (mine & 0x7f80u ? 0x80u : 0u);
+        float zmine = 0.f;
+        if (BITS == 4) zmine = reinterpret_cast<const float*>(from + GEO::CODES + 32)[lane & 15];
+        // a row that bounds cannot hold
+        const bool bad = __any_sync(0xffffffffu, inside && ((mine & 0x7fffu) >= PB_HUGE_BITS || !(fabsf(zmine) < PB_HUGE)));
+        const int least = __reduce_min_sync(0xffffffffu, m ? E : 255), most = __reduce_max_sync(0xffffffffu, m ? E : 0);
+        const bool whole = rows == PIKV_PAGE_TOKENS && least >= 8 && most - least <= 15 &&
+                           __all_sync(0xffffffffu, mine < 0x8000u && (BITS == 8 || (fabsf(zmine) <= 127.f && zmine == rintf(zmine))));
+        float hi[CH], lo[CH];
+        if (whole) {
+            // m 2^(E - least) of the rows, as the lanes of their rows have it, and (4 bit) the zero point
+            const int factor = (int)(m << (m ? E - least : 0)), off = BITS == 4 ? -(int)zmine : 0;
+            int ihi[CH], ilo[CH];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = rg + 4 * i;
-            if (r >= rows) continue;
-            const float s = bf16_bits_to_f32(__ldg(d.c.k_scale + base + r));
-            bad |= !(fabsf(s) < INFINITY);
-            if (BITS == 8) {
-                const uint4 w = __ldg(reinterpret_cast<const uint4*>(d.c.k_codes + (base + r) * 128) + (ch ^ (r & 7)));
-                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+            for (int k = 0; k < CH; ++k) ihi[k] = -0x7fffffff, ilo[k] = 0x7fffffff;
+            auto keys = [&](int i, int (&x)[CH]) {
+                const int r = BITS == 8 ? i : 2 * i + (lane >> 4);
+                const int mr = __shfl_sync(0xffffffffu, factor, r);
+                if constexpr (BITS == 8) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float x = unit_code(ww[j >> 2], j & 3) * s;
-                    hi[j] = fmaxf(hi[j], x);
-                    lo[j] = fminf(lo[j], x);
+                    for (int k = 0; k < 4; ++k) {
+                        int p;                                               // byte k, with its sign
+                        asm("dp4a.s32.u32 %0, %1, %2, 0;" : "=r"(p) : "r"(w[i]), "r"(1u << (8 * k)));
+                        x[k] = p * mr;
+                    }
+                } else {
+                    const int c = __shfl_sync(0xffffffffu, off, r);
+                    const uint32_t n0 = w[i] & 0x0f0f0f0fu, n1 = (w[i] >> 4) & 0x0f0f0f0fu;       // even and odd channels
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        int p, q;                                            // code less zero point
+                        asm("dp4a.s32.u32 %0, %1, %2, %3;" : "=r"(p) : "r"(n0), "r"(1u << (8 * k)), "r"(c));
+                        asm("dp4a.s32.u32 %0, %1, %2, %3;" : "=r"(q) : "r"(n1), "r"(1u << (8 * k)), "r"(c));
+                        x[2 * k] = p * mr;
+                        x[2 * k + 1] = q * mr;
+                    }
                 }
-            } else {
-                const float z = __ldg(d.c.k_zp + base + r);
-                bad |= !(fabsf(z) < INFINITY);
-                const uint2 w = __ldg(reinterpret_cast<const uint2*>(d.c.k_codes + (base + r) * 64) + (ch ^ (r & 4)));
-                const uint32_t ww[2] = {w.x, w.y};
+            };
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float x = __fmul_rn(__fsub_rn((float)((ww[j >> 3] >> (4 * (j & 7))) & 15u), z), s);
-                    hi[j] = fmaxf(hi[j], x);
-                    lo[j] = fminf(lo[j], x);
+            for (int i = 0; i < ROWS; i += 2) {
+                int x[CH], y[CH];
+                keys(i, x);
+                keys(i + 1, y);
+#pragma unroll
+                for (int k = 0; k < CH; ++k) {
+                    ihi[k] = __vimax3_s32(ihi[k], x[k], y[k]);
+                    ilo[k] = __vimin3_s32(ilo[k], x[k], y[k]);
+                }
+            }
+            // (16 bits and a shift: exact)
+            const float unit_of = exp2_int(least - 134);
+#pragma unroll
+            for (int k = 0; k < CH; ++k) hi[k] = (float)ihi[k] * unit_of, lo[k] = (float)ilo[k] * unit_of;
+        } else {
+            const uint4 s_lo = *reinterpret_cast<const uint4*>(from + GEO::CODES), s_hi = *reinterpret_cast<const uint4*>(from + GEO::CODES + 16);
+            const uint32_t sw[8] = {s_lo.x, s_lo.y, s_lo.z, s_lo.w, s_hi.x, s_hi.y, s_hi.z, s_hi.w};
+#pragma unroll
+            for (int i = 0; i < CH; ++i) hi[i] = -INFINITY, lo[i] = INFINITY;
+            auto scale = [&](int r) { return __uint_as_float(r & 1 ? sw[r >> 1] & 0xffff0000u : sw[r >> 1] << 16); };
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                float x[CH];
+                if constexpr (BITS == 8) {
+                    const float s = scale(i), c = -32896.f * s;
+                    const uint32_t u = w[i] ^ 0x80808080u;                   // code + 128
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = fmaf(__uint_as_float(__byte_perm(u, 0x47000000u, 0x7504u + 16u * k)), s, c);
+                } else {
+                    const float s = lane >> 4 ? scale(2 * i + 1) : scale(2 * i), z = reinterpret_cast<const float*>(from + GEO::CODES + 32)[2 * i + (lane >> 4)];
+                    // even channels in the low nibbles; less the zero point, times the scale, each rounded as the cache's reader does
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(__fsub_rn((float)((w[i] >> (4 * k)) & 15u), z), s);
+                }
+                if ((BITS == 8 ? i : 2 * i + (lane >> 4)) < rows) {
+#pragma unroll
+                    for (int k = 0; k < CH; ++k) {
+                        hi[k] = fmaxf(hi[k], x[k]);
+                        lo[k] = fminf(lo[k], x[k]);
+                    }
                 }
             }
         }
-        // lanes l and l ^ 16 keep channels 0..7 / 8..15 of their chunk, then l and l ^ 8 four of those
-        const bool up16 = lane & 16, up8 = lane & 8;
+        int at = 4 * lane;
+        if (BITS == 4) {
+            // lanes l and l + 16 have the same channels: each keeps four of the eight
+            const bool up = lane >> 4;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float gh = __shfl_xor_sync(0xffffffffu, up16 ? hi[j] : hi[j + 8], 16);
-            const float gl = __shfl_xor_sync(0xffffffffu, up16 ? lo[j] : lo[j + 8], 16);
-            hi[j] = fmaxf(up16 ? hi[j + 8] : hi[j], gh);
-            lo[j] = fminf(up16 ? lo[j + 8] : lo[j], gl);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float gh = __shfl_xor_sync(0xffffffffu, up8 ? hi[j] : hi[j + 4], 8);
-            const float gl = __shfl_xor_sync(0xffffffffu, up8 ? lo[j] : lo[j + 4], 8);
-            hi[j] = fmaxf(up8 ? hi[j + 4] : hi[j], gh);
-            lo[j] = fminf(up8 ? lo[j + 4] : lo[j], gl);
+            for (int k = 0; k < 4; ++k) {
+                const float gh = __shfl_xor_sync(0xffffffffu, up ? hi[k] : hi[CH - 4 + k], 16), gl = __shfl_xor_sync(0xffffffffu, up ? lo[k] : lo[CH - 4 + k], 16);
+                hi[k] = fmaxf(up ? hi[CH - 4 + k] : hi[k], gh);
+                lo[k] = fminf(up ? lo[CH - 4 + k] : lo[k], gl);
+            }
+            at = 8 * (lane & 15) + (up ? 4 : 0);
         }
         float a = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a = fmaxf(a, fmaxf(fabsf(hi[j]), fabsf(lo[j])));
-        a = warp_max(a);
-        bad = __any_sync(0xffffffffu, bad || !(a < INFINITY));
-        const int e = bad ? 0 : step_exponent(a);
+        for (int k = 0; k < 4; ++k) a = fmaxf(a, fmaxf(fabsf(hi[k]), fabsf(lo[k])));
+        // (bits of a float that is not negative order as it does)
+        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(a));
+        const bool odd = bad || top >= 0x7f800000u;
+        const int e = odd ? 0 : step_exponent(__uint_as_float(top));
         const float inv = exp2_int(-e);
         uint32_t ph = 0, pl = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int ih = bad ? 0 : __float2int_ru(hi[j] * inv), il = bad ? 0 : __float2int_rd(lo[j] * inv);
-            ph |= (uint32_t)(ih & 0xff) << (8 * j);
-            pl |= (uint32_t)(il & 0xff) << (8 * j);
+        for (int k = 0; k < 4; ++k) {
+            const int ih = odd ? 0 : __float2int_ru(hi[k] * inv), il = odd ? 0 : __float2int_rd(lo[k] * inv);
+            ph |= (uint32_t)(ih & 0xff) << (8 * k);
+            pl |= (uint32_t)(il & 0xff) << (8 * k);
         }
-        const size_t out = ((size_t)page * n_kv + h) * 256;
-        const int at = 16 * ch + (up16 ? 8 : 0) + (up8 ? 4 : 0);
-        *reinterpret_cast<uint32_t*>(d.codes + out + at) = ph;
-        *reinterpret_cast<uint32_t*>(d.codes + out + 128 + at) = pl;
-        if (lane == 0) d.scale[(size_t)page * n_kv + h] = bad ? INFINITY : exp2_int(e);
+        *reinterpret_cast<uint32_t*>(d.codes + unit * 256 + at) = ph;
+        *reinterpret_cast<uint32_t*>(d.codes + unit * 256 + 128 + at) = pl;
+        if (lane == 0) d.scale[unit] = odd ? INFINITY : exp2_int(e);
+        __syncwarp();                                             // the stage is copied into again
+        if (++stage == PB_STAGES) stage = 0, phase ^= 1u;
+    }
+    if (late) {
+        if (lane == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_WAIT_TIMEOUT);
+        // what is on its way lands before the block leaves
+        for (int i = 0; i < PB_STAGES; ++i) (void)lr_mbar_wait(bar0 + 8 * i, i < stage ? phase ^ 1u : phase);
     }
 }
 
 // ---- scores ---------------------------------------------------------------------------------------------------
 constexpr int PS_THREADS = 256;
-constexpr int PS_CTAS = 4;               // per SM
+constexpr int PS_CTAS = 3;               // per SM
 constexpr int PS_GROUP = 8;              // query heads per KV head, at most
 
 struct SelectDev {
@@ -179,17 +310,33 @@ __global__ void __launch_bounds__(PS_THREADS, PS_CTAS) page_score_kernel(SelectD
     const long long items = (long long)total * n_kv;                       // per stream: head by head, 16 pages each
     const int warps = gridDim.x * (PS_THREADS / 32);
     const int self = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
-    const long long per = (items + warps - 1) / warps, end = min(items, (self + 1ll) * per);
+    const long long run = (items + warps - 1) / warps, it0 = min(items, self * run);
+    int left = (int)(min(items, it0 + run) - it0);
+    if (left <= 0) return;
+    int b = stream_of(pre, d.B, (int)(it0 / n_kv)), h, g, groups, cand, row;
+    auto enter = [&]() {
+        groups = pre[b + 1] - pre[b];
+        cand = candidates(b);
+        row = stream_row(d.c, d.seq_ids, b);
+    };
+    enter();
+    {
+        const int in_b = (int)(it0 - (long long)pre[b] * n_kv);
+        h = in_b / groups;
+        g = in_b % groups;
+    }
+    // physical pages of candidates g * 16 + r and 8 on, of the next item while this one is scored
+    auto pages = [&](int& lo, int& hi) {
+        const int p = g * 16 + r;
+        lo = p < cand ? stream_page(d.c, row, d.first + p) : 0;
+        hi = p + 8 < cand ? stream_page(d.c, row, d.first + p + 8) : 0;
+    };
+    int page_lo, page_hi;
+    pages(page_lo, page_hi);
     int have_b = -1, have_h = -1;
     uint32_t qf[16];
     float sq0 = 0.f, sq1 = 0.f;                                            // scale of query heads 2j, 2j+1; 0: no say
-    for (long long it = self * per; it < end; ++it) {
-        const int b = stream_of(pre, d.B, (int)(it / n_kv));
-        const int groups = pre[b + 1] - pre[b];
-        const long long in_b = it - (long long)pre[b] * n_kv;
-        const int h = (int)(in_b / groups), g = (int)(in_b % groups);
-        const int cand = candidates(b);
-        const int row = stream_row(d.c, d.seq_ids, b);
+    for (;; --left) {
         if (b != have_b || h != have_h) {
             have_b = b;
             have_h = h;
@@ -237,9 +384,6 @@ __global__ void __launch_bounds__(PS_THREADS, PS_CTAS) page_score_kernel(SelectD
             sq0 = __shfl_sync(0xffffffffu, sq, 8 * j);
             sq1 = __shfl_sync(0xffffffffu, sq, 8 * j + 4);
         }
-        const int p_lo = g * 16 + r, p_hi = p_lo + 8;                       // candidates behind the first pages
-        const int page_lo = p_lo < cand ? stream_page(d.c, row, d.first + p_lo) : 0;
-        const int page_hi = p_hi < cand ? stream_page(d.c, row, d.first + p_hi) : 0;
         const uint4* lo = reinterpret_cast<const uint4*>(d.bound_codes + ((size_t)page_lo * n_kv + h) * 256);
         const uint4* hi = reinterpret_cast<const uint4*>(d.bound_codes + ((size_t)page_hi * n_kv + h) * 256);
         uint4 wl[4], wh[4];
@@ -249,6 +393,20 @@ __global__ void __launch_bounds__(PS_THREADS, PS_CTAS) page_score_kernel(SelectD
             wh[i] = ld_stream_16(hi + j + 4 * i);
         }
         const float s_lo = __ldg(d.bound_scale + (size_t)page_lo * n_kv + h), s_hi = __ldg(d.bound_scale + (size_t)page_hi * n_kv + h);
+        const int p_lo = g * 16 + r, p_hi = p_lo + 8;                       // candidates behind the first pages
+        uint32_t* to = d.keys + ((size_t)b * n_kv + h) * d.c.max_pages;
+        const int cand_now = cand;
+        if (left > 1) {
+            if (++g == groups) {
+                g = 0;
+                if (++h == n_kv) {
+                    h = 0;
+                    do ++b; while (pre[b + 1] == pre[b]);
+                    enter();
+                }
+            }
+            pages(page_lo, page_hi);
+        }
         int acc[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -271,23 +429,28 @@ __global__ void __launch_bounds__(PS_THREADS, PS_CTAS) page_score_kernel(SelectD
             return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
         };
         if (j == 0) {
-            uint32_t* to = d.keys + ((size_t)b * n_kv + h) * d.c.max_pages;
-            if (p_lo < cand) to[p_lo] = key(t_lo);
-            if (p_hi < cand) to[p_hi] = key(t_hi);
+            if (p_lo < cand_now) to[p_lo] = key(t_lo);
+            if (p_hi < cand_now) to[p_hi] = key(t_hi);
         }
+        if (left == 1) return;
     }
 }
 
 // ---- selection ------------------------------------------------------------------------------------------------
 constexpr int SL_THREADS = 512;
+constexpr int SL_LOG_BINS = 11, SL_BINS = 1 << SL_LOG_BINS;
 
-// One CTA per (stream, KV head): the want-th largest key by three rounds of counting (11, 11 and 10 bits), then the kept
-// pages in ascending order.  Keys are read once into shared memory.
+// One CTA per (stream, KV head): the want-th largest key, then the kept pages in ascending order.  Keys are read once into
+// shared memory.  The threshold: bins of equal width over the range that the keys really have (bins over the bits of the
+// key would put neighbouring exponents' keys on a few counters, one after the other), then the few keys of the bin that it
+// falls into are ranked against one another; a bin that holds too many is cut into bins again.
 __global__ void __launch_bounds__(SL_THREADS) page_select_kernel(SelectDev d) {
     extern __shared__ uint32_t keys[];
-    __shared__ int hist[2048];
+    __shared__ int hist[SL_BINS];
+    __shared__ uint32_t few[SL_THREADS];
+    __shared__ uint32_t warp_lo[SL_THREADS / 32], warp_hi[SL_THREADS / 32];
     __shared__ int warp_tot[2][SL_THREADS / 32];
-    __shared__ int pick[2];
+    __shared__ int pick[3];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n_kv = d.c.n_kv, b = blockIdx.x / n_kv, h = blockIdx.x % n_kv;
     dependency_release();
@@ -320,23 +483,39 @@ __global__ void __launch_bounds__(SL_THREADS) page_select_kernel(SelectDev d) {
     for (int i = tid; i < d.recent; i += SL_THREADS) put(d.first + want + i, n - d.recent + i);
     if (want == 0) return;
     const uint32_t* from = d.keys + (size_t)blockIdx.x * d.c.max_pages;
-    for (int i = tid; i < cand; i += SL_THREADS) keys[i] = __ldcg(from + i);
-    uint32_t prefix = 0, known = 0;
-    int left = want;                                                        // of the keys that agree with prefix on known
-#pragma unroll 1
-    for (int round = 0; round < 3; ++round) {
-        const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bins = round == 2 ? 1024 : 2048;
-        for (int i = tid; i < bins; i += SL_THREADS) hist[i] = 0;
-        __syncthreads();
+    uint32_t lo = 0xffffffffu, hi = 0u;
+    for (int i = tid; i < cand; i += SL_THREADS) {
+        const uint32_t k = __ldcg(from + i);
+        keys[i] = k;
+        lo = min(lo, k);
+        hi = max(hi, k);
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) warp_lo[warp] = lo, warp_hi[warp] = hi;
+    for (int i = tid; i < SL_BINS; i += SL_THREADS) hist[i] = 0;
+    __syncthreads();
+    lo = __reduce_min_sync(0xffffffffu, warp_lo[lane % (SL_THREADS / 32)]);
+    hi = __reduce_max_sync(0xffffffffu, warp_hi[lane % (SL_THREADS / 32)]);
+    int left = want;                        // of the keys in [lo, hi], from the top
+    uint32_t threshold;
+    for (;;) {
+        // bins of 2^shift keys over [lo, hi], the last one from the top
+        const int shift = max(0, 32 - __clz((int)((hi - lo) | 1u)) - SL_LOG_BINS);
         for (int i = tid; i < cand; i += SL_THREADS) {
             const uint32_t k = keys[i];
-            if ((k & known) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+            if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1);
         }
         __syncthreads();
-        // bins from the top: thread t owns bins - 1 - per t downwards
-        const int per = bins / SL_THREADS, top = bins - 1 - per * tid;
-        int sum = 0;
-        for (int i = 0; i < per; ++i) sum += hist[top - i];
+        // thread t owns bins per (t + 1) - 1 .. per t below the top
+        constexpr int per = SL_BINS / SL_THREADS;
+        const int top = SL_BINS - 1 - per * tid;
+        int c[per], sum = 0;
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            c[i] = hist[top - i];
+            sum += c[i];
+        }
         int inc = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -344,26 +523,61 @@ __global__ void __launch_bounds__(SL_THREADS) page_select_kernel(SelectDev d) {
             if (lane >= o) inc += x;
         }
         if (lane == 31) warp_tot[0][warp] = inc;
+        if (tid == 0) pick[2] = 0;
         __syncthreads();
         int before = inc - sum;
         for (int w = 0; w < warp; ++w) before += warp_tot[0][w];
         if (before < left && before + sum >= left) {
             int i = 0, run = before;
-            while (run + hist[top - i] < left) run += hist[top - i++];
+#pragma unroll
+            for (int k = 0; k < per - 1; ++k)
+                if (i == k && run + c[k] < left) run += c[k], ++i;
             pick[0] = top - i;
             pick[1] = left - run;
         }
+#pragma unroll
+        for (int i = 0; i < per; ++i) hist[top - i] = 0;
         __syncthreads();
-        prefix |= (uint32_t)pick[0] << shift;
-        known |= (uint32_t)(bins - 1) << shift;
         left = pick[1];
+        lo += (uint32_t)pick[0] << shift;
+        if (shift == 0) {
+            threshold = lo;                 // a bin is one key
+            break;
+        }
+        hi = min(hi, lo + ((1u << shift) - 1u));
+        for (int i = tid; i < cand; i += SL_THREADS) {
+            const uint32_t k = keys[i];
+            if (k >= lo && k <= hi) {
+                const int at = atomicAdd(&pick[2], 1);
+                if (at < SL_THREADS) few[at] = k;
+            }
+        }
+        __syncthreads();
+        const int m = pick[2];
+        if (m <= SL_THREADS) {
+            if (tid < m) {
+                const uint32_t mine = few[tid];
+                int above = 0, same = 0;
+                for (int i = 0; i < m; ++i) {
+                    above += few[i] > mine;
+                    same += few[i] == mine;
+                }
+                // (threads with equal keys write the same)
+                if (above < left && above + same >= left) pick[0] = (int)mine, pick[1] = left - above;
+            }
+            __syncthreads();
+            threshold = (uint32_t)pick[0];
+            left = pick[1];
+            break;
+        }
+        __syncthreads();
     }
     // thread t owns a run of candidates: those above the threshold, and the first `left` equal to it
-    const int per = (cand + SL_THREADS - 1) / SL_THREADS, lo = min(cand, tid * per), hi = min(cand, lo + per);
+    const int per = (cand + SL_THREADS - 1) / SL_THREADS, c0 = min(cand, tid * per), c1 = min(cand, c0 + per);
     int above = 0, equal = 0;
-    for (int i = lo; i < hi; ++i) {
-        above += keys[i] > prefix;
-        equal += keys[i] == prefix;
+    for (int i = c0; i < c1; ++i) {
+        above += keys[i] > threshold;
+        equal += keys[i] == threshold;
     }
     int ia = above, ie = equal;
 #pragma unroll
@@ -376,9 +590,9 @@ __global__ void __launch_bounds__(SL_THREADS) page_select_kernel(SelectDev d) {
     int at = ia - above, eq = ie - equal;
     for (int w = 0; w < warp; ++w) at += warp_tot[0][w], eq += warp_tot[1][w];
     at += min(eq, left);
-    for (int i = lo; i < hi; ++i) {
+    for (int i = c0; i < c1; ++i) {
         const uint32_t k = keys[i];
-        if (k < prefix || (k == prefix && eq++ >= left)) continue;
+        if (k < threshold || (k == threshold && eq++ >= left)) continue;
         put(d.first + at++, d.first + i);
     }
 }
@@ -422,8 +636,13 @@ extern "C" int pikv_page_bounds_update(const pikv_paged_cache* c, void* bound_co
         d.seq_len = seq_len + b0;
         const long long most = (long long)d.B * c->max_pages * c->n_kv;
         const int grid = (int)std::min<long long>((long long)sm_count() * PB_CTAS, (most + PB_THREADS / 32 - 1) / (PB_THREADS / 32));
-        if (c->bits == 8) launch_dependent(page_bounds_kernel<8>, grid, PB_THREADS, 0, static_cast<cudaStream_t>(stream), d);
-        else launch_dependent(page_bounds_kernel<4>, grid, PB_THREADS, 0, static_cast<cudaStream_t>(stream), d);
+        if (c->bits == 8) {
+            if (!allow_smem<page_bounds_kernel<8>>(PBGeom<8>::SMEM)) return check_launch("page_bounds smem attribute");
+            launch_dependent(page_bounds_kernel<8>, grid, PB_THREADS, PBGeom<8>::SMEM, static_cast<cudaStream_t>(stream), d);
+        } else {
+            if (!allow_smem<page_bounds_kernel<4>>(PBGeom<4>::SMEM)) return check_launch("page_bounds smem attribute");
+            launch_dependent(page_bounds_kernel<4>, grid, PB_THREADS, PBGeom<4>::SMEM, static_cast<cudaStream_t>(stream), d);
+        }
         count_launch(1);
     }
     return check_launch("page_bounds_kernel");
@@ -474,7 +693,9 @@ extern "C" int pikv_sparse_attn(const pikv_paged_cache* c, const pikv_sparse_par
         if (c->max_pages > pages) {                                          // else nothing can need a choice
             const long long items = (long long)d.B * c->n_kv * ((most + 15) / 16);
             const int grid = (int)std::min<long long>((long long)sm_count() * PS_CTAS, (items + PS_THREADS / 32 - 1) / (PS_THREADS / 32));
-            launch_dependent(page_score_kernel, grid, PS_THREADS, 0, st, d);
+            // A plain launch: CTAs of a dependent one come to the SMs that the kernel before leaves first, several to one, and
+            // each has its share of the list already (64 x 32768: 191 us a step against 125)
+            page_score_kernel<<<grid, PS_THREADS, 0, st>>>(d);
             count_launch(1);
         }
         const size_t smem = c->max_pages > pages ? (size_t)most * sizeof(uint32_t) : 0;
