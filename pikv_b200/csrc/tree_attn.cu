@@ -82,8 +82,9 @@ template <int BITS> struct TRSmem {
                          VRING = KRING + TR_K_AHEAD * TR_PAGES * PAGE,
                          MRING = VRING + TR_V_AHEAD * TR_PAGES * PAGE,         // [ahead of K][page] scales, zero points
                          SIDE = MRING + TR_K_AHEAD * TR_PAGES * META,          // 4 bit: [4][2][64] fp32: z of K, of V, of four tiles
-                         VEXP = SIDE + 4 * SIDES * TR_KEYS * 4,                // [4] of four tiles: e_k + 9, e_v + 9, rows of V that are not finite (a bit each)
-                         BARS = VEXP + 64, NBARS = 14 + 2 * (TR_K_AHEAD + TR_V_AHEAD),
+                         VEXP = SIDE + 4 * SIDES * TR_KEYS * 4,                // [4] of four tiles: 2^(e_k + 9), e_v + 9, 2^-(e_v + 9) as floats, whether a row of V is not finite
+                         ODD = VEXP + 64,                                       // [4][2] even and odd rows of V that are not finite, a bit each
+                         BARS = ODD + 32, NBARS = 14 + 2 * (TR_K_AHEAD + TR_V_AHEAD),
                          PRE = BARS + NBARS * 8, MISC = PRE + (PIKV_STREAMS_PER_LAUNCH + 1) * 4, END = MISC + 16;
     static constexpr int BYTES = END + 1024;
 };
@@ -551,7 +552,11 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     va1_next = __uint_as_float(finite(scale(r0 + 8, 1))) * up_v;
                     // The four sets need no wait of their own: the one written here served tile j - 4, whose second product was
                     // issued before the Q K^T of tile j - 2, and this warp has seen that one done
-                    if (w == 0 && lane == 0) *reinterpret_cast<int4*>(smem + SM::VEXP + (j & 3) * 16) = make_int4(ke + 9, ve + 9, (int)odd0, (int)odd1);
+                    if (w == 0 && lane == 0) {
+                        *reinterpret_cast<float4*>(smem + SM::VEXP + (j & 3) * 16) =
+                            make_float4(exp2_int(ke + 9), (float)(ve + 9), exp2_int(-9 - ve), __uint_as_float(odd0 | odd1));
+                        *reinterpret_cast<uint2*>(smem + SM::ODD + (j & 3) * 8) = make_uint2(odd0, odd1);
+                    }
                     if (BITS == 4) {
                         // lanes 0-15: z of K, 16-31: of V
                         const int side = lane >> 4, r = lane & 15;
@@ -595,192 +600,193 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             int node = 0;
             bool live = false, warp_live = false;
             size_t out_row = 0;
-            for (int n = 0, f = f0; f < f1; ++f, ++n) {
-                const bool first = n == 0 || cur.tile == 0;
-                if (TR_RARE(first)) {
-                    // ---- this row's query ----
-                    const int row = cur.row_tile * TR_ROWS + tid, h = cur.head;
-                    node = row / d.G;
-                    live = node < cur.nodes;
-                    warp_live = __any_sync(0xffffffffu, live);
-                    ref = -INFINITY;
-                    den = corr = odd_v = 0.f;
-                    if (warp_live) {
-                        out_row = ((size_t)cur.b * d.N + (live ? node : 0)) * d.n_q + (size_t)h * d.G + row % d.G;
-                        const uint4* src = reinterpret_cast<const uint4*>(d.q + out_row * 128);
-                        float amax = 0.f, odd = 0.f;
-#pragma unroll 4
-                        for (int i = 0; i < 16; ++i) {
-                            const uint4 w4 = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-                            const uint32_t ww[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                float x, y;
-                                bf16x2_to_f32(ww[k], x, y);
-                                amax = fmaxf(amax, fmaxf(fabsf(x), fabsf(y)));
-                                odd += x * 0.f + y * 0.f;             // NaN where the row is not finite
-                            }
-                        }
-                        const int sh = amax > 0.f && amax < INFINITY ? min(126, 14 - ((int)(__float_as_uint(amax) >> 23) - 127)) : 0;
-                        const float up = exp2_int(max(sh, -126));
-                        qsum = 0.f;
-#pragma unroll 4
-                        for (int i = 0; i < 16; ++i) {
-                            const uint4 w4 = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-                            float x[8];
-                            bf16x2_to_f32(w4.x, x[0], x[1]);
-                            bf16x2_to_f32(w4.y, x[2], x[3]);
-                            bf16x2_to_f32(w4.z, x[4], x[5]);
-                            bf16x2_to_f32(w4.w, x[6], x[7]);
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                x[k] *= up;
-                                qsum += x[k];
-                            }
-                            uint4 y;
-                            y.x = tr_pack(x[tr_channel<BITS>(0)], x[tr_channel<BITS>(1)]);
-                            y.y = tr_pack(x[tr_channel<BITS>(2)], x[tr_channel<BITS>(3)]);
-                            y.z = tr_pack(x[tr_channel<BITS>(4)], x[tr_channel<BITS>(5)]);
-                            y.w = tr_pack(x[tr_channel<BITS>(6)], x[tr_channel<BITS>(7)]);
-                            *reinterpret_cast<uint4*>(smem + SM::Q + (i >> 3) * TR_ROWS * 128 + tid * 128 + 16 * ((i & 7) ^ (tid & 7))) = y;
-                        }
-                        qmul = exp2_int(-max(sh, -126)) * (0.08838834764831845f * 1.4426950408889634f) + odd;
-                        // what this node sees of the tree, a bit per node
-                        tree = 0;
-                        if (live) {
-                            const uint8_t* m = d.mask + (size_t)cur.b * d.mask_stride + (size_t)node * d.N;
-                            for (int i = 0; i < cur.nodes; ++i) tree |= (uint64_t)(__ldg(m + i) != 0) << i;
-                        }
-                        tr_fence_smem();
-                    }
-                    __syncwarp();
-                    if (lane == 0) lr_mbar_arrive(q_full);
+            // one tile: scores out, weights in.  EDGE: some of its positions lie behind the context
+            auto step = [&](auto edge_c, int n, int tile, bool first) {
+                constexpr bool EDGE = decltype(edge_c)::value;
+                if (TR_RARE(!tr_wait2(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u, side_full + 8 * (n & 3), (uint32_t)(n >> 2) & 1u))) return false;
+                if (!warp_live) {
+                    if (lane == 0) lr_mbar_arrive(p_full + 8 * (n & 1));
+                    return true;
                 }
-                if (TR_RARE(!tr_wait2(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u, side_full + 8 * (n & 3), (uint32_t)(n >> 2) & 1u))) { failed = true; break; }
-                const bool last = f + 1 == f1 || cur.tile + 1 == cur.tiles;
+                tr_fence_after();
+                const uint32_t scores = tmem + lanes + TR_COL_S + TR_KEYS * (n & 1);
+                float x0[32], x1[32];
+                tr_tmem_ld32(scores, x0);
+                tr_tmem_ld32(scores + 32, x1);
+                const float* kz = reinterpret_cast<const float*>(smem + SM::SIDE) + (n & 3) * SM::SIDES * TR_KEYS;      // 4 bit only
+                const float* vz = kz + TR_KEYS;
+                const float4 of = *reinterpret_cast<const float4*>(smem + SM::VEXP + (n & 3) * 16);
+                float mul = qmul * of.x;
+                if (mul == 0.f) mul = 1.17549435e-38f;                   // (masked scores are -infinity: times 0 they would not be a number)
+                uint64_t seen = ~0ull;
+                if (EDGE) {
+                    // the positions behind the context show only where the mask opens them
+                    const int sh = cur.ctx - tile * TR_KEYS;             // the tree's first bit
+                    seen = sh >= 0 ? (sh < 64 ? tree << sh : 0ull) | (sh < 64 ? (1ull << sh) - 1 : ~0ull) : (sh > -64 ? tree >> -sh : 0ull);
+                }
+                if (TR_RARE(__float_as_uint(of.w) != 0u)) {
+                    const uint2 odd = *reinterpret_cast<const uint2*>(smem + SM::ODD + (n & 3) * 8);
+                    for (int j = 0; j < TR_KEYS; ++j)
+                        if (((j & 1 ? odd.y : odd.x) >> (j >> 1)) & (uint32_t)(seen >> j) & 1u) odd_v = __uint_as_float(0x7fffffffu);
+                }
+                tr_tmem_ld_wait(x0);
+                tr_tmem_ld_wait(x1);
+                const float mx = fmaxf(tr_scores<BITS, EDGE>(x0, kz, qsum, (uint32_t)seen), tr_scores<BITS, EDGE>(x1, kz + 32, qsum, (uint32_t)(seen >> 32)));
+                // does the reference hold?  (-inf while nothing has been seen)
+                const float want = mx * mul + of.y;
+                const bool move = mx > -INFINITY && want > ref + TR_SLACK;
+                if (TR_RARE(__any_sync(0xffffffffu, move))) {
+                    const float next = move ? want : ref;
+                    const float fac = move ? tr_ex2(ref - next) : 1.f;     // 0 from -inf
+                    ref = next;
+                    den *= fac;
+                    corr *= fac;
+                    if (!first) {
+                        if (TR_RARE(!tr_wait(pv_done + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) return false;
+                        tr_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < 128; c += 16) {             // few registers: the scores are in the others
+                            float o[16];
+                            lr_tmem_ld16(tmem + lanes + TR_COL_O + c, o);
+                            uint32_t r[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(o[i] * fac);
+                            tr_tmem_st16(tmem + lanes + TR_COL_O + c, r);
+                        }
+                        tr_tmem_st_wait();
+                    }
+                }
+                const float off = of.y - (ref == -INFINITY ? 0.f : ref);
+                float total = 0.f;
+                // the weights take the place of the scores that they come from, two to a column
+                uint32_t wgt[16];
+                tr_weights<BITS, EDGE>(x0, wgt, vz, mul, off, (uint32_t)seen, total, corr);
+                tr_tmem_st16(scores, wgt);
+                tr_weights<BITS, EDGE>(x1, wgt, vz + 32, mul, off, (uint32_t)(seen >> 32), total, corr);
+                tr_tmem_st16(scores + 16, wgt);
+                den += total * of.z;
+                tr_tmem_st_wait();
+                tr_fence_before();
+                __syncwarp();
+                if (lane == 0) lr_mbar_arrive(p_full + 8 * (n & 1));
+                return true;
+            };
+            for (int n = 0, f = f0; f < f1;) {
+                // ---- a unit, or the part of it that this CTA has: tiles t0 .. t1 - 1 ----
+                const int t0 = cur.tile, t1 = min(cur.tiles, t0 + f1 - f), edge = max(t0, min(t1, cur.ctx / TR_KEYS));
+                // ---- this row's query ----
+                const int row = cur.row_tile * TR_ROWS + tid, h = cur.head;
+                node = row / d.G;
+                live = node < cur.nodes;
+                warp_live = __any_sync(0xffffffffu, live);
+                ref = -INFINITY;
+                den = corr = odd_v = 0.f;
+                if (warp_live) {
+                    out_row = ((size_t)cur.b * d.N + (live ? node : 0)) * d.n_q + (size_t)h * d.G + row % d.G;
+                    const uint4* src = reinterpret_cast<const uint4*>(d.q + out_row * 128);
+                    // what a node sees of the tree, a bit per node: the warp reads the mask rows of its nodes together
+                    const int node0 = __shfl_sync(0xffffffffu, node, 0), node1 = min(__shfl_sync(0xffffffffu, node, 31), cur.nodes - 1);
+                    const uint8_t* masks = d.mask + (size_t)cur.b * d.mask_stride;
+                    tree = 0;
+#pragma unroll 4
+                    for (int i = node0; i <= node1; ++i) {
+                        const bool lo = lane < cur.nodes && __ldg(masks + (size_t)i * d.N + lane) != 0;
+                        const bool hi = lane + 32 < cur.nodes && __ldg(masks + (size_t)i * d.N + lane + 32) != 0;
+                        const uint32_t m0 = __ballot_sync(0xffffffffu, lo), m1 = __ballot_sync(0xffffffffu, hi);
+                        if (node == i) tree = (uint64_t)m1 << 32 | m0;
+                    }
+                    float amax = 0.f, odd = 0.f;
+#pragma unroll 8
+                    for (int i = 0; i < 16; ++i) {
+                        const uint4 q4 = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+                        const uint32_t ww[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float x, y;
+                            bf16x2_to_f32(ww[k], x, y);
+                            amax = fmaxf(amax, fmaxf(fabsf(x), fabsf(y)));
+                            odd += x * 0.f + y * 0.f;                 // NaN where the row is not finite
+                        }
+                    }
+                    const int sh = amax > 0.f && amax < INFINITY ? min(126, 14 - ((int)(__float_as_uint(amax) >> 23) - 127)) : 0;
+                    const float up = exp2_int(max(sh, -126));
+                    qsum = 0.f;
+#pragma unroll 4
+                    for (int i = 0; i < 16; ++i) {
+                        const uint4 q4 = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+                        float x[8];
+                        bf16x2_to_f32(q4.x, x[0], x[1]);
+                        bf16x2_to_f32(q4.y, x[2], x[3]);
+                        bf16x2_to_f32(q4.z, x[4], x[5]);
+                        bf16x2_to_f32(q4.w, x[6], x[7]);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            x[k] *= up;
+                            if (BITS == 4) qsum += x[k];
+                        }
+                        uint4 y;
+                        y.x = tr_pack(x[tr_channel<BITS>(0)], x[tr_channel<BITS>(1)]);
+                        y.y = tr_pack(x[tr_channel<BITS>(2)], x[tr_channel<BITS>(3)]);
+                        y.z = tr_pack(x[tr_channel<BITS>(4)], x[tr_channel<BITS>(5)]);
+                        y.w = tr_pack(x[tr_channel<BITS>(6)], x[tr_channel<BITS>(7)]);
+                        *reinterpret_cast<uint4*>(smem + SM::Q + (i >> 3) * TR_ROWS * 128 + tid * 128 + 16 * ((i & 7) ^ (tid & 7))) = y;
+                    }
+                    qmul = exp2_int(-max(sh, -126)) * (0.08838834764831845f * 1.4426950408889634f) + odd;
+                    tr_fence_smem();
+                }
+                __syncwarp();
+                if (lane == 0) lr_mbar_arrive(q_full);
+                for (int t = t0; t < edge && !failed; ++t, ++n) failed = !step(std::false_type{}, n, t, t == t0);
+                for (int t = edge; t < t1 && !failed; ++t, ++n) failed = !step(std::true_type{}, n, t, t == t0);
+                if (failed) break;
+                // ---- this CTA's share of the unit is done ----
+                if (TR_RARE(!tr_wait(pv_done + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) { failed = true; break; }
                 if (warp_live) {
                     tr_fence_after();
-                    const uint32_t scores = tmem + lanes + TR_COL_S + TR_KEYS * (n & 1);
-                    float x0[32], x1[32];
-                    tr_tmem_ld32(scores, x0);
-                    tr_tmem_ld32(scores + 32, x1);
-                    const float* kz = reinterpret_cast<const float*>(smem + SM::SIDE) + (n & 3) * SM::SIDES * TR_KEYS;      // 4 bit only
-                    const float* vz = kz + TR_KEYS;
-                    const int4 of = *reinterpret_cast<const int4*>(smem + SM::VEXP + (n & 3) * 16);
-                    float mul = qmul * exp2_int(of.x);
-                    if (mul == 0.f) mul = 1.17549435e-38f;               // (masked scores are -infinity: times 0 they would not be a number)
-                    const int pos0 = cur.tile * TR_KEYS;
-                    uint64_t seen = ~0ull;
-                    const bool edge = pos0 + TR_KEYS > cur.ctx;          // the same for the whole CTA
-                    if (TR_RARE(edge)) {
-                        // the positions behind the context show only where the mask opens them
-                        const int sh = cur.ctx - pos0;                   // the tree's first bit
-                        seen = sh >= 0 ? (sh < 64 ? tree << sh : 0ull) | ((1ull << sh) - 1) : (sh > -64 ? tree >> -sh : 0ull);
-                    }
-                    if (TR_RARE(of.z | of.w)) {                                   // (their bits: even rows in one word, odd ones in the other)
-                        for (int j = 0; j < TR_KEYS; ++j)
-                            if (((j & 1 ? of.w : of.z) >> (j >> 1)) & (int)(seen >> j) & 1) odd_v = __uint_as_float(0x7fffffffu);
-                    }
-                    tr_tmem_ld_wait(x0);
-                    tr_tmem_ld_wait(x1);
-                    float mx;
-                    if (TR_RARE(edge)) mx = fmaxf(tr_scores<BITS, true>(x0, kz, qsum, (uint32_t)seen), tr_scores<BITS, true>(x1, kz + 32, qsum, (uint32_t)(seen >> 32)));
-                    else mx = fmaxf(tr_scores<BITS, false>(x0, kz, qsum, ~0u), tr_scores<BITS, false>(x1, kz + 32, qsum, ~0u));
-                    // does the reference hold?  (-inf while nothing has been seen)
-                    const float want = mx * mul + (float)of.y;
-                    const bool move = mx > -INFINITY && want > ref + TR_SLACK;
-                    if (TR_RARE(__any_sync(0xffffffffu, move))) {
-                        const float next = move ? want : ref;
-                        const float fac = move ? tr_ex2(ref - next) : 1.f;     // 0 from -inf
-                        ref = next;
-                        den *= fac;
-                        corr *= fac;
-                        if (!first) {
-                            if (TR_RARE(!tr_wait(pv_done + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) { failed = true; break; }
-                            tr_fence_after();
+                    const bool begun = t0 == 0;                          // here, and not by the CTA before
+                    const bool whole = begun && t1 == cur.tiles;
+                    const float inv = den == 0.f ? 0.f : 1.f / den;
+                    const size_t slot = (size_t)(2 * blockIdx.x + (begun ? 1 : 0)) * parts.rows + tid;
 #pragma unroll 1
-                            for (int c = 0; c < 128; c += 16) {             // few registers: the scores are in the others
-                                float o[16];
-                                lr_tmem_ld16(tmem + lanes + TR_COL_O + c, o);
-                                uint32_t r[16];
+                    for (int c = 0; c < 128; c += 32) {
+                        float o[32];
+                        tr_tmem_ld32(tmem + lanes + TR_COL_O + c, o);
+                        tr_tmem_ld_wait(o);
+                        if (BITS == 4) {
+                            float t[32];
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(o[i] * fac);
-                                tr_tmem_st16(tmem + lanes + TR_COL_O + c, r);
-                            }
-                            tr_tmem_st_wait();
+                            for (int i = 0; i < 32; ++i) t[tr_channel<BITS>(i)] = o[i] - corr;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = t[i];
                         }
-                    }
-                    const float off = (float)of.y - (ref == -INFINITY ? 0.f : ref);
-                    float total = 0.f;
-                    // the weights take the place of the scores that they come from, two to a column
-                    {
-                        uint32_t wgt[16];
-                        if (TR_RARE(edge)) tr_weights<BITS, true>(x0, wgt, vz, mul, off, (uint32_t)seen, total, corr);
-                        else tr_weights<BITS, false>(x0, wgt, vz, mul, off, ~0u, total, corr);
-                        tr_tmem_st16(scores, wgt);
-                    }
-                    {
-                        uint32_t wgt[16];
-                        if (TR_RARE(edge)) tr_weights<BITS, true>(x1, wgt, vz + 32, mul, off, (uint32_t)(seen >> 32), total, corr);
-                        else tr_weights<BITS, false>(x1, wgt, vz + 32, mul, off, ~0u, total, corr);
-                        tr_tmem_st16(scores + 16, wgt);
-                    }
-                    den += total * exp2_int(-of.y);
-                    tr_tmem_st_wait();
-                    tr_fence_before();
-                    __syncwarp();
-                    if (lane == 0) lr_mbar_arrive(p_full + 8 * (n & 1));
-                } else if (lane == 0) {
-                    lr_mbar_arrive(p_full + 8 * (n & 1));
-                }
-                if (TR_RARE(last)) {
-                    // ---- this CTA's share of the unit is done ----
-                    if (TR_RARE(!tr_wait(pv_done + 8 * (n & 1), (uint32_t)(n >> 1) & 1u))) { failed = true; break; }
-                    if (warp_live) {
-                        tr_fence_after();
-                        const int begun = f - cur.tile;                  // place of the unit's first tile
-                        const bool whole = begun >= f0 && cur.tile + 1 == cur.tiles;
-                        const float inv = den == 0.f ? 0.f : 1.f / den;
-                        const size_t slot = (size_t)(2 * blockIdx.x + (begun >= f0 ? 1 : 0)) * parts.rows + tid;
-#pragma unroll 1
-                        for (int c = 0; c < 128; c += 32) {
-                            float o[32];
-                            tr_tmem_ld32(tmem + lanes + TR_COL_O + c, o);
-                            tr_tmem_ld_wait(o);
-                            if (BITS == 4) {
-                                float t[32];
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) t[tr_channel<BITS>(i)] = o[i] - corr;
+                        for (int i = 0; i < 32; ++i) o[i] += odd_v;
+                        if (live && whole) {
+                            uint4* to = reinterpret_cast<uint4*>(d.out + out_row * 128 + c);
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = t[i];
-                            }
+                            for (int i = 0; i < 4; ++i) {
+                                uint32_t r[4];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] += odd_v;
-                            if (live && whole) {
-                                uint4* to = reinterpret_cast<uint4*>(d.out + out_row * 128 + c);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    uint32_t r[4];
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k) {
-                                        const __nv_bfloat162 h2 = __floats2bfloat162_rn(den == 0.f ? 0.f : o[8 * i + 2 * k] * inv, den == 0.f ? 0.f : o[8 * i + 2 * k + 1] * inv);
-                                        r[k] = *reinterpret_cast<const uint32_t*>(&h2);
-                                    }
-                                    to[i] = make_uint4(r[0], r[1], r[2], r[3]);
+                                for (int k = 0; k < 4; ++k) {
+                                    const __nv_bfloat162 h2 = __floats2bfloat162_rn(den == 0.f ? 0.f : o[8 * i + 2 * k] * inv, den == 0.f ? 0.f : o[8 * i + 2 * k + 1] * inv);
+                                    r[k] = *reinterpret_cast<const uint32_t*>(&h2);
                                 }
-                            } else if (live) {
-                                float4* to = reinterpret_cast<float4*>(parts.o + slot * 128 + c);
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                                to[i] = make_uint4(r[0], r[1], r[2], r[3]);
                             }
-                            __syncwarp();
+                        } else if (live) {
+                            float4* to = reinterpret_cast<float4*>(parts.o + slot * 128 + c);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                         }
-                        if (live && whole && d.lse) d.lse[out_row] = den == 0.f ? -INFINITY : ref * 0.6931471805599453f + logf(den);
-                        if (live && !whole) parts.ml[slot] = make_float2(ref, den);
-                        tr_fence_before();
+                        __syncwarp();
                     }
+                    if (live && whole && d.lse) d.lse[out_row] = den == 0.f ? -INFINITY : ref * 0.6931471805599453f + logf(den);
+                    if (live && !whole) parts.ml[slot] = make_float2(ref, den);
+                    tr_fence_before();
                 }
-                if (f + 1 < f1) cur.next(d, pre, f + 1);
+                f += t1 - t0;
+                cur.tile = t1 - 1;
+                if (f < f1) cur.next(d, pre, f);
             }
         }
         if (failed && lane == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_WAIT_TIMEOUT);
