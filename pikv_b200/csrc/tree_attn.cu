@@ -44,7 +44,7 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // A CTA's warps:
 //   0-3  softmax: thread = row.  S comes out of tensor memory, the weights go back into it as the A operand of the second
 //        product; a row's maximum, denominator and the rescaling of its O live in its thread
-//   4-7  one page of every tile each: codes to f16 (exact integers), into the swizzled layout that both products read
+//   4-5, 6-7  two pages of every tile each: codes of K, of V, to f16, into the swizzled layout that both products read
 //   8    issues the MMAs: Q K^T of tile n + 1 before P V of tile n, so that the products of one tile run while the softmax
 //        of another does
 //   9    bulk copies of pages into two rings, K three tiles ahead and V two
@@ -60,7 +60,7 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // the fp32 sum of 2^(logit - R).  A row of V that is not finite enters as zeros and makes the result of the rows that see it
 // not a number; one that a row does not see does not reach it.
 constexpr int TR_THREADS = 384;          // three warpgroups: warps 10 and 11 only complete the last
-constexpr int TR_CONVERT = 4, TR_MMA = 8, TR_COPY = 9;      // first converting warp, and the two single ones
+constexpr int TR_K = 4, TR_V = 6, TR_MMA = 8, TR_COPY = 9;      // first converting warps of K and of V, and the two single ones
 constexpr int TR_ROWS = 128;             // rows of a unit
 constexpr int TR_KEYS = 64;              // keys of a tile
 constexpr int TR_PAGES = TR_KEYS / PIKV_PAGE_TOKENS;
@@ -76,12 +76,13 @@ constexpr int TR_K_AHEAD = 3, TR_V_AHEAD = 2;                                   
 // shared memory behind a 1024-byte boundary
 template <int BITS> struct TRSmem {
     static constexpr int SIDES = BITS == 8 ? 0 : 2;
-    static constexpr int PAGE = 256 * BITS, META = BITS == 8 ? 64 : 192;       // codes of a page of one head; scales (and zero points) of K and V
+    static constexpr int PAGE = 256 * BITS, META = BITS == 8 ? 32 : 96;        // codes of a page of one head; its scales (and zero points)
     static constexpr int Q = 0, K = Q + 2 * TR_ROWS * 128, V = K + TR_TILE,
                          KRING = V + TR_TILE,                                  // [ahead][page of the tile] codes of K
                          VRING = KRING + TR_K_AHEAD * TR_PAGES * PAGE,
-                         MRING = VRING + TR_V_AHEAD * TR_PAGES * PAGE,         // [ahead of K][page] scales, zero points
-                         SIDE = MRING + TR_K_AHEAD * TR_PAGES * META,          // 4 bit: [4][2][64] fp32: z of K, of V, of four tiles
+                         KMETA = VRING + TR_V_AHEAD * TR_PAGES * PAGE,         // [ahead][page] scales, zero points of K, of V
+                         VMETA = KMETA + TR_K_AHEAD * TR_PAGES * META,
+                         SIDE = VMETA + TR_V_AHEAD * TR_PAGES * META,          // 4 bit: [4][2][64] fp32: z of K, of V, of four tiles
                          VEXP = SIDE + 4 * SIDES * TR_KEYS * 4,                // [4] of four tiles: 2^(e_k + 9), e_v + 9, 2^-(e_v + 9) as floats, whether a row of V is not finite
                          ODD = VEXP + 64,                                       // [4][2] even and odd rows of V that are not finite, a bit each
                          BARS = ODD + 32, NBARS = 14 + 2 * (TR_K_AHEAD + TR_V_AHEAD),
@@ -369,13 +370,13 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                    kr_full = bars + 112, kr_empty = kr_full + 8 * TR_K_AHEAD, vr_full = kr_empty + 8 * TR_K_AHEAD, vr_empty = vr_full + 8 * TR_V_AHEAD;
     dependency_release();
     if (tid == 0) {
-        lr_mbar_init(k_full, 4);
-        lr_mbar_init(v_full, 4);
+        lr_mbar_init(k_full, 2);
+        lr_mbar_init(v_full, 2);
         lr_mbar_init(q_full, 4);
         for (int i = 0; i < 2; ++i) lr_mbar_init(s_full + 8 * i, 1), lr_mbar_init(p_full + 8 * i, 4), lr_mbar_init(pv_done + 8 * i, 1);
         for (int i = 0; i < 4; ++i) lr_mbar_init(side_full + 8 * i, 4);
-        for (int i = 0; i < TR_K_AHEAD; ++i) lr_mbar_init(kr_full + 8 * i, 1), lr_mbar_init(kr_empty + 8 * i, 4);
-        for (int i = 0; i < TR_V_AHEAD; ++i) lr_mbar_init(vr_full + 8 * i, 1), lr_mbar_init(vr_empty + 8 * i, 4);
+        for (int i = 0; i < TR_K_AHEAD; ++i) lr_mbar_init(kr_full + 8 * i, 1), lr_mbar_init(kr_empty + 8 * i, 2);
+        for (int i = 0; i < TR_V_AHEAD; ++i) lr_mbar_init(vr_full + 8 * i, 1), lr_mbar_init(vr_empty + 8 * i, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // keys behind a stream's last page keep what was in the tile: weights of 0 times something finite
@@ -488,106 +489,99 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                         if (lane == 0) lr_mbar_expect_tx(bar, (uint32_t)np * (SM::PAGE + SM::META));
                         __syncwarp();
                         if (lane < np) {
-                            const uint32_t dst = sbase + SM::MRING + (ks * TR_PAGES + i) * SM::META;
+                            const uint32_t dst = sbase + SM::KMETA + (ks * TR_PAGES + i) * SM::META;
                             tr_bulk(sbase + SM::KRING + (ks * TR_PAGES + i) * SM::PAGE, d.c.k_codes + (size_t)unit * SM::PAGE, SM::PAGE, bar);
                             tr_bulk(dst, d.c.k_scale + (size_t)unit * 16, 32, bar);
-                            tr_bulk(dst + 32, d.c.v_scale + (size_t)unit * 16, 32, bar);
-                            if (BITS == 4) {
-                                tr_bulk(dst + 64, d.c.k_zp + (size_t)unit * 16, 64, bar);
-                                tr_bulk(dst + 128, d.c.v_zp + (size_t)unit * 16, 64, bar);
-                            }
+                            if (BITS == 4) tr_bulk(dst + 32, d.c.k_zp + (size_t)unit * 16, 64, bar);
                         }
                         if (++ks == TR_K_AHEAD) ks = 0, kph ^= 1u;
                         if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
                     }
                     if (n == 0) continue;
                     if (TR_RARE(!tr_wait(vr_empty + 8 * vs, vph))) { failed = true; break; }
-                    if (lane == 4) lr_mbar_expect_tx(vr_full + 8 * vs, (uint32_t)v_np * SM::PAGE);
+                    const uint32_t bar = vr_full + 8 * vs;
+                    if (lane == 4) lr_mbar_expect_tx(bar, (uint32_t)v_np * (SM::PAGE + SM::META));
                     __syncwarp();
-                    if (lane >= 4 && lane < 4 + v_np)
-                        tr_bulk(sbase + SM::VRING + (vs * TR_PAGES + i) * SM::PAGE, d.c.v_codes + (size_t)v_unit * SM::PAGE, SM::PAGE, vr_full + 8 * vs);
+                    if (lane >= 4 && lane < 4 + v_np) {
+                        const uint32_t dst = sbase + SM::VMETA + (vs * TR_PAGES + i) * SM::META;
+                        tr_bulk(sbase + SM::VRING + (vs * TR_PAGES + i) * SM::PAGE, d.c.v_codes + (size_t)v_unit * SM::PAGE, SM::PAGE, bar);
+                        tr_bulk(dst, d.c.v_scale + (size_t)v_unit * 16, 32, bar);
+                        if (BITS == 4) tr_bulk(dst + 32, d.c.v_zp + (size_t)v_unit * 16, 64, bar);
+                    }
                     if (++vs == TR_V_AHEAD) vs = 0, vph ^= 1u;
                 }
                 // copies that a warp which gave up no longer waits for land before this CTA's shared memory goes to another
                 for (int k = 0; k < TR_K_AHEAD; ++k) (void)tr_wait(kr_full + 8 * k, k < ks ? kph ^ 1u : kph);
                 for (int k = 0; k < TR_V_AHEAD; ++k) (void)tr_wait(vr_full + 8 * k, k < vs ? vph ^ 1u : vph);
             }
-        } else if (warp >= TR_CONVERT) {
+        } else if (warp >= TR_K) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
             cur.start(d, pre, f0);
-            // ---- codes to f16: warp w takes page w of every tile, the K of tile m + 1 before the V of tile m ----
-            const int w = warp - TR_CONVERT, count = f1 - f0;
-            const int at = tr_place<BITS>(lane);
-            int ks = 0, vs = 0, rows = 0;                             // stages; rows of page w that are inside the stream, of the tile whose K went last
-            uint32_t kph = 0, vph = 0;
-            float va0_next = 0.f, va1_next = 0.f;                     // factors of the V of the tile whose K went last
-            for (int m = -1; m < count; ++m) {
-                const int j = m + 1, v_rows = rows;
-                const float va0 = va0_next, va1 = va1_next;
-                if (j < count) {
-                    if (j > 0) cur.next(d, pre, f0 + j);
-                    rows = max(0, min(PIKV_PAGE_TOKENS, cur.end() - (cur.tile * TR_PAGES + w) * PIKV_PAGE_TOKENS));
-                    if (TR_RARE(!tr_wait(kr_full + 8 * ks, kph))) { failed = true; break; }
-                    TRPage<BITS> x;
-                    if (rows > 0) x.load(smem + SM::KRING + (ks * TR_PAGES + w) * SM::PAGE, at);
-                    // the tile's exponents: lane = two neighbouring rows of page lane / 8, scales of K in one word, of V in another; rows
-                    // behind the end have none
-                    const unsigned char* metas = smem + SM::MRING + ks * TR_PAGES * SM::META;
-                    const unsigned char* pair = metas + (lane >> 3) * SM::META + (lane & 7) * 4;
-                    const int left = cur.end() - cur.tile * TR_KEYS - 2 * lane;       // rows from the pair's first on
-                    uint32_t k2 = left > 0 ? *reinterpret_cast<const uint32_t*>(pair) : 0u, v2 = left > 0 ? *reinterpret_cast<const uint32_t*>(pair + 32) : 0u;
-                    if (left == 1) k2 &= 0xffffu, v2 &= 0xffffu;
-                    const int ke = __reduce_max_sync(0xffffffffu, max(tr_exponent(k2 << 16), tr_exponent(k2 & 0xffff0000u)));
-                    const int ve = __reduce_max_sync(0xffffffffu, max(tr_exponent(v2 << 16), tr_exponent(v2 & 0xffff0000u)));
-                    // rows of V that are not finite
-                    const uint32_t odd0 = __ballot_sync(0xffffffffu, (v2 & 0x7f80u) == 0x7f80u), odd1 = __ballot_sync(0xffffffffu, (v2 & 0x7f800000u) == 0x7f800000u);
-                    // this warp's rows: tr_row(lane) and 8 on
-                    const unsigned char* meta = metas + w * SM::META;
-                    const int r0 = tr_row(lane);
-                    auto scale = [&](int r, int side) { return r < rows ? (uint32_t)reinterpret_cast<const uint16_t*>(meta + 32 * side)[r] << 16 : 0u; };
-                    const float up_k = exp2_int(15 - ke), up_v = exp2_int(15 - ve);
-                    const float ka0 = __uint_as_float(scale(r0, 0)) * up_k, ka1 = __uint_as_float(scale(r0 + 8, 0)) * up_k;
-                    auto finite = [](uint32_t s) { return (s & 0x7f800000u) == 0x7f800000u ? 0u : s; };
-                    va0_next = __uint_as_float(finite(scale(r0, 1))) * up_v;
-                    va1_next = __uint_as_float(finite(scale(r0 + 8, 1))) * up_v;
-                    // The four sets need no wait of their own: the one written here served tile j - 4, whose second product was
-                    // issued before the Q K^T of tile j - 2, and this warp has seen that one done
+            // ---- codes to f16: warp w of the two of K, of V, takes pages 2 w and 2 w + 1 of every tile ----
+            const bool of_v = warp >= TR_V;
+            const int w = (warp - TR_K) & 1, count = f1 - f0, ahead = of_v ? TR_V_AHEAD : TR_K_AHEAD;
+            const int at = tr_place<BITS>(lane), r0 = tr_row(lane);
+            const unsigned char* ring = smem + (of_v ? SM::VRING : SM::KRING);
+            const unsigned char* metas = smem + (of_v ? SM::VMETA : SM::KMETA);
+            unsigned char* tile = smem + (of_v ? SM::V : SM::K);
+            const uint32_t full = of_v ? vr_full : kr_full, empty = of_v ? vr_empty : kr_empty, read = of_v ? pv_done : s_full, ready = of_v ? v_full : k_full;
+            int s = 0;
+            uint32_t ph = 0;
+            for (int n = 0; n < count; ++n) {
+                const int left = cur.end() - cur.tile * TR_KEYS;                   // rows of the tile inside the stream
+                if (TR_RARE(!tr_wait(full + 8 * s, ph))) { failed = true; break; }
+                TRPage<BITS> x0, x1;
+                x0.load(ring + (s * TR_PAGES + 2 * w) * SM::PAGE, at);             // (what a page behind the end left there is finite)
+                x1.load(ring + (s * TR_PAGES + 2 * w + 1) * SM::PAGE, at);
+                // the tile's exponent: lane = two neighbouring rows of page lane / 8; rows behind the end have no scale
+                const unsigned char* meta = metas + s * TR_PAGES * SM::META;
+                uint32_t two = 2 * lane < left ? *reinterpret_cast<const uint32_t*>(meta + (lane >> 3) * SM::META + (lane & 7) * 4) : 0u;
+                if (2 * lane + 1 == left) two &= 0xffffu;
+                const int e = __reduce_max_sync(0xffffffffu, max(tr_exponent(two << 16), tr_exponent(two & 0xffff0000u)));
+                // factors of this lane's rows: r0 and 8 on of both pages.  A K that is not finite makes its logit so; a V enters as zeros
+                const float up = exp2_int(15 - e);
+                auto factor = [&](int page, int r) {
+                    const uint32_t x = page * PIKV_PAGE_TOKENS + r < left ? (uint32_t)reinterpret_cast<const uint16_t*>(meta + page * SM::META)[r] << 16 : 0u;
+                    return __uint_as_float(of_v && (x & 0x7f800000u) == 0x7f800000u ? 0u : x) * up;
+                };
+                const float a00 = factor(2 * w, r0), a01 = factor(2 * w, r0 + 8), a10 = factor(2 * w + 1, r0), a11 = factor(2 * w + 1, r0 + 8);
+                // What the softmax needs of the tile.  The four sets need no wait of their own: the one written here served tile n - 4,
+                // whose second product was issued before the Q K^T of tile n - 2, and these warps have seen that one, or the second
+                // product of tile n - 2, done
+                float* of = reinterpret_cast<float*>(smem + SM::VEXP + (n & 3) * 16);
+                if (!of_v) {
+                    if (w == 0 && lane == 0) of[0] = exp2_int(e + 9);
+                } else {
+                    const uint32_t odd0 = __ballot_sync(0xffffffffu, (two & 0x7f80u) == 0x7f80u), odd1 = __ballot_sync(0xffffffffu, (two & 0x7f800000u) == 0x7f800000u);
                     if (w == 0 && lane == 0) {
-                        *reinterpret_cast<float4*>(smem + SM::VEXP + (j & 3) * 16) =
-                            make_float4(exp2_int(ke + 9), (float)(ve + 9), exp2_int(-9 - ve), __uint_as_float(odd0 | odd1));
-                        *reinterpret_cast<uint2*>(smem + SM::ODD + (j & 3) * 8) = make_uint2(odd0, odd1);
+                        of[1] = (float)(e + 9);
+                        of[2] = exp2_int(-9 - e);
+                        of[3] = __uint_as_float(odd0 | odd1);
+                        *reinterpret_cast<uint2*>(smem + SM::ODD + (n & 3) * 8) = make_uint2(odd0, odd1);
                     }
-                    if (BITS == 4) {
-                        // lanes 0-15: z of K, 16-31: of V
-                        const int side = lane >> 4, r = lane & 15;
-                        const float z = r < rows ? (reinterpret_cast<const float*>(meta + 64)[lane] - 8.f) * (__uint_as_float(scale(r, side)) * exp2_int(-9 - (side ? ve : ke))) : 0.f;
-                        reinterpret_cast<float*>(smem + SM::SIDE)[((j & 3) * 2 + side) * TR_KEYS + w * PIKV_PAGE_TOKENS + r] = z;
-                    }
-                    // Q K^T of the tile before has read the buffer
-                    if (j > 0 && !tr_wait(s_full + 8 * ((j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u)) { failed = true; break; }
-                    if (rows > 0) x.store(smem + SM::K, w, lane, ka0, ka1);
-                    tr_fence_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        lr_mbar_arrive(side_full + 8 * (j & 3));
-                        lr_mbar_arrive(k_full);
-                        lr_mbar_arrive(kr_empty + 8 * ks);
-                    }
-                    if (++ks == TR_K_AHEAD) ks = 0, kph ^= 1u;
                 }
-                if (m < 0) continue;
-                if (TR_RARE(!tr_wait(vr_full + 8 * vs, vph))) { failed = true; break; }
-                TRPage<BITS> x;
-                if (v_rows > 0) x.load(smem + SM::VRING + (vs * TR_PAGES + w) * SM::PAGE, at);
-                if (m > 0 && !tr_wait(pv_done + 8 * ((m - 1) & 1), (uint32_t)((m - 1) >> 1) & 1u)) { failed = true; break; }
-                if (v_rows > 0) x.store(smem + SM::V, w, lane, va0, va1);
+                if (BITS == 4) {
+                    const int page = 2 * w + (lane >> 4), r = lane & 15;
+                    const unsigned char* own = meta + page * SM::META;
+                    reinterpret_cast<float*>(smem + SM::SIDE)[((n & 3) * 2 + of_v) * TR_KEYS + 32 * w + lane] =
+                        32 * w + lane < left ? (reinterpret_cast<const float*>(own + 32)[r] - 8.f) *
+                                                   (__uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(own)[r] << 16) * exp2_int(-9 - e))
+                                             : 0.f;
+                }
+                __syncwarp();
+                if (lane == 0) lr_mbar_arrive(side_full + 8 * (n & 3));
+                // the product of the tile before has read the buffer
+                if (n > 0 && TR_RARE(!tr_wait(read + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) { failed = true; break; }
+                x0.store(tile, 2 * w, lane, a00, a01);
+                x1.store(tile, 2 * w + 1, lane, a10, a11);
                 tr_fence_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    lr_mbar_arrive(v_full);
-                    lr_mbar_arrive(vr_empty + 8 * vs);
+                    lr_mbar_arrive(ready);
+                    lr_mbar_arrive(empty + 8 * s);
                 }
-                if (++vs == TR_V_AHEAD) vs = 0, vph ^= 1u;
+                if (++s == ahead) s = 0, ph ^= 1u;
+                if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
             }
         } else {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
