@@ -24,6 +24,7 @@ static inline int cache_dev(const pikv_paged_cache* c, CacheDev& d, const char* 
     PIKV_REQUIRE(c->num_seqs > 0 && c->max_pages > 0 && c->num_pages > 0 && c->n_kv > 0, PIKV_EINVAL, "%s: bad cache geometry", what);
     PIKV_REQUIRE(c->bits == 8 || c->bits == 4, PIKV_EINVAL, "%s: bits must be 4 or 8", what);
     PIKV_REQUIRE((long long)c->max_pages * PIKV_PAGE_TOKENS < (1ll << 31), PIKV_ELIMIT, "%s: positions must stay below 2^31", what);
+    PIKV_REQUIRE((long long)c->num_pages * c->n_kv < (1ll << 32), PIKV_ELIMIT, "%s: num_pages * n_kv must stay below 2^32", what);
     for (const void* pool : {(const void*)c->k_codes, (const void*)c->v_codes, (const void*)c->k_scale, (const void*)c->v_scale, (const void*)c->k_zp, (const void*)c->v_zp})
         PIKV_REQUIRE((reinterpret_cast<uintptr_t>(pool) & 15) == 0, PIKV_EINVAL, "%s: the cache's pools must be 16-byte aligned", what);
     if (decodable) {

@@ -379,9 +379,6 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
         for (int i = 0; i < TR_V_AHEAD; ++i) lr_mbar_init(vr_full + 8 * i, 1), lr_mbar_init(vr_empty + 8 * i, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // keys behind a stream's last page keep what was in the tile: weights of 0 times something finite
-    for (int i = tid; i < 2 * TR_TILE / 16; i += TR_THREADS) reinterpret_cast<uint4*>(smem + SM::K)[i] = make_uint4(0u, 0u, 0u, 0u);
-    tr_fence_smem();
     if (warp == TR_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lr_smem_u32(tmem_slot)), "r"(TR_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -794,6 +791,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
 }
 
 constexpr int TM_THREADS = 128;
+constexpr int TM_BATCH = 8;
 
 // Joins the pieces of units that were cut, and answers for the rows that no unit has.  One warp per (stream, node, query head),
 // lane = 4 channels: O = sum_i O_i 2^(R_i - R), the denominator likewise.
@@ -820,26 +818,28 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
     if (c0 == c1) return;                                               // whole: written by its CTA
     auto slot = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * parts.rows + r % TR_ROWS; };
     float M = -INFINITY, den = 0.f;
-    for (int g = c0; g <= c1; g += 32) M = fmaxf(M, warp_max(g + lane <= c1 ? parts.ml[slot(g + lane)].x : -INFINITY));
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int g = c0; g <= c1; g += 32) {
-        const int cnt = min(32, c1 - g + 1);
+    // pieces in batches: their outputs are on the way while the references are looked at
+    for (int g = c0; g <= c1; g += TM_BATCH) {
+        const int cnt = min(TM_BATCH, c1 - g + 1);
         float2 ml = make_float2(-INFINITY, 0.f);
         if (lane < cnt) ml = parts.ml[slot(g + lane)];
+        float4 o[TM_BATCH];
+#pragma unroll
+        for (int u = 0; u < TM_BATCH; ++u) o[u] = u < cnt ? reinterpret_cast<const float4*>(parts.o + slot(g + u) * 128)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float top = fmaxf(M, warp_max(ml.x)), base = top == -INFINITY ? 0.f : top;
+        const float keep = M == -INFINITY ? (den == 0.f ? 0.f : 1.f) : exp2f(M - base);
         // a piece that saw nothing has no weight; one that is not a number keeps it
-        const float w_l = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - (M == -INFINITY ? 0.f : M));
-        for (int i = 0; i < cnt; i += 4) {
-            float4 o[4];
+        const float w_l = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - base);
+        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+        den *= keep;
+        M = top;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (i + u < cnt) o[u] = reinterpret_cast<const float4*>(parts.o + slot(g + i + u) * 128)[lane];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (i + u >= cnt) break;
-                const float w = __shfl_sync(0xffffffffu, w_l, i + u), l = __shfl_sync(0xffffffffu, ml.y, i + u);
-                acc.x += o[u].x * w; acc.y += o[u].y * w; acc.z += o[u].z * w; acc.w += o[u].w * w;
-                den += l * w;
-            }
+        for (int u = 0; u < TM_BATCH; ++u) {
+            if (u >= cnt) break;
+            const float w = __shfl_sync(0xffffffffu, w_l, u), l = __shfl_sync(0xffffffffu, ml.y, u);
+            acc.x += o[u].x * w; acc.y += o[u].y * w; acc.z += o[u].z * w; acc.w += o[u].w * w;
+            den += l * w;
         }
     }
     const bool any = den != 0.f;
@@ -1028,8 +1028,8 @@ extern "C" int pikv_tree_accept(const pikv_paged_cache* c, const int32_t* path, 
     AcceptDev d;
     const int rc = cache_dev(c, d.c, "tree_accept", false);
     if (rc != PIKV_OK) return rc;
-    PIKV_REQUIRE(path && ctx_len && new_len, PIKV_EINVAL, "tree_accept: null pointer");
-    PIKV_REQUIRE(B > 0 && depth > 0 && (seq_ids || B <= c->num_seqs), PIKV_EINVAL, "tree_accept: bad sizes");
+    PIKV_REQUIRE((path || depth == 0) && ctx_len && new_len, PIKV_EINVAL, "tree_accept: null pointer");
+    PIKV_REQUIRE(B > 0 && depth >= 0 && (seq_ids || B <= c->num_seqs), PIKV_EINVAL, "tree_accept: bad sizes");
     PIKV_REQUIRE(!(seq_ids && ctx_len == length), PIKV_EINVAL, "tree_accept: with seq_ids, ctx_len has an entry per stream of the call");
     d.depth = depth;
     d.all_ids = seq_ids;

@@ -326,3 +326,35 @@ def test_captured_and_on_another_stream():
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(held, outs)) and torch.equal(cache.length, length)
     cache.check_status()
+
+
+def test_two_streams_at_once():
+    """Two caches stepped on two CUDA streams, their kernels side by side on the GPU, against the same steps one after the other."""
+    n_kv, G, N, B = 2, 4, 24, 6
+    made = []
+    for seed, bits in ((51, 8), (52, 4)):
+        cache, gen = filled_cache([3000 + 100 * i for i in range(B)], n_kv, bits, seed=seed)
+        cache.length.copy_(torch.tensor([2900 + 100 * i for i in range(B)], dtype=torch.int32))
+        q = torch.randn(B, N, n_kv * G, D, generator=gen, device="cuda").bfloat16()
+        made.append((cache, cache.page_bounds(), q, torch.rand(B, N, N, generator=gen, device="cuda") < 0.4))
+
+    def step(cache, bounds, q, mask):
+        cache.update_bounds(bounds)
+        return [cache.decode_attention_tree(q, mask), cache.decode_attention_sparse(q[:, 0].contiguous(), bounds, 40, first=1), bounds.codes.clone()]
+
+    want = [step(*m) for m in made]
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(5):
+        for m in made:
+            m[1].codes.zero_()
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        got = []
+        for s, m in zip(streams, made):
+            with torch.cuda.stream(s):
+                got.append(step(*m))
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        assert all(torch.equal(x, y) for a, b in zip(got, want) for x, y in zip(a, b))
+    for m in made:
+        m[0].check_status()

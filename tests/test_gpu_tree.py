@@ -266,6 +266,10 @@ def test_accept_refused_paths():
     new = cache.accept_tree(p, seq_ids=torch.tensor([2, 4, 2], dtype=torch.int32, device="cuda"))
     assert int(cache.status) == 1 and new.tolist() == [45, 0, 0] and cache.length.tolist() == [40, 41, 45, 50]
     cache.status.zero_()
+    new = cache.accept_tree(p[:, :0], seq_ids=torch.tensor([3, 0, 2], dtype=torch.int32, device="cuda"))     # nothing accepted
+    assert new.tolist() == [50, 40, 45] and cache.length.tolist() == [40, 41, 45, 50]
+    assert cache.accept_tree(p[:0]).shape == (0,)
+    cache.check_status()
     cache.page_table[1, 2] = -1
     held = buffers(cache)
     new = cache.accept_tree(p[:1], seq_ids=torch.tensor([1], dtype=torch.int32, device="cuda"))

@@ -91,7 +91,8 @@ def test_abi_refusals():
     assert lib.pikv_page_bounds_update(ref(c), at, at, None, None, at, 1, None) == -1 and b"aligned" in lib.pikv_last_error()
     c.k_codes = at
     assert lib.pikv_page_bounds_update(ref(c), at, at, None, None, at, 5, None) == -1         # five streams of four
-    assert lib.pikv_tree_accept(ref(c), at, None, None, at, 1, 0, None, at, None) == -1
+    assert lib.pikv_tree_accept(ref(c), at, None, None, at, 1, -1, None, at, None) == -1
+    assert lib.pikv_tree_accept(ref(c), None, None, None, at, 1, 1, None, at, None) == -1
     assert lib.pikv_tree_accept(ref(c), at, None, at, at, 1, 1, at, at, None) == -1           # ctx_len is `length`, with ids
 
     t = _lib.TreeParams()
