@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(PS_THREADS, PS_CTAS) page_score_kernel(SelectD
 
 // ---- selection ------------------------------------------------------------------------------------------------
 constexpr int SL_THREADS = 512;
-constexpr int SL_LOG_BINS = 11, SL_BINS = 1 << SL_LOG_BINS;
+constexpr int SL_LOG_BINS = 10, SL_BINS = 1 << SL_LOG_BINS;
 
 // One CTA per (stream, KV head): the want-th largest key, then the kept pages in ascending order.  Keys are read once into
 // shared memory.  The threshold: bins of equal width over the range that the keys really have (bins over the bits of the

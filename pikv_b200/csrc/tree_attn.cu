@@ -52,7 +52,7 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // that entry.  Keys and values enter as f16 of code * scale, in units of a power of two per tile (2^(e - 9), 2^e above the tile's
 // largest scale): one rounding, 2^-11 of the entry, the size of the weights' own; in return the softmax neither loads nor
 // multiplies by the scales (shared-memory reads of the scales by every row were the busiest pipe of the kernel that applied
-// them to exact integer products: 58 % busy, 248 us for 16 x 16384 x 32 nodes against XXX).
+// them to exact integer products: 16 x 16384 x 32 nodes, 248 -> 221 us).
 //   logit = 2^(e_k + 9) / sqrt(128) (q . K16 - z)      z: the zero points' part, (zp - 8) scale sum(q), 4 bit only
 //   O     = sum w V16 - sum w z_v,  w = f16(2^(logit - R + e_v + 9))
 // R is a row's reference: the largest logit (log2 domain) plus e_v + 9 of the tile it was seen in, so that the weights sit at
@@ -675,41 +675,28 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 if (warp_live) {
                     out_row = ((size_t)cur.b * d.N + (live ? node : 0)) * d.n_q + (size_t)h * d.G + row % d.G;
                     const uint4* src = reinterpret_cast<const uint4*>(d.q + out_row * 128);
-                    // what a node sees of the tree, a bit per node: the warp reads the mask rows of its nodes together
-                    const int node0 = __shfl_sync(0xffffffffu, node, 0), node1 = min(__shfl_sync(0xffffffffu, node, 31), cur.nodes - 1);
-                    const uint8_t* masks = d.mask + (size_t)cur.b * d.mask_stride;
-                    tree = 0;
-#pragma unroll 4
-                    for (int i = node0; i <= node1; ++i) {
-                        const bool lo = lane < cur.nodes && __ldg(masks + (size_t)i * d.N + lane) != 0;
-                        const bool hi = lane + 32 < cur.nodes && __ldg(masks + (size_t)i * d.N + lane + 32) != 0;
-                        const uint32_t m0 = __ballot_sync(0xffffffffu, lo), m1 = __ballot_sync(0xffffffffu, hi);
-                        if (node == i) tree = (uint64_t)m1 << 32 | m0;
-                    }
-                    float amax = 0.f, odd = 0.f;
-#pragma unroll 8
-                    for (int i = 0; i < 16; ++i) {
-                        const uint4 q4 = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-                        const uint32_t ww[4] = {q4.x, q4.y, q4.z, q4.w};
+                    uint4 q4[16];                                     // (one trip: shared memory leaves next to no L1)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            float x, y;
-                            bf16x2_to_f32(ww[k], x, y);
-                            amax = fmaxf(amax, fmaxf(fabsf(x), fabsf(y)));
-                            odd += x * 0.f + y * 0.f;                 // NaN where the row is not finite
-                        }
+                    for (int i = 0; i < 16; ++i) q4[i] = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+                    // largest entry by its bits, two to a word; what is not finite is above all that is
+                    uint32_t top2 = 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t a = __vmaxu2(q4[i].x & 0x7fff7fffu, q4[i].y & 0x7fff7fffu), b = __vmaxu2(q4[i].z & 0x7fff7fffu, q4[i].w & 0x7fff7fffu);
+                        top2 = __vmaxu2(top2, __vmaxu2(a, b));
                     }
+                    const uint32_t top = max(top2 & 0xffffu, top2 >> 16) << 16;
+                    const float amax = __uint_as_float(top), odd = top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : 0.f;
                     const int sh = amax > 0.f && amax < INFINITY ? min(126, 14 - ((int)(__float_as_uint(amax) >> 23) - 127)) : 0;
                     const float up = exp2_int(max(sh, -126));
                     qsum = 0.f;
-#pragma unroll 4
+#pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const uint4 q4 = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
                         float x[8];
-                        bf16x2_to_f32(q4.x, x[0], x[1]);
-                        bf16x2_to_f32(q4.y, x[2], x[3]);
-                        bf16x2_to_f32(q4.z, x[4], x[5]);
-                        bf16x2_to_f32(q4.w, x[6], x[7]);
+                        bf16x2_to_f32(q4[i].x, x[0], x[1]);
+                        bf16x2_to_f32(q4[i].y, x[2], x[3]);
+                        bf16x2_to_f32(q4[i].z, x[4], x[5]);
+                        bf16x2_to_f32(q4[i].w, x[6], x[7]);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             x[k] *= up;
@@ -727,6 +714,19 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 }
                 __syncwarp();
                 if (lane == 0) lr_mbar_arrive(q_full);
+                if (warp_live) {
+                    // what a node sees of the tree, a bit per node: the warp reads the mask rows of its nodes together
+                    const int node0 = __shfl_sync(0xffffffffu, node, 0), node1 = min(__shfl_sync(0xffffffffu, node, 31), cur.nodes - 1);
+                    const uint8_t* masks = d.mask + (size_t)cur.b * d.mask_stride;
+                    tree = 0;
+#pragma unroll 4
+                    for (int i = node0; i <= node1; ++i) {
+                        const bool lo = lane < cur.nodes && __ldg(masks + (size_t)i * d.N + lane) != 0;
+                        const bool hi = lane + 32 < cur.nodes && __ldg(masks + (size_t)i * d.N + lane + 32) != 0;
+                        const uint32_t m0 = __ballot_sync(0xffffffffu, lo), m1 = __ballot_sync(0xffffffffu, hi);
+                        if (node == i) tree = (uint64_t)m1 << 32 | m0;
+                    }
+                }
                 for (int t = t0; t < edge && !failed; ++t, ++n) failed = !step(std::false_type{}, n, t, t == t0);
                 for (int t = edge; t < t1 && !failed; ++t, ++n) failed = !step(std::true_type{}, n, t, t == t0);
                 if (failed) break;
@@ -819,14 +819,18 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
     auto slot = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * parts.rows + r % TR_ROWS; };
     float M = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    // pieces in batches: their outputs are on the way while the references are looked at
-    for (int g = c0; g <= c1; g += TM_BATCH) {
-        const int cnt = min(TM_BATCH, c1 - g + 1);
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < cnt) ml = parts.ml[slot(g + lane)];
-        float4 o[TM_BATCH];
+    // pieces in batches, the next one on its way while one is joined
+    float4 o[TM_BATCH], next[TM_BATCH];
+    float2 ml, next_ml;
+    auto fetch = [&](int g, float4 (&to)[TM_BATCH], float2& to_ml) {
+        to_ml = g + lane <= c1 && lane < TM_BATCH ? parts.ml[slot(g + lane)] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int u = 0; u < TM_BATCH; ++u) o[u] = u < cnt ? reinterpret_cast<const float4*>(parts.o + slot(g + u) * 128)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int u = 0; u < TM_BATCH; ++u)
+            to[u] = g + u <= c1 ? reinterpret_cast<const float4*>(parts.o + slot(g + u) * 128)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    fetch(c0, o, ml);
+    for (int g = c0; g <= c1; g += TM_BATCH) {
+        if (g + TM_BATCH <= c1) fetch(g + TM_BATCH, next, next_ml);
         const float top = fmaxf(M, warp_max(ml.x)), base = top == -INFINITY ? 0.f : top;
         const float keep = M == -INFINITY ? (den == 0.f ? 0.f : 1.f) : exp2f(M - base);
         // a piece that saw nothing has no weight; one that is not a number keeps it
@@ -836,11 +840,14 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
         M = top;
 #pragma unroll
         for (int u = 0; u < TM_BATCH; ++u) {
-            if (u >= cnt) break;
+            if (g + u > c1) break;
             const float w = __shfl_sync(0xffffffffu, w_l, u), l = __shfl_sync(0xffffffffu, ml.y, u);
             acc.x += o[u].x * w; acc.y += o[u].y * w; acc.z += o[u].z * w; acc.w += o[u].w * w;
             den += l * w;
         }
+#pragma unroll
+        for (int u = 0; u < TM_BATCH; ++u) o[u] = next[u];
+        ml = next_ml;
     }
     const bool any = den != 0.f;
     const __nv_bfloat162 lo = __floats2bfloat162_rn(any ? acc.x / den : 0.f, any ? acc.y / den : 0.f);
