@@ -799,13 +799,13 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
     dependency_release();
     dependency_wait();
     const int lane = threadIdx.x & 31;
-    const long long at = (long long)blockIdx.x * (TM_THREADS / 32) + (threadIdx.x >> 5);
-    if (at >= (long long)d.B * d.N * d.n_q) return;
-    const int qh = (int)(at % d.n_q), node = (int)(at / d.n_q % d.N), b = (int)(at / d.n_q / d.N);
+    const uint32_t at = blockIdx.x * (TM_THREADS / 32) + (threadIdx.x >> 5), rows = (uint32_t)d.N * (uint32_t)d.n_q;
+    if (at >= (uint32_t)d.B * rows) return;
+    const int b = (int)(at / rows), node = (int)(at % rows) / d.n_q, qh = (int)(at % rows) % d.n_q;
     const int per = parts.plan[0], pre0 = parts.plan[1 + b];
     int row, nodes;
     const int ctx = tree_lengths(d, b, row, nodes);
-    uint2* out = reinterpret_cast<uint2*>(d.out + at * 128) + lane;
+    uint2* out = reinterpret_cast<uint2*>(d.out + (size_t)at * 128) + lane;
     if (node >= nodes) {
         *out = make_uint2(0u, 0u);
         if (lane == 0 && d.lse) d.lse[at] = -INFINITY;
@@ -816,21 +816,25 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
     const int f0 = pre0 + ((qh / d.G) * row_tiles + r / TR_ROWS) * tiles, f1 = f0 + tiles;
     const int c0 = f0 / per, c1 = (f1 - 1) / per;
     if (c0 == c1) return;                                               // whole: written by its CTA
-    auto slot = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * parts.rows + r % TR_ROWS; };
+    // piece i lies in slot 2 (c0 + i), the first one in the slot behind that
+    const size_t slot0 = (size_t)2 * c0 * parts.rows + r % TR_ROWS;
+    const float4* o0 = reinterpret_cast<const float4*>(parts.o + slot0 * 128) + lane;
+    const float2* ml0 = parts.ml + slot0;
+    const int pieces = c1 - c0 + 1, stride = 2 * parts.rows;
     float M = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     // pieces in batches, the next one on its way while one is joined
     float4 o[TM_BATCH], next[TM_BATCH];
     float2 ml, next_ml;
     auto fetch = [&](int g, float4 (&to)[TM_BATCH], float2& to_ml) {
-        to_ml = g + lane <= c1 && lane < TM_BATCH ? parts.ml[slot(g + lane)] : make_float2(-INFINITY, 0.f);
+        to_ml = g + lane < pieces && lane < TM_BATCH ? ml0[(size_t)(g + lane) * stride + (g + lane ? 0 : parts.rows)] : make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int u = 0; u < TM_BATCH; ++u)
-            to[u] = g + u <= c1 ? reinterpret_cast<const float4*>(parts.o + slot(g + u) * 128)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (g + u < pieces) to[u] = o0[((size_t)(g + u) * stride + (g + u ? 0 : parts.rows)) * 32];
     };
-    fetch(c0, o, ml);
-    for (int g = c0; g <= c1; g += TM_BATCH) {
-        if (g + TM_BATCH <= c1) fetch(g + TM_BATCH, next, next_ml);
+    fetch(0, o, ml);
+    for (int g = 0; g < pieces; g += TM_BATCH) {
+        if (g + TM_BATCH < pieces) fetch(g + TM_BATCH, next, next_ml);
         const float top = fmaxf(M, warp_max(ml.x)), base = top == -INFINITY ? 0.f : top;
         const float keep = M == -INFINITY ? (den == 0.f ? 0.f : 1.f) : exp2f(M - base);
         // a piece that saw nothing has no weight; one that is not a number keeps it
@@ -840,7 +844,7 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
         M = top;
 #pragma unroll
         for (int u = 0; u < TM_BATCH; ++u) {
-            if (g + u > c1) break;
+            if (g + u >= pieces) break;
             const float w = __shfl_sync(0xffffffffu, w_l, u), l = __shfl_sync(0xffffffffu, ml.y, u);
             acc.x += o[u].x * w; acc.y += o[u].y * w; acc.z += o[u].z * w; acc.w += o[u].w * w;
             den += l * w;
