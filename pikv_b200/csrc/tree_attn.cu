@@ -791,10 +791,14 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
 }
 
 constexpr int TM_THREADS = 128;
-constexpr int TM_BATCH = 8;
+constexpr int TM_RESIDENT = 5;                                          // blocks of tree_merge_kernel<8> on an SM
 
 // Joins the pieces of units that were cut, and answers for the rows that no unit has.  One warp per (stream, node, query head),
 // lane = 4 channels: O = sum_i O_i 2^(R_i - R), the denominator likewise.
+// Bound by the trips to the pieces (in L2): BATCH of them are on their way while as many are joined.  BATCH = 8 takes 96 registers and is right
+// while all rows' warps are resident with them (few rows have many pieces each: 1 stream x 8 nodes 6.7 us against 8.5 with 4);
+// more rows have fewer pieces and want the warps (16 streams x 16 nodes: 12.4 us with 4 against 16.0).
+template <int BATCH>
 __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeParts parts) {
     dependency_release();
     dependency_wait();
@@ -824,17 +828,17 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
     float M = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     // pieces in batches, the next one on its way while one is joined
-    float4 o[TM_BATCH], next[TM_BATCH];
+    float4 o[BATCH], next[BATCH];
     float2 ml, next_ml;
-    auto fetch = [&](int g, float4 (&to)[TM_BATCH], float2& to_ml) {
-        to_ml = g + lane < pieces && lane < TM_BATCH ? ml0[(size_t)(g + lane) * stride + (g + lane ? 0 : parts.rows)] : make_float2(-INFINITY, 0.f);
+    auto fetch = [&](int g, float4 (&to)[BATCH], float2& to_ml) {
+        to_ml = g + lane < pieces && lane < BATCH ? ml0[(size_t)(g + lane) * stride + (g + lane ? 0 : parts.rows)] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int u = 0; u < TM_BATCH; ++u)
+        for (int u = 0; u < BATCH; ++u)
             if (g + u < pieces) to[u] = o0[((size_t)(g + u) * stride + (g + u ? 0 : parts.rows)) * 32];
     };
     fetch(0, o, ml);
-    for (int g = 0; g < pieces; g += TM_BATCH) {
-        if (g + TM_BATCH < pieces) fetch(g + TM_BATCH, next, next_ml);
+    for (int g = 0; g < pieces; g += BATCH) {
+        if (g + BATCH < pieces) fetch(g + BATCH, next, next_ml);
         const float top = fmaxf(M, warp_max(ml.x)), base = top == -INFINITY ? 0.f : top;
         const float keep = M == -INFINITY ? (den == 0.f ? 0.f : 1.f) : exp2f(M - base);
         // a piece that saw nothing has no weight; one that is not a number keeps it
@@ -843,14 +847,14 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
         den *= keep;
         M = top;
 #pragma unroll
-        for (int u = 0; u < TM_BATCH; ++u) {
+        for (int u = 0; u < BATCH; ++u) {
             if (g + u >= pieces) break;
             const float w = __shfl_sync(0xffffffffu, w_l, u), l = __shfl_sync(0xffffffffu, ml.y, u);
             acc.x += o[u].x * w; acc.y += o[u].y * w; acc.z += o[u].z * w; acc.w += o[u].w * w;
             den += l * w;
         }
 #pragma unroll
-        for (int u = 0; u < TM_BATCH; ++u) o[u] = next[u];
+        for (int u = 0; u < BATCH; ++u) o[u] = next[u];
         ml = next_ml;
     }
     const bool any = den != 0.f;
@@ -1028,7 +1032,9 @@ extern "C" int pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params*
             if (!allow_smem<tree_attn_kernel<4>>(TRSmem<4>::BYTES)) return check_launch("tree_attn smem attribute");
             launch_dependent(tree_attn_kernel<4>, grid, TR_THREADS, TRSmem<4>::BYTES, st, d, parts);
         }
-        launch_dependent(tree_merge_kernel, (int)((d.B * rows + TM_THREADS / 32 - 1) / (TM_THREADS / 32)), TM_THREADS, 0, st, d, parts);
+        const int blocks = (int)((d.B * rows + TM_THREADS / 32 - 1) / (TM_THREADS / 32));
+        if (blocks <= sm_count() * TM_RESIDENT) launch_dependent(tree_merge_kernel<8>, blocks, TM_THREADS, 0, st, d, parts);
+        else launch_dependent(tree_merge_kernel<4>, blocks, TM_THREADS, 0, st, d, parts);
         count_launch(2);
     }
     return check_launch("tree_attn_kernel");
