@@ -47,7 +47,8 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 //   4-5, 6-7  two pages of every tile each: codes of K, of V, to f16, into the swizzled layout that both products read
 //   8    issues the MMAs: Q K^T of tile n + 1 before P V of tile n, so that the products of one tile run while the softmax
 //        of another does
-//   9    bulk copies of pages into two rings, K three tiles ahead and V two
+//   9, 10  bulk copies of pages into two rings, K three tiles ahead, V two (one warp for both is late: 130 cycles a copy)
+//   11   the rows' scales in the forms that the converting warps and the softmax use
 // The query enters exactly: bf16 times a power of two per row that brings its largest entry to 2^14 is f16 down to 2^-38 of
 // that entry.  Keys and values enter as f16 of code * scale, in units of a power of two per tile (2^(e - 9), 2^e above the tile's
 // largest scale): one rounding, 2^-11 of the entry, the size of the weights' own; in return the softmax neither loads nor
@@ -64,8 +65,8 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // burst, 235 us in long runs under the power cap (the bytes alone take 85 us, the products 82).  Bound by the conversions, the
 // weights and their handing over: 3180 warp instructions per tile (1126 convert K and V, 548 make weights, 150 read scores) in
 // 0.56 of the issue slots, tensor pipe 36 %, DRAM 35 %.  No single pipe is full; the 24 warps wait for one another.
-constexpr int TR_THREADS = 384;          // three warpgroups: warps 10 and 11 only complete the last
-constexpr int TR_K = 4, TR_V = 6, TR_MMA = 8, TR_COPY = 9;      // first converting warps of K and of V, and the two single ones
+constexpr int TR_THREADS = 384;          // three warpgroups
+constexpr int TR_K = 4, TR_V = 6, TR_MMA = 8, TR_COPY = 9, TR_SCALES = 11;      // first warps of each kind
 constexpr int TR_ROWS = 128;             // rows of a unit
 constexpr int TR_KEYS = 64;              // keys of a tile
 constexpr int TR_PAGES = TR_KEYS / PIKV_PAGE_TOKENS;
@@ -77,6 +78,7 @@ constexpr uint32_t TR_COL_O = 0, TR_COL_S = 128, TR_COLS = 256;      // S of eve
 
 constexpr int TR_TILE = 2 * TR_KEYS * 128;                                     // bytes of a tile of f16: [2 halves of the channels][64 keys][128 bytes]
 constexpr int TR_K_AHEAD = 3, TR_V_AHEAD = 2;                                   // tiles whose copies are on their way
+constexpr int TR_SETS = 8;                                                      // tiles whose scales are kept as the warps want them
 
 // shared memory behind a 1024-byte boundary
 template <int BITS> struct TRSmem {
@@ -87,13 +89,17 @@ template <int BITS> struct TRSmem {
                          VRING = KRING + TR_K_AHEAD * TR_PAGES * PAGE,
                          KMETA = VRING + TR_V_AHEAD * TR_PAGES * PAGE,         // [ahead][page] scales, zero points of K, of V
                          VMETA = KMETA + TR_K_AHEAD * TR_PAGES * META,
-                         SIDE = VMETA + TR_V_AHEAD * TR_PAGES * META,          // 4 bit: [4][2][64] fp32: z of K, of V, of four tiles
-                         VEXP = SIDE + 4 * SIDES * TR_KEYS * 4,                // [4] of four tiles: 2^(e_k + 9), e_v + 9, 2^-(e_v + 9) as floats, whether a row of V is not finite
-                         ODD = VEXP + 64,                                       // [4][2] even and odd rows of V that are not finite, a bit each
-                         BARS = ODD + 32, NBARS = 14 + 2 * (TR_K_AHEAD + TR_V_AHEAD),
+                         SIDE = VMETA + TR_V_AHEAD * TR_PAGES * META,          // 4 bit: [sets][2][64] fp32: z of K, of V
+                         FACT = SIDE + TR_SETS * SIDES * TR_KEYS * 4,          // [sets][2][64] f16: factors of the rows of K, of V
+                         VEXP = FACT + TR_SETS * 2 * TR_KEYS * 2,              // [sets] 2^(e_k + 9), e_v + 9, 2^-(e_v + 9) as floats, whether a row of V is not finite
+                         ODD = VEXP + TR_SETS * 16,                            // [sets][2] even and odd rows of V that are not finite, a bit each
+                         BARS = ODD + TR_SETS * 8, NBARS = 9 + 2 * TR_SETS + 2 * (TR_K_AHEAD + TR_V_AHEAD),
                          PRE = BARS + NBARS * 8, MISC = PRE + (PIKV_STREAMS_PER_LAUNCH + 1) * 4, END = MISC + 16;
     static constexpr int BYTES = END + 1024;
 };
+
+__device__ __forceinline__ uint32_t tr_set(int n) { return (uint32_t)n % TR_SETS; }
+__device__ __forceinline__ uint32_t tr_set_phase(int n) { return (uint32_t)n / TR_SETS & 1u; }
 
 // what hardly ever happens goes behind the loops: a jump over it costs the instruction cache
 #define TR_RARE(x) __builtin_expect(!!(x), 0)
@@ -277,13 +283,12 @@ template <int BITS> struct TRPage {
         const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
-    // a0, a1: of rows base and base + 8
-    __device__ __forceinline__ void store(unsigned char* tile, int page, int lane, float a0, float a1) const {
+    // a: factors of rows base and base + 8
+    __device__ __forceinline__ void store(unsigned char* tile, int page, int lane, const __half2 (&a)[2]) const {
         const int r = tr_row(lane), c = lane & 3;
         unsigned char* row = tile + (page * PIKV_PAGE_TOKENS + r) * 128;
         const int d0 = 16 * ((2 * c) ^ (r & 7)), d1 = 16 * ((2 * c + 1) ^ (r & 7));
-        constexpr float OFFSET = (BITS == 8 ? -128.f : -8.f) / 16777216.f;
-        const __half2 a[2] = {__float2half2_rn(a0), __float2half2_rn(a1)}, b[2] = {__float2half2_rn(a0 * OFFSET), __float2half2_rn(a1 * OFFSET)};
+        const __half2 offset = __float2half2_rn((BITS == 8 ? -128.f : -8.f) / 16777216.f), b[2] = {__hmul2(a[0], offset), __hmul2(a[1], offset)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             unsigned char* to = row + (i & 1) * TR_KEYS * 128 + (i >> 1) * 8 * 128;
@@ -371,17 +376,17 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
     int* pre = reinterpret_cast<int*>(smem + SM::PRE);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::MISC);
     const uint32_t bars = sbase + SM::BARS;
-    const uint32_t k_full = bars, v_full = bars + 8, q_full = bars + 16, s_full = bars + 24, p_full = bars + 40, pv_done = bars + 56, side_full = bars + 72,
-                   kr_full = bars + 112, kr_empty = kr_full + 8 * TR_K_AHEAD, vr_full = kr_empty + 8 * TR_K_AHEAD, vr_empty = vr_full + 8 * TR_V_AHEAD;
+    const uint32_t k_full = bars, v_full = bars + 8, q_full = bars + 16, s_full = bars + 24, p_full = bars + 40, pv_done = bars + 56, k_side = bars + 72, v_side = k_side + 8 * TR_SETS,
+                   kr_full = v_side + 8 * TR_SETS, kr_empty = kr_full + 8 * TR_K_AHEAD, vr_full = kr_empty + 8 * TR_K_AHEAD, vr_empty = vr_full + 8 * TR_V_AHEAD;
     dependency_release();
     if (tid == 0) {
         lr_mbar_init(k_full, 2);
         lr_mbar_init(v_full, 2);
         lr_mbar_init(q_full, 4);
         for (int i = 0; i < 2; ++i) lr_mbar_init(s_full + 8 * i, 1), lr_mbar_init(p_full + 8 * i, 4), lr_mbar_init(pv_done + 8 * i, 1);
-        for (int i = 0; i < 4; ++i) lr_mbar_init(side_full + 8 * i, 4);
-        for (int i = 0; i < TR_K_AHEAD; ++i) lr_mbar_init(kr_full + 8 * i, 1), lr_mbar_init(kr_empty + 8 * i, 2);
-        for (int i = 0; i < TR_V_AHEAD; ++i) lr_mbar_init(vr_full + 8 * i, 1), lr_mbar_init(vr_empty + 8 * i, 2);
+        for (int i = 0; i < TR_SETS; ++i) lr_mbar_init(k_side + 8 * i, 1), lr_mbar_init(v_side + 8 * i, 1);
+        for (int i = 0; i < TR_K_AHEAD; ++i) lr_mbar_init(kr_full + 8 * i, 1), lr_mbar_init(kr_empty + 8 * i, 3);
+        for (int i = 0; i < TR_V_AHEAD; ++i) lr_mbar_init(vr_full + 8 * i, 1), lr_mbar_init(vr_empty + 8 * i, 3);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == TR_MMA) {
@@ -462,128 +467,139 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             if (!failed) failed = !pv(count - 1, first_before);
             // nothing of this CTA's is in flight when its tensor memory goes back
             if (!failed) failed = !tr_wait(pv_done + 8 * ((count - 1) & 1), (uint32_t)((count - 1) >> 1) & 1u);
-            } else if (warp == TR_COPY) {
-                // ---- pages into the rings: lanes 0-3 the K and the scales of a tile's pages, lanes 4-7 the V of the tile before ----
+            } else if (warp < TR_SCALES) {
+                // ---- pages into the rings, with their scales: a warp for K, one for V; lane = page of the tile ----
                 cur.start(d, pre, f0);
-                const int count = f1 - f0, i = lane & 3;
+                const bool of_v = warp > TR_COPY;
+                const int count = f1 - f0, i = lane & 3, ahead = of_v ? TR_V_AHEAD : TR_K_AHEAD;
+                const uint8_t* codes = of_v ? d.c.v_codes : d.c.k_codes;
+                const uint16_t* scale = of_v ? d.c.v_scale : d.c.k_scale;
+                const float* zp = of_v ? d.c.v_zp : d.c.k_zp;
+                const uint32_t ring = sbase + (of_v ? SM::VRING : SM::KRING), metas = sbase + (of_v ? SM::VMETA : SM::KMETA);
+                const uint32_t full = of_v ? vr_full : kr_full, empty = of_v ? vr_empty : kr_empty;
                 int ids = -1, ids_row = -2, ids_at = 0;              // page numbers of this stream, 32 at a time: eight tiles
-                int ks = 0, vs = 0, np = 0;                          // stages; pages of the tile whose K went last
-                uint32_t kph = 1, vph = 1, unit = 0;                 // unit: place of page i in the pools
-                for (int n = 0; n <= count; ++n) {
-                    const uint32_t v_unit = unit;
-                    const int v_np = np;
+                int s = 0;
+                uint32_t ph = 1;
+                for (int n = 0; n < count; ++n) {
+                    const int p = cur.tile * TR_PAGES, np = cur.pages();
+                    if (TR_RARE(cur.row != ids_row || p < ids_at || p >= ids_at + 32)) {
+                        ids_row = cur.row;
+                        ids_at = p;
+                        ids = p + lane < d.c.max_pages ? __ldg(d.c.page_table + (size_t)cur.row * d.c.max_pages + p + lane) : -1;
+                    }
+                    int page = __shfl_sync(0xffffffffu, ids, (p + i - ids_at) & 31);
+                    if (TR_RARE(i < np && (page < 0 || page >= d.c.num_pages))) {
+                        if (lane < 4 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_PAGE);
+                        page = 0;
+                    }
+                    const uint32_t unit = (uint32_t)page * (uint32_t)d.c.n_kv + (uint32_t)cur.head;
+                    if (TR_RARE(!tr_wait(empty + 8 * s, ph))) { failed = true; break; }
+                    const uint32_t bar = full + 8 * s;
+                    if (lane == 0) lr_mbar_expect_tx(bar, (uint32_t)np * (SM::PAGE + SM::META));
+                    __syncwarp();
+                    if (lane < np) {
+                        const uint32_t dst = metas + (s * TR_PAGES + i) * SM::META;
+                        tr_bulk(ring + (s * TR_PAGES + i) * SM::PAGE, codes + (size_t)unit * SM::PAGE, SM::PAGE, bar);
+                        tr_bulk(dst, scale + (size_t)unit * 16, 32, bar);
+                        if (BITS == 4) tr_bulk(dst + 32, zp + (size_t)unit * 16, 64, bar);
+                    }
+                    if (++s == ahead) s = 0, ph ^= 1u;
+                    if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
+                }
+                // copies that a warp which gave up no longer waits for land before this CTA's shared memory goes to another
+                for (int k = 0; k < ahead; ++k) (void)tr_wait(full + 8 * k, k < s ? ph ^ 1u : ph);
+            } else {
+                // ---- scales as the other warps want them, K of tile n + 1 before V of tile n; lane = rows 2 lane and 2 lane + 1 ----
+                // The sets need no wait of their own: K of tile n + 1 takes that of tile n - 7, V of tile n - 1 has come, into a place that
+                // V of tile n - 3 left after the second product of tile n - 5
+                cur.start(d, pre, f0);
+                const int count = f1 - f0;
+                auto side = [&](auto v_c, int n, int left, int s, uint32_t ph) {
+                    constexpr bool OF_V = decltype(v_c)::value;
+                    if (TR_RARE(!tr_wait((OF_V ? vr_full : kr_full) + 8 * s, ph))) return false;
+                    const unsigned char* own = smem + (OF_V ? SM::VMETA : SM::KMETA) + (s * TR_PAGES + (lane >> 3)) * SM::META;
+                    uint32_t two = 2 * lane < left ? *reinterpret_cast<const uint32_t*>(own + (lane & 7) * 4) : 0u;     // rows behind the end have none
+                    if (2 * lane + 1 == left) two &= 0xffffu;
+                    const int e = __reduce_max_sync(0xffffffffu, max(tr_exponent(two << 16), tr_exponent(two & 0xffff0000u)));
+                    const float up = exp2_int(15 - e);
+                    const bool odd0 = (two & 0x7f80u) == 0x7f80u, odd1 = (two & 0x7f800000u) == 0x7f800000u;
+                    // a K that is not finite makes its logit so; a V enters as zeros
+                    const float a0 = OF_V && odd0 ? 0.f : __uint_as_float(two << 16) * up, a1 = OF_V && odd1 ? 0.f : __uint_as_float(two & 0xffff0000u) * up;
+                    reinterpret_cast<uint32_t*>(smem + SM::FACT)[(tr_set(n) * 2 + OF_V) * (TR_KEYS / 2) + lane] = tr_pack(a0, a1);
+                    if (BITS == 4) {
+                        float2 z = make_float2(0.f, 0.f);
+                        if (2 * lane < left) {
+                            const float2 zp = *reinterpret_cast<const float2*>(own + 32 + (lane & 7) * 8);
+                            const float down = exp2_int(-9 - e);
+                            z.x = (zp.x - 8.f) * (__uint_as_float(two << 16) * down);
+                            if (2 * lane + 1 < left) z.y = (zp.y - 8.f) * (__uint_as_float(two & 0xffff0000u) * down);
+                        }
+                        reinterpret_cast<float2*>(smem + SM::SIDE)[(tr_set(n) * 2 + OF_V) * (TR_KEYS / 2) + lane] = z;
+                    }
+                    float* of = reinterpret_cast<float*>(smem + SM::VEXP + tr_set(n) * 16);
+                    if (OF_V) {
+                        const uint32_t m0 = __ballot_sync(0xffffffffu, odd0), m1 = __ballot_sync(0xffffffffu, odd1);
+                        if (lane == 0) {
+                            of[1] = (float)(e + 9);
+                            of[2] = exp2_int(-9 - e);
+                            of[3] = __uint_as_float(m0 | m1);
+                            *reinterpret_cast<uint2*>(smem + SM::ODD + tr_set(n) * 8) = make_uint2(m0, m1);
+                        }
+                    } else if (lane == 0) {
+                        of[0] = exp2_int(e + 9);
+                    }
+                    __syncwarp();
+                    if (lane == 0) {
+                        lr_mbar_arrive((OF_V ? v_side : k_side) + 8 * tr_set(n));
+                        lr_mbar_arrive((OF_V ? vr_empty : kr_empty) + 8 * s);
+                    }
+                    return true;
+                };
+                int ks = 0, vs = 0, left = 0;
+                uint32_t kph = 0, vph = 0;
+                for (int n = 0; n <= count && !failed; ++n) {
+                    const int v_left = left;
                     if (n < count) {
-                        const int p = cur.tile * TR_PAGES;
-                        np = cur.pages();
-                        if (TR_RARE(cur.row != ids_row || p < ids_at || p >= ids_at + 32)) {
-                            ids_row = cur.row;
-                            ids_at = p;
-                            ids = p + lane < d.c.max_pages ? __ldg(d.c.page_table + (size_t)cur.row * d.c.max_pages + p + lane) : -1;
-                        }
-                        int page = __shfl_sync(0xffffffffu, ids, (p + i - ids_at) & 31);
-                        if (TR_RARE(i < np && (page < 0 || page >= d.c.num_pages))) {
-                            if (lane < 4 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_PAGE);
-                            page = 0;
-                        }
-                        unit = (uint32_t)page * (uint32_t)d.c.n_kv + (uint32_t)cur.head;
-                        if (TR_RARE(!tr_wait(kr_empty + 8 * ks, kph))) { failed = true; break; }
-                        const uint32_t bar = kr_full + 8 * ks;
-                        if (lane == 0) lr_mbar_expect_tx(bar, (uint32_t)np * (SM::PAGE + SM::META));
-                        __syncwarp();
-                        if (lane < np) {
-                            const uint32_t dst = sbase + SM::KMETA + (ks * TR_PAGES + i) * SM::META;
-                            tr_bulk(sbase + SM::KRING + (ks * TR_PAGES + i) * SM::PAGE, d.c.k_codes + (size_t)unit * SM::PAGE, SM::PAGE, bar);
-                            tr_bulk(dst, d.c.k_scale + (size_t)unit * 16, 32, bar);
-                            if (BITS == 4) tr_bulk(dst + 32, d.c.k_zp + (size_t)unit * 16, 64, bar);
-                        }
+                        left = cur.end() - cur.tile * TR_KEYS;
+                        if (TR_RARE(!side(std::false_type{}, n, left, ks, kph))) { failed = true; break; }
                         if (++ks == TR_K_AHEAD) ks = 0, kph ^= 1u;
                         if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
                     }
                     if (n == 0) continue;
-                    if (TR_RARE(!tr_wait(vr_empty + 8 * vs, vph))) { failed = true; break; }
-                    const uint32_t bar = vr_full + 8 * vs;
-                    if (lane == 4) lr_mbar_expect_tx(bar, (uint32_t)v_np * (SM::PAGE + SM::META));
-                    __syncwarp();
-                    if (lane >= 4 && lane < 4 + v_np) {
-                        const uint32_t dst = sbase + SM::VMETA + (vs * TR_PAGES + i) * SM::META;
-                        tr_bulk(sbase + SM::VRING + (vs * TR_PAGES + i) * SM::PAGE, d.c.v_codes + (size_t)v_unit * SM::PAGE, SM::PAGE, bar);
-                        tr_bulk(dst, d.c.v_scale + (size_t)v_unit * 16, 32, bar);
-                        if (BITS == 4) tr_bulk(dst + 32, d.c.v_zp + (size_t)v_unit * 16, 64, bar);
-                    }
+                    if (TR_RARE(!side(std::true_type{}, n - 1, v_left, vs, vph))) { failed = true; break; }
                     if (++vs == TR_V_AHEAD) vs = 0, vph ^= 1u;
                 }
-                // copies that a warp which gave up no longer waits for land before this CTA's shared memory goes to another
-                for (int k = 0; k < TR_K_AHEAD; ++k) (void)tr_wait(kr_full + 8 * k, k < ks ? kph ^ 1u : kph);
-                for (int k = 0; k < TR_V_AHEAD; ++k) (void)tr_wait(vr_full + 8 * k, k < vs ? vph ^ 1u : vph);
             }
         } else if (warp >= TR_K) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-            cur.start(d, pre, f0);
             // ---- codes to f16: warp w of the two of K, of V, takes pages 2 w and 2 w + 1 of every tile ----
             const bool of_v = warp >= TR_V;
             const int w = (warp - TR_K) & 1, count = f1 - f0, ahead = of_v ? TR_V_AHEAD : TR_K_AHEAD;
-            const int at = tr_place<BITS>(lane), r0 = tr_row(lane);
-            const unsigned char* ring = smem + (of_v ? SM::VRING : SM::KRING);
-            const unsigned char* metas = smem + (of_v ? SM::VMETA : SM::KMETA);
+            const int at = tr_place<BITS>(lane);
+            const unsigned char* ring = smem + (of_v ? SM::VRING : SM::KRING) + 2 * w * SM::PAGE;
+            const __half* facts = reinterpret_cast<const __half*>(smem + SM::FACT) + of_v * TR_KEYS + 2 * w * PIKV_PAGE_TOKENS + tr_row(lane);
             unsigned char* tile = smem + (of_v ? SM::V : SM::K);
-            const uint32_t full = of_v ? vr_full : kr_full, empty = of_v ? vr_empty : kr_empty, read = of_v ? pv_done : s_full, ready = of_v ? v_full : k_full;
+            const uint32_t full = of_v ? vr_full : kr_full, empty = of_v ? vr_empty : kr_empty, read = of_v ? pv_done : s_full, ready = of_v ? v_full : k_full,
+                           sides = of_v ? v_side : k_side;
             int s = 0;
             uint32_t ph = 0;
             for (int n = 0; n < count; ++n) {
-                const int left = cur.end() - cur.tile * TR_KEYS;                   // rows of the tile inside the stream
-                if (TR_RARE(!tr_wait(full + 8 * s, ph))) { failed = true; break; }
+                if (TR_RARE(!tr_wait2(full + 8 * s, ph, sides + 8 * tr_set(n), tr_set_phase(n)))) { failed = true; break; }
                 TRPage<BITS> x0, x1;
-                x0.load(ring + (s * TR_PAGES + 2 * w) * SM::PAGE, at);             // (what a page behind the end left there is finite)
-                x1.load(ring + (s * TR_PAGES + 2 * w + 1) * SM::PAGE, at);
-                // the tile's exponent: lane = two neighbouring rows of page lane / 8; rows behind the end have no scale
-                const unsigned char* meta = metas + s * TR_PAGES * SM::META;
-                uint32_t two = 2 * lane < left ? *reinterpret_cast<const uint32_t*>(meta + (lane >> 3) * SM::META + (lane & 7) * 4) : 0u;
-                if (2 * lane + 1 == left) two &= 0xffffu;
-                const int e = __reduce_max_sync(0xffffffffu, max(tr_exponent(two << 16), tr_exponent(two & 0xffff0000u)));
-                // factors of this lane's rows: r0 and 8 on of both pages.  A K that is not finite makes its logit so; a V enters as zeros
-                const float up = exp2_int(15 - e);
-                auto factor = [&](int page, int r) {
-                    const uint32_t x = page * PIKV_PAGE_TOKENS + r < left ? (uint32_t)reinterpret_cast<const uint16_t*>(meta + page * SM::META)[r] << 16 : 0u;
-                    return __uint_as_float(of_v && (x & 0x7f800000u) == 0x7f800000u ? 0u : x) * up;
-                };
-                const float a00 = factor(2 * w, r0), a01 = factor(2 * w, r0 + 8), a10 = factor(2 * w + 1, r0), a11 = factor(2 * w + 1, r0 + 8);
-                // What the softmax needs of the tile.  The four sets need no wait of their own: the one written here served tile n - 4,
-                // whose second product was issued before the Q K^T of tile n - 2, and these warps have seen that one, or the second
-                // product of tile n - 2, done
-                float* of = reinterpret_cast<float*>(smem + SM::VEXP + (n & 3) * 16);
-                if (!of_v) {
-                    if (w == 0 && lane == 0) of[0] = exp2_int(e + 9);
-                } else {
-                    const uint32_t odd0 = __ballot_sync(0xffffffffu, (two & 0x7f80u) == 0x7f80u), odd1 = __ballot_sync(0xffffffffu, (two & 0x7f800000u) == 0x7f800000u);
-                    if (w == 0 && lane == 0) {
-                        of[1] = (float)(e + 9);
-                        of[2] = exp2_int(-9 - e);
-                        of[3] = __uint_as_float(odd0 | odd1);
-                        *reinterpret_cast<uint2*>(smem + SM::ODD + (n & 3) * 8) = make_uint2(odd0, odd1);
-                    }
-                }
-                if (BITS == 4) {
-                    const int page = 2 * w + (lane >> 4), r = lane & 15;
-                    const unsigned char* own = meta + page * SM::META;
-                    reinterpret_cast<float*>(smem + SM::SIDE)[((n & 3) * 2 + of_v) * TR_KEYS + 32 * w + lane] =
-                        32 * w + lane < left ? (reinterpret_cast<const float*>(own + 32)[r] - 8.f) *
-                                                   (__uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(own)[r] << 16) * exp2_int(-9 - e))
-                                             : 0.f;
-                }
+                x0.load(ring + s * TR_PAGES * SM::PAGE, at);                       // (what a page behind the end left there is finite)
+                x1.load(ring + s * TR_PAGES * SM::PAGE + SM::PAGE, at);
+                const __half* f = facts + tr_set(n) * 2 * TR_KEYS;
+                const __half2 a0[2] = {__half2half2(f[0]), __half2half2(f[8])}, a1[2] = {__half2half2(f[16]), __half2half2(f[24])};
                 __syncwarp();
-                if (lane == 0) lr_mbar_arrive(side_full + 8 * (n & 3));
+                if (lane == 0) lr_mbar_arrive(empty + 8 * s);
                 // the product of the tile before has read the buffer
                 if (n > 0 && TR_RARE(!tr_wait(read + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) { failed = true; break; }
-                x0.store(tile, 2 * w, lane, a00, a01);
-                x1.store(tile, 2 * w + 1, lane, a10, a11);
+                x0.store(tile, 2 * w, lane, a0);
+                x1.store(tile, 2 * w + 1, lane, a1);
                 tr_fence_smem();
                 __syncwarp();
-                if (lane == 0) {
-                    lr_mbar_arrive(ready);
-                    lr_mbar_arrive(empty + 8 * s);
-                }
+                if (lane == 0) lr_mbar_arrive(ready);
                 if (++s == ahead) s = 0, ph ^= 1u;
-                if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
             }
         } else {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
@@ -599,7 +615,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             // one tile: scores out, weights in.  EDGE: some of its positions lie behind the context
             auto step = [&](auto edge_c, int n, int tile, bool first) {
                 constexpr bool EDGE = decltype(edge_c)::value;
-                if (TR_RARE(!tr_wait2(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u, side_full + 8 * (n & 3), (uint32_t)(n >> 2) & 1u))) return false;
+                if (TR_RARE(!tr_wait2(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u, v_side + 8 * tr_set(n), tr_set_phase(n)))) return false;
                 if (!warp_live) {
                     if (lane == 0) lr_mbar_arrive(p_full + 8 * (n & 1));
                     return true;
@@ -609,9 +625,9 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 float x0[32], x1[32];
                 tr_tmem_ld32(scores, x0);
                 tr_tmem_ld32(scores + 32, x1);
-                const float* kz = reinterpret_cast<const float*>(smem + SM::SIDE) + (n & 3) * SM::SIDES * TR_KEYS;      // 4 bit only
+                const float* kz = reinterpret_cast<const float*>(smem + SM::SIDE) + tr_set(n) * SM::SIDES * TR_KEYS;      // 4 bit only
                 const float* vz = kz + TR_KEYS;
-                const float4 of = *reinterpret_cast<const float4*>(smem + SM::VEXP + (n & 3) * 16);
+                const float4 of = *reinterpret_cast<const float4*>(smem + SM::VEXP + tr_set(n) * 16);
                 float mul = qmul * of.x;
                 if (mul == 0.f) mul = 1.17549435e-38f;                   // (masked scores are -infinity: times 0 they would not be a number)
                 uint64_t seen = ~0ull;
@@ -621,7 +637,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     seen = sh >= 0 ? (sh < 64 ? tree << sh : 0ull) | (sh < 64 ? (1ull << sh) - 1 : ~0ull) : (sh > -64 ? tree >> -sh : 0ull);
                 }
                 if (TR_RARE(__float_as_uint(of.w) != 0u)) {
-                    const uint2 odd = *reinterpret_cast<const uint2*>(smem + SM::ODD + (n & 3) * 8);
+                    const uint2 odd = *reinterpret_cast<const uint2*>(smem + SM::ODD + tr_set(n) * 8);
                     for (int j = 0; j < TR_KEYS; ++j)
                         if (((j & 1 ? odd.y : odd.x) >> (j >> 1)) & (uint32_t)(seen >> j) & 1u) odd_v = __uint_as_float(0x7fffffffu);
                 }
