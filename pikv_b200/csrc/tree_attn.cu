@@ -54,8 +54,10 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // largest scale): one rounding, 2^-11 of the entry, the size of the weights' own; in return the softmax neither loads nor
 // multiplies by the scales (shared-memory reads of the scales by every row were the busiest pipe of the kernel that applied
 // them to exact integer products: 16 x 16384 x 32 nodes, 248 -> 221 us).
-//   logit = 2^(e_k + 9) / sqrt(128) (q . K16 - z)      z: the zero points' part, (zp - 8) scale sum(q), 4 bit only
-//   O     = sum w V16 - sum w z_v,  w = f16(2^(logit - R + e_v + 9))
+//   logit = 2^(e_k + 9) / sqrt(128) q . K16
+//   O     = sum w V16,  w = f16(2^(logit - R + e_v + 9))
+// A 4-bit code has its zero point taken off first, exactly where that is a whole number below 2048 (with the zero points' parts
+// as products of their own in the softmax, it had to reload registers as well: 24 ragged streams to 6001, 103 -> 78 us).
 // R is a row's reference: the largest logit (log2 domain) plus e_v + 9 of the tile it was seen in, so that the weights sit at
 // the top of f16's range whatever the size of V; it moves only when a tile exceeds it by 2^TR_SLACK.  The denominator is
 // the fp32 sum of 2^(logit - R).  A row of V that is not finite enters as zeros and makes the result of the rows that see it
@@ -82,16 +84,15 @@ constexpr int TR_SETS = 8;                                                      
 
 // shared memory behind a 1024-byte boundary
 template <int BITS> struct TRSmem {
-    static constexpr int SIDES = BITS == 8 ? 0 : 2;
+    static constexpr int FACTOR = BITS == 8 ? 2 : 8;                            // bytes of a row's factors
     static constexpr int PAGE = 256 * BITS, META = BITS == 8 ? 32 : 96;        // codes of a page of one head; its scales (and zero points)
     static constexpr int Q = 0, K = Q + 2 * TR_ROWS * 128, V = K + TR_TILE,
                          KRING = V + TR_TILE,                                  // [ahead][page of the tile] codes of K
                          VRING = KRING + TR_K_AHEAD * TR_PAGES * PAGE,
                          KMETA = VRING + TR_V_AHEAD * TR_PAGES * PAGE,         // [ahead][page] scales, zero points of K, of V
                          VMETA = KMETA + TR_K_AHEAD * TR_PAGES * META,
-                         SIDE = VMETA + TR_V_AHEAD * TR_PAGES * META,          // 4 bit: [sets][2][64] fp32: z of K, of V
-                         FACT = SIDE + TR_SETS * SIDES * TR_KEYS * 4,          // [sets][2][64] f16: factors of the rows of K, of V
-                         VEXP = FACT + TR_SETS * 2 * TR_KEYS * 2,              // [sets] 2^(e_k + 9), e_v + 9, 2^-(e_v + 9) as floats, whether a row of V is not finite
+                         FACT = VMETA + TR_V_AHEAD * TR_PAGES * META,          // [sets][2][64] factors of the rows of K, of V
+                         VEXP = FACT + TR_SETS * 2 * TR_KEYS * FACTOR,              // [sets] 2^(e_k + 9), e_v + 9, 2^-(e_v + 9) as floats, whether a row of V is not finite
                          ODD = VEXP + TR_SETS * 16,                            // [sets][2] even and odd rows of V that are not finite, a bit each
                          BARS = ODD + TR_SETS * 8, NBARS = 9 + 2 * TR_SETS + 2 * (TR_K_AHEAD + TR_V_AHEAD),
                          PRE = BARS + NBARS * 8, MISC = PRE + (PIKV_STREAMS_PER_LAUNCH + 1) * 4, END = MISC + 16;
@@ -261,6 +262,23 @@ __device__ __forceinline__ void tr_bulk(uint32_t dst, const void* src, uint32_t 
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
+// What makes an entry of a row's codes: 8 bit a n 2^-24 + b, 4 bit a (n 2^-24 + c) + b (b 0 where c and a are exact, otherwise what
+// their roundings left out)
+template <int BITS> struct TRFactor {
+    __half2 a, b, c;
+    __device__ __forceinline__ void load(const unsigned char* f) {
+        if constexpr (BITS == 8) {
+            a = __half2half2(*reinterpret_cast<const __half*>(f));
+            b = __hmul2(a, __float2half2_rn(-128.f / 16777216.f));
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(f);
+            const __half2 ac = *reinterpret_cast<const __half2*>(&x.x), b0 = *reinterpret_cast<const __half2*>(&x.y);
+            a = __low2half2(ac);
+            c = __high2half2(ac);
+            b = b0;
+        }
+    }
+};
 template <int BITS> struct TRPage {
     uint32_t w[4][BITS / 2];
     __device__ __forceinline__ void load(const unsigned char* page, int at) {
@@ -277,52 +295,51 @@ template <int BITS> struct TRPage {
             }
         }
     }
-    // A byte or nibble n in the low bits of an f16 is n 2^-24, exactly (a subnormal).  With a = scale 2^(15 - e) and b the offset's
-    // part, the fused a n 2^-24 + b is (n - offset) scale 2^(-9 - e), rounded once.
+    // A byte or nibble n in the low bits of an f16 is n 2^-24, exactly (a subnormal).  With a = scale 2^(15 - e), the fused
+    // a n 2^-24 + b is (n - 128) scale 2^(-9 - e), rounded once, b the offset's part.
     static __device__ __forceinline__ uint32_t fma2(uint32_t x, __half2 a, __half2 b) {
         const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
-    // a: factors of rows base and base + 8
-    __device__ __forceinline__ void store(unsigned char* tile, int page, int lane, const __half2 (&a)[2]) const {
+    // f0, f1: factors of rows base and base + 8
+    __device__ __forceinline__ void store(unsigned char* tile, int page, int lane, const TRFactor<BITS>& f0, const TRFactor<BITS>& f1) const {
         const int r = tr_row(lane), c = lane & 3;
         unsigned char* row = tile + (page * PIKV_PAGE_TOKENS + r) * 128;
         const int d0 = 16 * ((2 * c) ^ (r & 7)), d1 = 16 * ((2 * c + 1) ^ (r & 7));
-        const __half2 offset = __float2half2_rn((BITS == 8 ? -128.f : -8.f) / 16777216.f), b[2] = {__hmul2(a[0], offset), __hmul2(a[1], offset)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             unsigned char* to = row + (i & 1) * TR_KEYS * 128 + (i >> 1) * 8 * 128;
-            const __half2 s = a[i >> 1], o = b[i >> 1];
+            const TRFactor<BITS>& f = i >> 1 ? f1 : f0;
             if constexpr (BITS == 8) {
                 uint32_t x[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) x[k] = w[i][k] ^ 0x80808080u;             // code + 128
-                auto pair = [&](int k, uint32_t sel) { return fma2(__byte_perm(x[k], 0u, sel), s, o); };
+                auto pair = [&](int k, uint32_t sel) { return fma2(__byte_perm(x[k], 0u, sel), f.a, f.b); };
                 *reinterpret_cast<uint4*>(to + d0) = make_uint4(pair(0, 0x4140), pair(0, 0x4342), pair(1, 0x4140), pair(1, 0x4342));
                 *reinterpret_cast<uint4*>(to + d1) = make_uint4(pair(2, 0x4140), pair(2, 0x4342), pair(3, 0x4140), pair(3, 0x4342));
             } else {
-                auto pair = [&](uint32_t x) { return fma2(x & 0x000f000fu, s, o); };
+                auto low = [&](uint32_t x) {
+                    x &= 0x000f000fu;
+                    const __half2 t = __hadd2(*reinterpret_cast<const __half2*>(&x), f.c);
+                    return fma2(*reinterpret_cast<const uint32_t*>(&t), f.a, f.b);
+                };
+                auto high = [&](uint32_t x) {                                          // n 2^-20
+                    return fma2(fma2(x & 0x00f000f0u, __float2half2_rn(0.0625f), f.c), f.a, f.b);
+                };
                 const uint32_t x = w[i][0], y = w[i][1];
-                *reinterpret_cast<uint4*>(to + d0) = make_uint4(pair(x), pair(x >> 4), pair(x >> 8), pair(x >> 12));
-                *reinterpret_cast<uint4*>(to + d1) = make_uint4(pair(y), pair(y >> 4), pair(y >> 8), pair(y >> 12));
+                *reinterpret_cast<uint4*>(to + d0) = make_uint4(low(x), high(x), low(x >> 8), high(x >> 8));
+                *reinterpret_cast<uint4*>(to + d1) = make_uint4(low(y), high(y), low(y >> 8), high(y >> 8));
             }
         }
     }
 };
 
-// 32 products of a row to scores, in place: the zero points' part off (4 bit), what `open` has no bit for to -infinity; returns the
-// largest.  kz: z of K of these keys
-template <int BITS, bool EDGE>
-__device__ __forceinline__ float tr_scores(float (&x)[32], const float* kz, float qsum, uint32_t open) {
+// the largest of 32 products of a row; what `open` has no bit for becomes -infinity
+template <bool EDGE>
+__device__ __forceinline__ float tr_scores(float (&x)[32], uint32_t open) {
     float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-        if (BITS == 4) {
-            const float4 z4 = *reinterpret_cast<const float4*>(kz + j);
-            const float2 a = tr_fma2(make_float2(z4.x, z4.y), make_float2(-qsum, -qsum), make_float2(x[j], x[j + 1]));
-            const float2 c = tr_fma2(make_float2(z4.z, z4.w), make_float2(-qsum, -qsum), make_float2(x[j + 2], x[j + 3]));
-            x[j] = a.x; x[j + 1] = a.y; x[j + 2] = c.x; x[j + 3] = c.y;
-        }
         if (EDGE) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -333,10 +350,9 @@ __device__ __forceinline__ float tr_scores(float (&x)[32], const float* kz, floa
     }
     return fmaxf(m0, m1);
 }
-// 32 scores to weights f16(2^(score mul + off)), their sum and (4 bit) the sum of their zero points' parts; vz: z of V
-template <int BITS, bool EDGE>
-__device__ __forceinline__ void tr_weights(const float (&x)[32], uint32_t (&wgt)[16], const float* vz, float mul, float off, uint32_t open, float& total, float& corr) {
-    float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f), zsum = make_float2(0.f, 0.f);
+// 32 scores to weights f16(2^(score mul + off)), and their sum
+__device__ __forceinline__ void tr_weights(const float (&x)[32], uint32_t (&wgt)[16], float mul, float off, float& total) {
+    float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
         float2 a = tr_fma2(make_float2(x[j], x[j + 1]), make_float2(mul, mul), make_float2(off, off));
@@ -347,23 +363,9 @@ __device__ __forceinline__ void tr_weights(const float (&x)[32], uint32_t (&wgt)
         s1 = tr_add2(s1, c);
         wgt[j / 2] = tr_pack(a.x, a.y);
         wgt[j / 2 + 1] = tr_pack(c.x, c.y);
-        if (BITS == 4) {
-            float4 z4 = *reinterpret_cast<const float4*>(vz + j);
-            if (EDGE) {                                                  // 0 times something that need not be finite
-                if (!((open >> j) & 1u)) z4.x = 0.f;
-                if (!((open >> (j + 1)) & 1u)) z4.y = 0.f;
-                if (!((open >> (j + 2)) & 1u)) z4.z = 0.f;
-                if (!((open >> (j + 3)) & 1u)) z4.w = 0.f;
-            }
-            const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2]));
-            const float2 rc = __half22float2(*reinterpret_cast<const __half2*>(&wgt[j / 2 + 1]));
-            zsum = tr_fma2(ra, make_float2(z4.x, z4.y), zsum);
-            zsum = tr_fma2(rc, make_float2(z4.z, z4.w), zsum);
-        }
     }
     s0 = tr_add2(s0, s1);
     total += s0.x + s0.y;
-    if (BITS == 4) corr += zsum.x + zsum.y;
 }
 
 template <int BITS>
@@ -520,21 +522,34 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     const unsigned char* own = smem + (OF_V ? SM::VMETA : SM::KMETA) + (s * TR_PAGES + (lane >> 3)) * SM::META;
                     uint32_t two = 2 * lane < left ? *reinterpret_cast<const uint32_t*>(own + (lane & 7) * 4) : 0u;     // rows behind the end have none
                     if (2 * lane + 1 == left) two &= 0xffffu;
-                    const int e = __reduce_max_sync(0xffffffffu, max(tr_exponent(two << 16), tr_exponent(two & 0xffff0000u)));
-                    const float up = exp2_int(15 - e);
-                    const bool odd0 = (two & 0x7f80u) == 0x7f80u, odd1 = (two & 0x7f800000u) == 0x7f800000u;
-                    // a K that is not finite makes its logit so; a V enters as zeros
-                    const float a0 = OF_V && odd0 ? 0.f : __uint_as_float(two << 16) * up, a1 = OF_V && odd1 ? 0.f : __uint_as_float(two & 0xffff0000u) * up;
-                    reinterpret_cast<uint32_t*>(smem + SM::FACT)[(tr_set(n) * 2 + OF_V) * (TR_KEYS / 2) + lane] = tr_pack(a0, a1);
+                    const float s0 = __uint_as_float(two << 16), s1 = __uint_as_float(two & 0xffff0000u);
+                    float z0 = 0.f, z1 = 0.f, top0 = s0, top1 = s1;               // top: a sixteenth of a row's largest entry, 4 bit
                     if (BITS == 4) {
-                        float2 z = make_float2(0.f, 0.f);
                         if (2 * lane < left) {
                             const float2 zp = *reinterpret_cast<const float2*>(own + 32 + (lane & 7) * 8);
-                            const float down = exp2_int(-9 - e);
-                            z.x = (zp.x - 8.f) * (__uint_as_float(two << 16) * down);
-                            if (2 * lane + 1 < left) z.y = (zp.y - 8.f) * (__uint_as_float(two & 0xffff0000u) * down);
+                            z0 = zp.x;
+                            if (2 * lane + 1 < left) z1 = zp.y;
                         }
-                        reinterpret_cast<float2*>(smem + SM::SIDE)[(tr_set(n) * 2 + OF_V) * (TR_KEYS / 2) + lane] = z;
+                        if (!(fabsf(z0) <= 16.f)) top0 = s0 * (fabsf(z0) * 0.0625f);
+                        if (!(fabsf(z1) <= 16.f)) top1 = s1 * (fabsf(z1) * 0.0625f);
+                    }
+                    const int e = __reduce_max_sync(0xffffffffu, max(tr_exponent(__float_as_uint(top0)), tr_exponent(__float_as_uint(top1))));
+                    const bool odd0 = !(fabsf(top0) < INFINITY), odd1 = !(fabsf(top1) < INFINITY);
+                    // a K that is not finite makes its logit so; a V enters as zeros
+                    const float up = exp2_int(15 - e), a0 = OF_V && odd0 ? 0.f : s0 * up, a1 = OF_V && odd1 ? 0.f : s1 * up;
+                    unsigned char* fact = smem + SM::FACT + ((tr_set(n) * 2 + OF_V) * TR_KEYS + 2 * lane) * SM::FACTOR;
+                    if constexpr (BITS == 8) {
+                        *reinterpret_cast<uint32_t*>(fact) = tr_pack(a0, a1);
+                    } else {
+                        constexpr float UNIT = 1.f / 16777216.f;
+                        auto factors = [&](float a, float z) {
+                            const uint32_t ac = tr_pack(a, -z * UNIT);
+                            const float2 got = __half22float2(*reinterpret_cast<const __half2*>(&ac));
+                            const float b = -z * UNIT * a - got.x * got.y;
+                            return make_uint2(ac, tr_pack(b, b));
+                        };
+                        const uint2 f0 = factors(a0, OF_V && odd0 ? 0.f : z0), f1 = factors(a1, OF_V && odd1 ? 0.f : z1);
+                        *reinterpret_cast<uint4*>(fact) = make_uint4(f0.x, f0.y, f1.x, f1.y);
                     }
                     float* of = reinterpret_cast<float*>(smem + SM::VEXP + tr_set(n) * 16);
                     if (OF_V) {
@@ -577,7 +592,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             const int w = (warp - TR_K) & 1, count = f1 - f0, ahead = of_v ? TR_V_AHEAD : TR_K_AHEAD;
             const int at = tr_place<BITS>(lane);
             const unsigned char* ring = smem + (of_v ? SM::VRING : SM::KRING) + 2 * w * SM::PAGE;
-            const __half* facts = reinterpret_cast<const __half*>(smem + SM::FACT) + of_v * TR_KEYS + 2 * w * PIKV_PAGE_TOKENS + tr_row(lane);
+            const unsigned char* facts = smem + SM::FACT + (of_v * TR_KEYS + 2 * w * PIKV_PAGE_TOKENS + tr_row(lane)) * SM::FACTOR;
             unsigned char* tile = smem + (of_v ? SM::V : SM::K);
             const uint32_t full = of_v ? vr_full : kr_full, empty = of_v ? vr_empty : kr_empty, read = of_v ? pv_done : s_full, ready = of_v ? v_full : k_full,
                            sides = of_v ? v_side : k_side;
@@ -588,14 +603,18 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 TRPage<BITS> x0, x1;
                 x0.load(ring + s * TR_PAGES * SM::PAGE, at);                       // (what a page behind the end left there is finite)
                 x1.load(ring + s * TR_PAGES * SM::PAGE + SM::PAGE, at);
-                const __half* f = facts + tr_set(n) * 2 * TR_KEYS;
-                const __half2 a0[2] = {__half2half2(f[0]), __half2half2(f[8])}, a1[2] = {__half2half2(f[16]), __half2half2(f[24])};
+                const unsigned char* f = facts + tr_set(n) * 2 * TR_KEYS * SM::FACTOR;
+                TRFactor<BITS> f00, f01, f10, f11;
+                f00.load(f);
+                f01.load(f + 8 * SM::FACTOR);
+                f10.load(f + 16 * SM::FACTOR);
+                f11.load(f + 24 * SM::FACTOR);
                 __syncwarp();
                 if (lane == 0) lr_mbar_arrive(empty + 8 * s);
                 // the product of the tile before has read the buffer
                 if (n > 0 && TR_RARE(!tr_wait(read + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) { failed = true; break; }
-                x0.store(tile, 2 * w, lane, a0);
-                x1.store(tile, 2 * w + 1, lane, a1);
+                x0.store(tile, 2 * w, lane, f00, f01);
+                x1.store(tile, 2 * w + 1, lane, f10, f11);
                 tr_fence_smem();
                 __syncwarp();
                 if (lane == 0) lr_mbar_arrive(ready);
@@ -606,7 +625,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             cur.start(d, pre, f0);
             // ---- softmax: thread = row ----
             const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-            float qmul = 0.f, qsum = 0.f, ref = -INFINITY, den = 0.f, corr = 0.f;
+            float qmul = 0.f, ref = -INFINITY, den = 0.f;
             float odd_v = 0.f;                                        // not a number once the row has seen a V that is not finite
             uint64_t tree = 0;
             int node = 0;
@@ -625,8 +644,6 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 float x0[32], x1[32];
                 tr_tmem_ld32(scores, x0);
                 tr_tmem_ld32(scores + 32, x1);
-                const float* kz = reinterpret_cast<const float*>(smem + SM::SIDE) + tr_set(n) * SM::SIDES * TR_KEYS;      // 4 bit only
-                const float* vz = kz + TR_KEYS;
                 const float4 of = *reinterpret_cast<const float4*>(smem + SM::VEXP + tr_set(n) * 16);
                 float mul = qmul * of.x;
                 if (mul == 0.f) mul = 1.17549435e-38f;                   // (masked scores are -infinity: times 0 they would not be a number)
@@ -643,7 +660,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 }
                 tr_tmem_ld_wait(x0);
                 tr_tmem_ld_wait(x1);
-                const float mx = fmaxf(tr_scores<BITS, EDGE>(x0, kz, qsum, (uint32_t)seen), tr_scores<BITS, EDGE>(x1, kz + 32, qsum, (uint32_t)(seen >> 32)));
+                const float mx = fmaxf(tr_scores<EDGE>(x0, (uint32_t)seen), tr_scores<EDGE>(x1, (uint32_t)(seen >> 32)));
                 // does the reference hold?  (-inf while nothing has been seen)
                 const float want = mx * mul + of.y;
                 const bool move = mx > -INFINITY && want > ref + TR_SLACK;
@@ -652,7 +669,6 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     const float fac = move ? tr_ex2(ref - next) : 1.f;     // 0 from -inf
                     ref = next;
                     den *= fac;
-                    corr *= fac;
                     if (!first) {
                         if (TR_RARE(!tr_wait(pv_done + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) return false;
                         tr_fence_after();
@@ -672,9 +688,9 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 float total = 0.f;
                 // the weights take the place of the scores that they come from, two to a column
                 uint32_t wgt[16];
-                tr_weights<BITS, EDGE>(x0, wgt, vz, mul, off, (uint32_t)seen, total, corr);
+                tr_weights(x0, wgt, mul, off, total);
                 tr_tmem_st16(scores, wgt);
-                tr_weights<BITS, EDGE>(x1, wgt, vz + 32, mul, off, (uint32_t)(seen >> 32), total, corr);
+                tr_weights(x1, wgt, mul, off, total);
                 tr_tmem_st16(scores + 16, wgt);
                 den += total * of.z;
                 tr_tmem_st_wait();
@@ -692,7 +708,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 live = node < cur.nodes;
                 warp_live = __any_sync(0xffffffffu, live);
                 ref = -INFINITY;
-                den = corr = odd_v = 0.f;
+                den = odd_v = 0.f;
                 if (warp_live) {
                     out_row = ((size_t)cur.b * d.N + (live ? node : 0)) * d.n_q + (size_t)h * d.G + row % d.G;
                     const uint4* src = reinterpret_cast<const uint4*>(d.q + out_row * 128);
@@ -710,7 +726,6 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     const float amax = __uint_as_float(top), odd = top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : 0.f;
                     const int sh = amax > 0.f && amax < INFINITY ? min(126, 14 - ((int)(__float_as_uint(amax) >> 23) - 127)) : 0;
                     const float up = exp2_int(max(sh, -126));
-                    qsum = 0.f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float x[8];
@@ -719,10 +734,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                         bf16x2_to_f32(q4[i].z, x[4], x[5]);
                         bf16x2_to_f32(q4[i].w, x[6], x[7]);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            x[k] *= up;
-                            if (BITS == 4) qsum += x[k];
-                        }
+                        for (int k = 0; k < 8; ++k) x[k] *= up;
                         uint4 y;
                         y.x = tr_pack(x[tr_channel<BITS>(0)], x[tr_channel<BITS>(1)]);
                         y.y = tr_pack(x[tr_channel<BITS>(2)], x[tr_channel<BITS>(3)]);
@@ -767,7 +779,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                         if (BITS == 4) {
                             float t[32];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) t[tr_channel<BITS>(i)] = o[i] - corr;
+                            for (int i = 0; i < 32; ++i) t[tr_channel<BITS>(i)] = o[i];
 #pragma unroll
                             for (int i = 0; i < 32; ++i) o[i] = t[i];
                         }

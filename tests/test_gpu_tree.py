@@ -90,6 +90,39 @@ def test_tree_masks_and_sizes(bits, N, G, n_kv, shared):
     compare(cache, q, mask, ctx, nodes, out, lse, ids)
 
 
+def test_tree_zero_points():
+    """4-bit rows of one value, whose zero points are millions, between ordinary ones; zero points that are not whole numbers."""
+    ctx, N, n_kv = [150, 64], 9, 2
+    cache, gen = filled_cache([n + N for n in ctx], n_kv, 4, seed=11)
+    for s, n in enumerate(ctx):
+        k, v = (torch.randn(n, n_kv * D, generator=gen, device="cuda") for _ in range(2))
+        k[1::3] = torch.randn(len(k[1::3]), 1, generator=gen, device="cuda")
+        v[2::3] = 30 * torch.randn(len(v[2::3]), 1, generator=gen, device="cuda")
+        k[5], v[7] = 0, 0
+        append_rows(cache, s, 0, k.bfloat16(), v.bfloat16())
+    assert float(torch.nan_to_num(cache.k_zp).abs().max()) > 1e5
+    q = torch.randn(2, N, 4 * n_kv, D, generator=gen, device="cuda").bfloat16()
+    mask = random_trees(gen, 2, N)
+    length = torch.tensor(ctx, dtype=torch.int32, device="cuda")
+
+    def check():
+        out, lse = cache.decode_attention_tree(q, mask, ctx_len=length, want_lse=True)
+        cache.check_status()
+        for b, n in enumerate(ctx):
+            k, v = rows64(cache, b, n + N)
+            sees = torch.cat([torch.ones(N, n, dtype=torch.bool, device="cuda"), mask[b]], 1)
+            # An entry (code - zero point) scale is rounded twice here, by 2^-11 each (the difference, where it is above 2048 steps, and
+            # the entry), and what a factor lost comes back rounded by 2^-11 of at most 2^-10 of it; the dequantised rows that it is
+            # compared with are rounded to fp32 twice.  Units: 2^-25 where the tile's largest row has entries above 2^-6, of its own
+            value = 2.0 ** -10 + 2.0 ** -20 + 2.0 ** -19
+            check_attention(out[b], lse[b], *attend64(q[b], k, v, sees), value + (2 * 128 + 8) * 2.0 ** -24, value)
+
+    check()
+    for zp in (cache.k_zp, cache.v_zp):
+        zp.add_(torch.rand(zp.shape, generator=gen, device="cuda") - 0.5)
+    check()
+
+
 def test_tree_layouts():
     """Strided and unaligned queries, a strided mask."""
     N, n_q, n_kv = 9, 8, 2
