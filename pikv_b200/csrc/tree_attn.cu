@@ -67,38 +67,36 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // burst, 235 us in long runs under the power cap (the bytes alone take 85 us, the products 82).  Bound by the conversions, the
 // weights and their handing over: 3180 warp instructions per tile (1126 convert K and V, 548 make weights, 150 read scores) in
 // 0.56 of the issue slots, tensor pipe 36 %, DRAM 35 %.  No single pipe is full; the 24 warps wait for one another.
-constexpr int TR_THREADS = 384;          // three warpgroups
+constexpr int TR_THREADS = 384;          // of a half: three warpgroups
 constexpr int TR_K = 4, TR_V = 6, TR_MMA = 8, TR_COPY = 9, TR_SCALES = 11;      // first warps of each kind
 constexpr int TR_ROWS = 128;             // rows of a unit
 constexpr int TR_KEYS = 64;              // keys of a tile
 constexpr int TR_PAGES = TR_KEYS / PIKV_PAGE_TOKENS;
-constexpr int TR_CTAS = 2;               // per SM
-constexpr int TR_MIN_TILES = 1;          // per CTA
 constexpr float TR_SLACK = 8.f;
 constexpr unsigned TR_WAIT_LIMIT = 1u << 24;
-constexpr uint32_t TR_COL_O = 0, TR_COL_S = 128, TR_COLS = 256;      // S of even and odd tiles, the weights in its first columns
+constexpr uint32_t TR_COL_O = 0, TR_COL_S = 128, TR_COLS = 256;      // of a half: S of even and odd tiles, the weights in its first columns
 
 constexpr int TR_TILE = 2 * TR_KEYS * 128;                                     // bytes of a tile of f16: [2 halves of the channels][64 keys][128 bytes]
 constexpr int TR_K_AHEAD = 3, TR_V_AHEAD = 2;                                   // tiles whose copies are on their way
 constexpr int TR_SETS = 8;                                                      // tiles whose scales are kept as the warps want them
 
-// shared memory behind a 1024-byte boundary
-template <int BITS> struct TRSmem {
+// shared memory behind a 1024-byte boundary, of a CTA of H halves
+template <int BITS, int H> struct TRSmem {
     static constexpr int FACTOR = BITS == 8 ? 2 : 8;                            // bytes of a row's factors
     static constexpr int PAGE = 256 * BITS, META = BITS == 8 ? 32 : 96;        // codes of a page of one head; its scales (and zero points)
-    static constexpr int Q = 0, K = Q + 2 * TR_ROWS * 128, V = K + TR_TILE,
-                         KRING = V + TR_TILE,                                  // [ahead][page of the tile] codes of K
+    static constexpr int QTILE = 2 * TR_ROWS * 128;
+    static constexpr int Q = 0, K = Q + H * QTILE, V = K + H * TR_TILE,        // [H] each
+                         KRING = V + H * TR_TILE,                              // [ahead][page of the tile] codes of K
                          VRING = KRING + TR_K_AHEAD * TR_PAGES * PAGE,
                          KMETA = VRING + TR_V_AHEAD * TR_PAGES * PAGE,         // [ahead][page] scales, zero points of K, of V
                          VMETA = KMETA + TR_K_AHEAD * TR_PAGES * META,
                          FACT = VMETA + TR_V_AHEAD * TR_PAGES * META,          // [sets][2][64] factors of the rows of K, of V
-                         VEXP = FACT + TR_SETS * 2 * TR_KEYS * FACTOR,              // [sets] 2^(e_k + 9), e_v + 9, 2^-(e_v + 9) as floats, whether a row of V is not finite
+                         VEXP = FACT + TR_SETS * 2 * TR_KEYS * FACTOR,         // [sets] 2^(e_k + 9), e_v + 9, 2^-(e_v + 9) as floats, whether a row of V is not finite
                          ODD = VEXP + TR_SETS * 16,                            // [sets][2] even and odd rows of V that are not finite, a bit each
-                         BARS = ODD + TR_SETS * 8, NBARS = 9 + 2 * TR_SETS + 2 * (TR_K_AHEAD + TR_V_AHEAD),
+                         BARS = ODD + TR_SETS * 8, NBARS = 4 + 7 * H + 2 * TR_SETS + 2 * (TR_K_AHEAD + TR_V_AHEAD),
                          PRE = BARS + NBARS * 8, MISC = PRE + (PIKV_STREAMS_PER_LAUNCH + 1) * 4, END = MISC + 16;
     static constexpr int BYTES = END + 1024;
 };
-
 __device__ __forceinline__ uint32_t tr_set(int n) { return (uint32_t)n % TR_SETS; }
 __device__ __forceinline__ uint32_t tr_set_phase(int n) { return (uint32_t)n / TR_SETS & 1u; }
 
@@ -106,24 +104,26 @@ __device__ __forceinline__ uint32_t tr_set_phase(int n) { return (uint32_t)n / T
 #define TR_RARE(x) __builtin_expect(!!(x), 0)
 
 struct TreeParts {
-    float* o;                            // [2 C][rows][128]
-    float2* ml;                          // [2 C][rows] reference and denominator
+    float* o;                            // [C][2][halves][rows][128]
+    float2* ml;                          // [C][2][halves][rows] reference and denominator
     int* plan;                           // [0] tiles per CTA, [1 ..] prefix of the streams' tiles
     int rows;                            // rows of a slot
+    int halves;                          // of a CTA
 };
 
 __device__ __forceinline__ int tree_tiles(int ctx, int nodes) { return (ctx + nodes + TR_KEYS - 1) / TR_KEYS; }
-__device__ __forceinline__ int tree_row_tiles(int nodes, int G) { return (nodes * G + TR_ROWS - 1) / TR_ROWS; }
+// units of a head: TR_ROWS rows for each half of a CTA
+__device__ __forceinline__ int tree_row_tiles(int nodes, int G, int halves) { return (nodes * G + halves * TR_ROWS - 1) / (halves * TR_ROWS); }
 
-// a place in the list of tiles: stream b, unit (head, 128 rows) of it, tile of the unit
-struct TreeCursor {
+// a place in the list of tiles: stream b, unit (head, H x 128 rows) of it, tile of the unit
+template <int H> struct TreeCursor {
     int b, head, row_tile, tile;
     int tiles, row_tiles;                // of the stream
     int row, ctx, nodes;
     __device__ __forceinline__ void load(const TreeDev& d) {
         ctx = tree_lengths(d, b, row, nodes);
         tiles = tree_tiles(ctx, nodes);
-        row_tiles = tree_row_tiles(nodes, d.G);
+        row_tiles = tree_row_tiles(nodes, d.G, H);
     }
     __device__ __forceinline__ void start(const TreeDev& d, const int* pre, int f) {
         b = stream_of(pre, d.B, f);
@@ -368,54 +368,57 @@ __device__ __forceinline__ void tr_weights(const float (&x)[32], uint32_t (&wgt)
     total += s0.x + s0.y;
 }
 
-template <int BITS>
-__global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev d, TreeParts parts) {
-    using SM = TRSmem<BITS>;
+template <int BITS, int H>
+__global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDev d, TreeParts parts) {
+    using SM = TRSmem<BITS, H>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (lr_smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = lr_smem_u32(smem);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int half = H == 2 && threadIdx.x >= TR_THREADS, tid = threadIdx.x - half * TR_THREADS, lane = tid & 31, warp = tid >> 5;
     int* pre = reinterpret_cast<int*>(smem + SM::PRE);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::MISC);
     const uint32_t bars = sbase + SM::BARS;
-    const uint32_t k_full = bars, v_full = bars + 8, q_full = bars + 16, s_full = bars + 24, p_full = bars + 40, pv_done = bars + 56, k_side = bars + 72, v_side = k_side + 8 * TR_SETS,
-                   kr_full = v_side + 8 * TR_SETS, kr_empty = kr_full + 8 * TR_K_AHEAD, vr_full = kr_empty + 8 * TR_K_AHEAD, vr_empty = vr_full + 8 * TR_V_AHEAD;
+    const uint32_t k_full = bars, v_full = k_full + 16, k_side = v_full + 16, v_side = k_side + 8 * TR_SETS, kr_full = v_side + 8 * TR_SETS,
+                   kr_empty = kr_full + 8 * TR_K_AHEAD, vr_full = kr_empty + 8 * TR_K_AHEAD, vr_empty = vr_full + 8 * TR_V_AHEAD,
+                   own = vr_empty + 8 * TR_V_AHEAD;                      // the others are a half's own
+    const uint32_t q_full = own + 56 * half, s_full = q_full + 8, p_full = s_full + 16, pv_done = p_full + 16;
     dependency_release();
     if (tid == 0) {
-        lr_mbar_init(k_full, 2);
-        lr_mbar_init(v_full, 2);
         lr_mbar_init(q_full, 4);
         for (int i = 0; i < 2; ++i) lr_mbar_init(s_full + 8 * i, 1), lr_mbar_init(p_full + 8 * i, 4), lr_mbar_init(pv_done + 8 * i, 1);
-        for (int i = 0; i < TR_SETS; ++i) lr_mbar_init(k_side + 8 * i, 1), lr_mbar_init(v_side + 8 * i, 1);
-        for (int i = 0; i < TR_K_AHEAD; ++i) lr_mbar_init(kr_full + 8 * i, 1), lr_mbar_init(kr_empty + 8 * i, 3);
-        for (int i = 0; i < TR_V_AHEAD; ++i) lr_mbar_init(vr_full + 8 * i, 1), lr_mbar_init(vr_empty + 8 * i, 3);
+        if (half == 0) {
+            for (int i = 0; i < H; ++i) lr_mbar_init(k_full + 8 * i, 2 * H), lr_mbar_init(v_full + 8 * i, 2 * H);
+            for (int i = 0; i < TR_SETS; ++i) lr_mbar_init(k_side + 8 * i, 1), lr_mbar_init(v_side + 8 * i, 1);
+            for (int i = 0; i < TR_K_AHEAD; ++i) lr_mbar_init(kr_full + 8 * i, 1), lr_mbar_init(kr_empty + 8 * i, 2 * H + 1);
+            for (int i = 0; i < TR_V_AHEAD; ++i) lr_mbar_init(vr_full + 8 * i, 1), lr_mbar_init(vr_empty + 8 * i, 2 * H + 1);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == TR_MMA) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lr_smem_u32(tmem_slot)), "r"(TR_COLS) : "memory");
+    if (half == 0 && warp == TR_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lr_smem_u32(tmem_slot)), "r"(H * TR_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     dependency_wait();
-    const int total = stream_prefix<TR_THREADS>(d.B, pre, [&](int i) {
+    const int total = stream_prefix<H * TR_THREADS>(d.B, pre, [&](int i) {
         int row, nodes;
         const int ctx = tree_lengths(d, i, row, nodes);
         if (row < 0 && blockIdx.x == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_SEQ);
-        return nodes > 0 ? d.c.n_kv * tree_row_tiles(nodes, d.G) * tree_tiles(ctx, nodes) : 0;
+        return nodes > 0 ? d.c.n_kv * tree_row_tiles(nodes, d.G, H) * tree_tiles(ctx, nodes) : 0;
     });
-    const int per = max(TR_MIN_TILES, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int per = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     if (blockIdx.x == 0) {
         if (tid == 0) parts.plan[0] = per;
-        for (int i = tid; i <= d.B; i += TR_THREADS) parts.plan[1 + i] = pre[i];
+        for (int i = tid; i <= d.B; i += TR_THREADS) parts.plan[1 + i] = pre[i];       // (by either half)
     }
     tr_fence_before();
     __syncthreads();
     tr_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = *tmem_slot + half * TR_COLS;
     const int f0 = (int)min((long long)total, (long long)blockIdx.x * per), f1 = min(total, f0 + per);
     bool failed = false;
     if (f0 < f1) {
         // registers go where the scores are: 120 + 72 + 48 of the 3 x 80 a thread that the block was launched with
-        TreeCursor cur;
+        TreeCursor<H> cur;
         if (warp >= TR_MMA) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
             if (warp == TR_MMA) {
@@ -423,7 +426,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             // ---- the products ----
             const uint32_t idesc_qk = (1u << 4) | ((uint32_t)(TR_KEYS >> 3) << 17) | ((uint32_t)(TR_ROWS >> 4) << 24);
             const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(TR_ROWS >> 4) << 24);
-            const uint32_t q_lo = lr_desc_lo(sbase + SM::Q), k_lo = lr_desc_lo(sbase + SM::K);
+            const uint32_t q_lo = lr_desc_lo(sbase + SM::Q + half * SM::QTILE), k_lo = lr_desc_lo(sbase + SM::K);
             // V: [64 channels][keys], channels contiguous: 64-channel halves 8192 bytes apart (leading), 8-key groups 1024 (stride)
             const uint32_t v_lo = (((sbase + SM::V) & 0x3FFFFu) >> 4) | ((uint32_t)(TR_KEYS * 128 >> 4) << 16);
             const int count = f1 - f0;
@@ -431,12 +434,13 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             bool first_before = true;                                // whether tile n - 1 opened its unit here
             auto pv = [&](int m, bool first) {
                 const uint32_t b = m & 1, ph = (uint32_t)(m >> 1) & 1u;
-                if (TR_RARE(!tr_wait2(v_full, b, p_full + 8 * b, ph))) return false;
+                const uint32_t buf = (uint32_t)m % H;
+                if (TR_RARE(!tr_wait2(v_full + 8 * buf, (uint32_t)m / H & 1u, p_full + 8 * b, ph))) return false;
                 tr_fence_after();
                 if (lr_elect()) {
 #pragma unroll
                     for (int k = 0; k < TR_KEYS / 16; ++k)
-                        tr_mma_ta(tmem + TR_COL_O, tmem + TR_COL_S + TR_KEYS * b + 8 * k, lr_desc(v_lo + 128 * k), idesc_pv, !first || k ? 1u : 0u);
+                        tr_mma_ta(tmem + TR_COL_O, tmem + TR_COL_S + TR_KEYS * b + 8 * k, lr_desc(v_lo + buf * (TR_TILE >> 4) + 128 * k), idesc_pv, !first || k ? 1u : 0u);
                     lr_commit(pv_done + 8 * b);
                 }
                 __syncwarp();
@@ -452,13 +456,14 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     ++seg;
                 }
                 // (S of tile n lies where the weights of tile n - 2 were: their product has been issued before this one)
-                if (TR_RARE(!tr_wait(k_full, b))) { failed = true; break; }
+                const uint32_t buf = (uint32_t)n % H;
+                if (TR_RARE(!tr_wait(k_full + 8 * buf, (uint32_t)n / H & 1u))) { failed = true; break; }
                 tr_fence_after();
                 if (lr_elect()) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         lr_mma(tmem + TR_COL_S + TR_KEYS * b, lr_desc(q_lo + (k >> 2) * (TR_ROWS * 128 >> 4) + 2 * (k & 3)),
-                               lr_desc(k_lo + (k >> 2) * (TR_KEYS * 128 >> 4) + 2 * (k & 3)), idesc_qk, k ? 1u : 0u);
+                               lr_desc(k_lo + buf * (TR_TILE >> 4) + (k >> 2) * (TR_KEYS * 128 >> 4) + 2 * (k & 3)), idesc_qk, k ? 1u : 0u);
                     lr_commit(s_full + 8 * b);
                 }
                 __syncwarp();
@@ -469,6 +474,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             if (!failed) failed = !pv(count - 1, first_before);
             // nothing of this CTA's is in flight when its tensor memory goes back
             if (!failed) failed = !tr_wait(pv_done + 8 * ((count - 1) & 1), (uint32_t)((count - 1) >> 1) & 1u);
+            } else if (half == 1) {                                  // the copies and the scales are the first half's
             } else if (warp < TR_SCALES) {
                 // ---- pages into the rings, with their scales: a warp for K, one for V; lane = page of the tile ----
                 cur.start(d, pre, f0);
@@ -587,37 +593,43 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
             }
         } else if (warp >= TR_K) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-            // ---- codes to f16: warp w of the two of K, of V, takes pages 2 w and 2 w + 1 of every tile ----
+            // ---- codes to f16: warp w of the two or four of K, of V, takes pages 2 w and 2 w + 1, or page w, of every tile ----
+            constexpr int MINE = TR_PAGES / (2 * H);
             const bool of_v = warp >= TR_V;
-            const int w = (warp - TR_K) & 1, count = f1 - f0, ahead = of_v ? TR_V_AHEAD : TR_K_AHEAD;
+            const int page = (((warp - TR_K) & 1) + 2 * half) * MINE, count = f1 - f0, ahead = of_v ? TR_V_AHEAD : TR_K_AHEAD;
             const int at = tr_place<BITS>(lane);
-            const unsigned char* ring = smem + (of_v ? SM::VRING : SM::KRING) + 2 * w * SM::PAGE;
-            const unsigned char* facts = smem + SM::FACT + (of_v * TR_KEYS + 2 * w * PIKV_PAGE_TOKENS + tr_row(lane)) * SM::FACTOR;
+            const unsigned char* ring = smem + (of_v ? SM::VRING : SM::KRING) + page * SM::PAGE;
+            const unsigned char* facts = smem + SM::FACT + (of_v * TR_KEYS + page * PIKV_PAGE_TOKENS + tr_row(lane)) * SM::FACTOR;
             unsigned char* tile = smem + (of_v ? SM::V : SM::K);
-            const uint32_t full = of_v ? vr_full : kr_full, empty = of_v ? vr_empty : kr_empty, read = of_v ? pv_done : s_full, ready = of_v ? v_full : k_full,
+            const uint32_t full = of_v ? vr_full : kr_full, empty = of_v ? vr_empty : kr_empty, read = own + (of_v ? 40 : 8), ready = of_v ? v_full : k_full,
                            sides = of_v ? v_side : k_side;
             int s = 0;
             uint32_t ph = 0;
             for (int n = 0; n < count; ++n) {
                 if (TR_RARE(!tr_wait2(full + 8 * s, ph, sides + 8 * tr_set(n), tr_set_phase(n)))) { failed = true; break; }
-                TRPage<BITS> x0, x1;
-                x0.load(ring + s * TR_PAGES * SM::PAGE, at);                       // (what a page behind the end left there is finite)
-                x1.load(ring + s * TR_PAGES * SM::PAGE + SM::PAGE, at);
-                const unsigned char* f = facts + tr_set(n) * 2 * TR_KEYS * SM::FACTOR;
-                TRFactor<BITS> f00, f01, f10, f11;
-                f00.load(f);
-                f01.load(f + 8 * SM::FACTOR);
-                f10.load(f + 16 * SM::FACTOR);
-                f11.load(f + 24 * SM::FACTOR);
+                TRPage<BITS> x[MINE];
+                TRFactor<BITS> f[MINE][2];
+                const unsigned char* fact = facts + tr_set(n) * 2 * TR_KEYS * SM::FACTOR;
+#pragma unroll
+                for (int i = 0; i < MINE; ++i) {
+                    x[i].load(ring + (s * TR_PAGES + i) * SM::PAGE, at);           // (what a page behind the end left there is finite)
+                    f[i][0].load(fact + 16 * i * SM::FACTOR);
+                    f[i][1].load(fact + (16 * i + 8) * SM::FACTOR);
+                }
                 __syncwarp();
                 if (lane == 0) lr_mbar_arrive(empty + 8 * s);
-                // the product of the tile before has read the buffer
-                if (n > 0 && TR_RARE(!tr_wait(read + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) { failed = true; break; }
-                x0.store(tile, 2 * w, lane, f00, f01);
-                x1.store(tile, 2 * w + 1, lane, f10, f11);
+                // the products of the tile before in this buffer have read it
+                const int m = n - H;
+                if (m >= 0) {
+                    const uint32_t bar = read + 8 * (m & 1), was = (uint32_t)(m >> 1) & 1u;
+                    if (TR_RARE(H == 2 ? !tr_wait2(bar, was, bar + 56, was) : !tr_wait(bar, was))) { failed = true; break; }
+                }
+                unsigned char* to = tile + (uint32_t)n % H * TR_TILE;
+#pragma unroll
+                for (int i = 0; i < MINE; ++i) x[i].store(to, page + i, lane, f[i][0], f[i][1]);
                 tr_fence_smem();
                 __syncwarp();
-                if (lane == 0) lr_mbar_arrive(ready);
+                if (lane == 0) lr_mbar_arrive(ready + 8 * ((uint32_t)n % H));
                 if (++s == ahead) s = 0, ph ^= 1u;
             }
         } else {
@@ -703,7 +715,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                 // ---- a unit, or the part of it that this CTA has: tiles t0 .. t1 - 1 ----
                 const int t0 = cur.tile, t1 = min(cur.tiles, t0 + f1 - f), edge = max(t0, min(t1, cur.ctx / TR_KEYS));
                 // ---- this row's query ----
-                const int row = cur.row_tile * TR_ROWS + tid, h = cur.head;
+                const int row = (cur.row_tile * H + half) * TR_ROWS + tid, h = cur.head;
                 node = row / d.G;
                 live = node < cur.nodes;
                 warp_live = __any_sync(0xffffffffu, live);
@@ -740,7 +752,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                         y.y = tr_pack(x[tr_channel<BITS>(2)], x[tr_channel<BITS>(3)]);
                         y.z = tr_pack(x[tr_channel<BITS>(4)], x[tr_channel<BITS>(5)]);
                         y.w = tr_pack(x[tr_channel<BITS>(6)], x[tr_channel<BITS>(7)]);
-                        *reinterpret_cast<uint4*>(smem + SM::Q + (i >> 3) * TR_ROWS * 128 + tid * 128 + 16 * ((i & 7) ^ (tid & 7))) = y;
+                        *reinterpret_cast<uint4*>(smem + SM::Q + half * SM::QTILE + (i >> 3) * TR_ROWS * 128 + tid * 128 + 16 * ((i & 7) ^ (tid & 7))) = y;
                     }
                     qmul = exp2_int(-max(sh, -126)) * (0.08838834764831845f * 1.4426950408889634f) + odd;
                     tr_fence_smem();
@@ -770,7 +782,7 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
                     const bool begun = t0 == 0;                          // here, and not by the CTA before
                     const bool whole = begun && t1 == cur.tiles;
                     const float inv = den == 0.f ? 0.f : 1.f / den;
-                    const size_t slot = (size_t)(2 * blockIdx.x + (begun ? 1 : 0)) * parts.rows + tid;
+                    const size_t slot = (size_t)((2 * blockIdx.x + (begun ? 1 : 0)) * H + half) * parts.rows + tid;
 #pragma unroll 1
                     for (int c = 0; c < 128; c += 32) {
                         float o[32];
@@ -817,9 +829,9 @@ __global__ void __launch_bounds__(TR_THREADS, TR_CTAS) tree_attn_kernel(TreeDev 
     }
     tr_fence_before();
     __syncthreads();
-    if (warp == TR_MMA) {
+    if (half == 0 && warp == TR_MMA) {
         tr_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TR_COLS) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(H * TR_COLS) : "memory");
     }
 }
 
@@ -848,26 +860,26 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
         if (lane == 0 && d.lse) d.lse[at] = -INFINITY;
         return;
     }
-    const int tiles = tree_tiles(ctx, nodes), row_tiles = tree_row_tiles(nodes, d.G);
+    const int H = parts.halves, tiles = tree_tiles(ctx, nodes), row_tiles = tree_row_tiles(nodes, d.G, H);
     const int r = node * d.G + qh % d.G;
-    const int f0 = pre0 + ((qh / d.G) * row_tiles + r / TR_ROWS) * tiles, f1 = f0 + tiles;
+    const int f0 = pre0 + ((qh / d.G) * row_tiles + r / TR_ROWS / H) * tiles, f1 = f0 + tiles;
     const int c0 = f0 / per, c1 = (f1 - 1) / per;
     if (c0 == c1) return;                                               // whole: written by its CTA
-    // piece i lies in slot 2 (c0 + i), the first one in the slot behind that
-    const size_t slot0 = (size_t)2 * c0 * parts.rows + r % TR_ROWS;
+    // piece i lies in the first slot of CTA c0 + i, the first piece in the second
+    const size_t slot0 = (size_t)(2 * c0 * H + r / TR_ROWS % H) * parts.rows + r % TR_ROWS;
     const float4* o0 = reinterpret_cast<const float4*>(parts.o + slot0 * 128) + lane;
     const float2* ml0 = parts.ml + slot0;
-    const int pieces = c1 - c0 + 1, stride = 2 * parts.rows;
+    const int pieces = c1 - c0 + 1, stride = 2 * H * parts.rows;
     float M = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     // pieces in batches, the next one on its way while one is joined
     float4 o[BATCH], next[BATCH];
     float2 ml, next_ml;
     auto fetch = [&](int g, float4 (&to)[BATCH], float2& to_ml) {
-        to_ml = g + lane < pieces && lane < BATCH ? ml0[(size_t)(g + lane) * stride + (g + lane ? 0 : parts.rows)] : make_float2(-INFINITY, 0.f);
+        to_ml = g + lane < pieces && lane < BATCH ? ml0[(size_t)(g + lane) * stride + (g + lane ? 0 : H * parts.rows)] : make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int u = 0; u < BATCH; ++u)
-            if (g + u < pieces) to[u] = o0[((size_t)(g + u) * stride + (g + u ? 0 : parts.rows)) * 32];
+            if (g + u < pieces) to[u] = o0[((size_t)(g + u) * stride + (g + u ? 0 : H * parts.rows)) * 32];
     };
     fetch(0, o, ml);
     for (int g = 0; g < pieces; g += BATCH) {
@@ -902,7 +914,7 @@ struct TreeLayout {
     size_t ml, o, total;
 };
 static TreeLayout tree_layout(int N, int G) {
-    const size_t slots = (size_t)2 * sm_count() * TR_CTAS, rows = tree_slot_rows(N, G);
+    const size_t slots = (size_t)2 * sm_count() * 2, rows = tree_slot_rows(N, G);
     TreeLayout l;
     l.ml = ((size_t)(PIKV_STREAMS_PER_LAUNCH + 2) * sizeof(int) + 255) & ~(size_t)255;
     l.o = l.ml + slots * rows * sizeof(float2);
@@ -1021,6 +1033,13 @@ extern "C" size_t pikv_tree_attn_workspace_bytes(int32_t B, int32_t N, int32_t n
     return tree_layout(N, n_q / n_kv).total;
 }
 
+template <int BITS, int H>
+static bool tree_launch(int grid, cudaStream_t st, const TreeDev& d, const TreeParts& parts) {
+    if (!allow_smem<tree_attn_kernel<BITS, H>>(TRSmem<BITS, H>::BYTES)) return false;
+    launch_dependent(tree_attn_kernel<BITS, H>, grid, H * TR_THREADS, TRSmem<BITS, H>::BYTES, st, d, parts);
+    return true;
+}
+
 extern "C" int pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params* p, pikv_stream_t stream) {
     TreeDev d;
     const int rc = cache_dev(c, d.c, "tree_attn", true);
@@ -1057,14 +1076,14 @@ extern "C" int pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params*
         d.q = static_cast<const __nv_bfloat16*>(p->q) + b0 * rows * 128;
         d.out = static_cast<__nv_bfloat16*>(p->out) + b0 * rows * 128;
         d.lse = p->lse ? p->lse + b0 * rows : nullptr;
-        const int grid = (int)std::min<int64_t>(sm_count() * TR_CTAS, (int64_t)d.B * c->n_kv * ceil_div(d.N * d.G, TR_ROWS) * ceil_div(c->max_pages, TR_PAGES));
-        if (c->bits == 8) {
-            if (!allow_smem<tree_attn_kernel<8>>(TRSmem<8>::BYTES)) return check_launch("tree_attn smem attribute");
-            launch_dependent(tree_attn_kernel<8>, grid, TR_THREADS, TRSmem<8>::BYTES, st, d, parts);
-        } else {
-            if (!allow_smem<tree_attn_kernel<4>>(TRSmem<4>::BYTES)) return check_launch("tree_attn smem attribute");
-            launch_dependent(tree_attn_kernel<4>, grid, TR_THREADS, TRSmem<4>::BYTES, st, d, parts);
-        }
+        // Two CTAs per SM, or one whose halves share the tiles of K and V where a head has more rows than a tile
+        const bool wide = d.N * d.G > TR_ROWS;
+        parts.halves = wide ? 2 : 1;
+        const int64_t units = (int64_t)d.B * c->n_kv * ceil_div(d.N * d.G, parts.halves * TR_ROWS);
+        const int grid = (int)std::min<int64_t>(sm_count() * 2 / parts.halves, units * ceil_div(c->max_pages, TR_PAGES));
+        const bool sent = c->bits == 8 ? (wide ? tree_launch<8, 2>(grid, st, d, parts) : tree_launch<8, 1>(grid, st, d, parts))
+                                       : (wide ? tree_launch<4, 2>(grid, st, d, parts) : tree_launch<4, 1>(grid, st, d, parts));
+        if (!sent) return check_launch("tree_attn smem attribute");
         const int blocks = (int)((d.B * rows + TM_THREADS / 32 - 1) / (TM_THREADS / 32));
         if (blocks <= sm_count() * TM_RESIDENT) launch_dependent(tree_merge_kernel<8>, blocks, TM_THREADS, 0, st, d, parts);
         else launch_dependent(tree_merge_kernel<4>, blocks, TM_THREADS, 0, st, d, parts);
