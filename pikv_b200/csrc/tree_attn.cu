@@ -38,13 +38,14 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // ---- attention --------------------------------------------------------------------------------------------------
 // The nodes of a stream times the query heads of one KV head are the rows of one product: S = Q K^T for 128 rows and 64 keys
 // at a time, O += P V, both by tcgen05 with the accumulators in tensor memory.  The keys of all (stream, head, 128 rows)
-// units form one list of tiles that a persistent grid cuts into equal runs, two CTAs per SM; a unit that one CTA holds
+// units form one list of tiles that a persistent grid cuts into equal runs, two CTAs per SM (or one of two halves, which have 128
+// rows each of one head and share the converted tiles, so that these are made once: H = 2); a unit that one CTA holds
 // whole is finished there, the pieces of others go to the workspace and a second kernel joins them.
 //
-// A CTA's warps:
+// A half's warps (the second half has no copies to make and no scales to prepare):
 //   0-3  softmax: thread = row.  S comes out of tensor memory, the weights go back into it as the A operand of the second
 //        product; a row's maximum, denominator and the rescaling of its O live in its thread
-//   4-5, 6-7  two pages of every tile each: codes of K, of V, to f16, into the swizzled layout that both products read
+//   4-5, 6-7  two pages (one where there are two halves) of every tile each: codes of K, of V, to f16, into the swizzled layout that both products read
 //   8    issues the MMAs: Q K^T of tile n + 1 before P V of tile n, so that the products of one tile run while the softmax
 //        of another does
 //   9, 10  bulk copies of pages into two rings, K three tiles ahead, V two (one warp for both is late: 130 cycles a copy)
@@ -63,10 +64,10 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // the fp32 sum of 2^(logit - R).  A row of V that is not finite enters as zeros and makes the result of the rows that see it
 // not a number; one that a row does not see does not reach it.
 //
-// 16 streams x 16384 rows x 8 heads, 32 nodes x 4 query heads, int8: 196 us with the merge = 2.8 TB/s and 0.70 PFLOP/s in a
-// burst, 235 us in long runs under the power cap (the bytes alone take 85 us, the products 82).  Bound by the conversions, the
-// weights and their handing over: 3180 warp instructions per tile (1126 convert K and V, 548 make weights, 150 read scores) in
-// 0.56 of the issue slots, tensor pipe 36 %, DRAM 35 %.  No single pipe is full; the 24 warps wait for one another.
+// 16 streams x 16384 rows x 8 heads, 32 nodes x 4 query heads, int8: 183 us with the merge = 3.0 TB/s and 0.75 PFLOP/s in a
+// burst, 219 us in long runs under the power cap (the bytes alone take 85 us, the products 82); 8 x 32768, 64 nodes: 308 and
+// 359.  Bound by power and by the latency between the warps: the SM clock is at 1.6-1.75 GHz, and leaving out the conversion,
+// either product, the copies or the weights shortens it by 20, 9 and 5, 6 and 8 %, none by what it costs alone.
 constexpr int TR_THREADS = 384;          // of a half: three warpgroups
 constexpr int TR_K = 4, TR_V = 6, TR_MMA = 8, TR_COPY = 9, TR_SCALES = 11;      // first warps of each kind
 constexpr int TR_ROWS = 128;             // rows of a unit
@@ -1076,8 +1077,10 @@ extern "C" int pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params*
         d.q = static_cast<const __nv_bfloat16*>(p->q) + b0 * rows * 128;
         d.out = static_cast<__nv_bfloat16*>(p->out) + b0 * rows * 128;
         d.lse = p->lse ? p->lse + b0 * rows : nullptr;
-        // Two CTAs per SM, or one whose halves share the tiles of K and V where a head has more rows than a tile
-        const bool wide = d.N * d.G > TR_ROWS;
+        // Two CTAs per SM, or one whose halves share the tiles of K and V, where at least three quarters of its rows are used: 8 x 32768
+        // with 256 rows 348 us against 308, with 208 rows 335 against 299; 8 x 8192 with 416 of 512 rows 106 against 102, with 336 86
+        // against 97; 128 rows, a half idle, 187 against 272.  (Streams may have fewer nodes than N: with half as many 190 against 277.)
+        const bool wide = 4 * d.N * d.G > 3 * 2 * TR_ROWS * ceil_div(d.N * d.G, 2 * TR_ROWS);
         parts.halves = wide ? 2 : 1;
         const int64_t units = (int64_t)d.B * c->n_kv * ceil_div(d.N * d.G, parts.halves * TR_ROWS);
         const int grid = (int)std::min<int64_t>(sm_count() * 2 / parts.halves, units * ceil_div(c->max_pages, TR_PAGES));
