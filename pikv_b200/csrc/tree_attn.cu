@@ -519,8 +519,8 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                 for (int k = 0; k < ahead; ++k) (void)tr_wait(full + 8 * k, k < s ? ph ^ 1u : ph);
             } else {
                 // ---- scales as the other warps want them, K of tile n + 1 before V of tile n; lane = rows 2 lane and 2 lane + 1 ----
-                // The sets need no wait of their own: K of tile n + 1 takes that of tile n - 7, V of tile n - 1 has come, into a place that
-                // V of tile n - 3 left after the second product of tile n - 5
+                // The sets need no wait of their own: when K of tile n + 1 takes that of tile n - 7, V of tile n - 1 has come, into a
+                // place that V of tile n - 3 left, behind the second product of tile n - 3 - H
                 cur.start(d, pre, f0);
                 const int count = f1 - f0;
                 auto side = [&](auto v_c, int n, int left, int s, uint32_t ph) {
@@ -570,6 +570,7 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                     } else if (lane == 0) {
                         of[0] = exp2_int(e + 9);
                     }
+                    tr_fence_smem();                                 // before the ring's place is given back
                     __syncwarp();
                     if (lane == 0) {
                         lr_mbar_arrive((OF_V ? v_side : k_side) + 8 * tr_set(n));
@@ -617,8 +618,6 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                     f[i][0].load(fact + 16 * i * SM::FACTOR);
                     f[i][1].load(fact + (16 * i + 8) * SM::FACTOR);
                 }
-                __syncwarp();
-                if (lane == 0) lr_mbar_arrive(empty + 8 * s);
                 // the products of the tile before in this buffer have read it
                 const int m = n - H;
                 if (m >= 0) {
@@ -628,9 +627,13 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                 unsigned char* to = tile + (uint32_t)n % H * TR_TILE;
 #pragma unroll
                 for (int i = 0; i < MINE; ++i) x[i].store(to, page + i, lane, f[i][0], f[i][1]);
+                // also before the ring's place is given back: without the fence, a bulk copy may land under these warps' own reads
                 tr_fence_smem();
                 __syncwarp();
-                if (lane == 0) lr_mbar_arrive(ready + 8 * ((uint32_t)n % H));
+                if (lane == 0) {
+                    lr_mbar_arrive(ready + 8 * ((uint32_t)n % H));
+                    lr_mbar_arrive(empty + 8 * s);
+                }
                 if (++s == ahead) s = 0, ph ^= 1u;
             }
         } else {
