@@ -90,6 +90,21 @@ def test_tree_masks_and_sizes(bits, N, G, n_kv, shared):
     compare(cache, q, mask, ctx, nodes, out, lse, ids)
 
 
+# long enough for copies, conversions and products of many tiles to run into one another where a wait or a fence is missing
+@pytest.mark.parametrize("bits,N", [(8, 32), (4, 32), (8, 64), (4, 50)])
+def test_tree_repeats(bits, N):
+    ctx = [6000 + 37 * i for i in range(12)]
+    cache, gen = filled_cache([n + N for n in ctx], 8, bits, seed=N)
+    q = torch.randn(len(ctx), N, 32, D, generator=gen, device="cuda").bfloat16() * 3
+    mask = random_trees(gen, len(ctx), N)
+    length = torch.tensor(ctx, dtype=torch.int32, device="cuda")
+    first = cache.decode_attention_tree(q, mask, ctx_len=length)
+    for _ in range(12):
+        assert torch.equal(cache.decode_attention_tree(q, mask, ctx_len=length), first)
+    compare(cache, q[-1:], mask[-1:], length[-1:], None, first[-1:], None, ids=[len(ctx) - 1])
+    cache.check_status()
+
+
 def test_tree_zero_points():
     """4-bit rows of one value, whose zero points are millions, between ordinary ones; zero points that are not whole numbers."""
     ctx, N, n_kv = [150, 64], 9, 2
