@@ -65,8 +65,8 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 // not a number; one that a row does not see does not reach it.
 //
 // 16 streams x 16384 rows x 8 heads, 32 nodes x 4 query heads, int8: 183 us with the merge = 3.0 TB/s and 0.75 PFLOP/s in a
-// burst, 219 us in long runs under the power cap (the bytes alone take 85 us, the products 82); 8 x 32768, 64 nodes: 308 and
-// 359.  Bound by power and by the latency between the warps: the SM clock is at 1.6-1.75 GHz, and leaving out the conversion,
+// burst, 217 us in long runs under the power cap (the bytes alone take 85 us, the products 82); 8 x 32768, 64 nodes: 308 and
+// 355.  Bound by power and by the latency between the warps: the SM clock is at 1.6-1.75 GHz, and leaving out the conversion,
 // either product, the copies or the weights shortens it by 20, 9 and 5, 6 and 8 %, none by what it costs alone.
 constexpr int TR_THREADS = 384;          // of a half: three warpgroups
 constexpr int TR_K = 4, TR_V = 6, TR_MMA = 8, TR_COPY = 9, TR_SCALES = 11;      // first warps of each kind
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
         if (row < 0 && blockIdx.x == 0 && d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_SEQ);
         return nodes > 0 ? d.c.n_kv * tree_row_tiles(nodes, d.G, H) * tree_tiles(ctx, nodes) : 0;
     });
-    const int per = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int per = (max(total, 1) - 1) / (int)gridDim.x + 1;
     if (blockIdx.x == 0) {
         if (tid == 0) parts.plan[0] = per;
         for (int i = tid; i <= d.B; i += TR_THREADS) parts.plan[1 + i] = pre[i];       // (by either half)
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
     __syncthreads();
     tr_fence_after();
     const uint32_t tmem = *tmem_slot + half * TR_COLS;
-    const int f0 = (int)min((long long)total, (long long)blockIdx.x * per), f1 = min(total, f0 + per);
+    const int f0 = (int)min((long long)total, (long long)blockIdx.x * per), f1 = (int)min((long long)total, (long long)f0 + per);
     bool failed = false;
     if (f0 < f1) {
         // registers go where the scores are: 120 + 72 + 48 of the 3 x 80 a thread that the block was launched with
