@@ -383,7 +383,6 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                    kr_empty = kr_full + 8 * TR_K_AHEAD, vr_full = kr_empty + 8 * TR_K_AHEAD, vr_empty = vr_full + 8 * TR_V_AHEAD,
                    own = vr_empty + 8 * TR_V_AHEAD;                      // the others are a half's own
     const uint32_t q_full = own + 56 * half, s_full = q_full + 8, p_full = s_full + 16, pv_done = p_full + 16;
-    dependency_release();
     if (tid == 0) {
         lr_mbar_init(q_full, 4);
         for (int i = 0; i < 2; ++i) lr_mbar_init(s_full + 8 * i, 1), lr_mbar_init(p_full + 8 * i, 4), lr_mbar_init(pv_done + 8 * i, 1);
@@ -395,11 +394,13 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // Tensor memory is taken when the kernels before have given theirs back, and nothing behind this one starts until it is taken:
+    // a kernel that waits for its predecessors with tensor memory in hand could keep it from one of them
+    dependency_wait();
     if (half == 0 && warp == TR_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lr_smem_u32(tmem_slot)), "r"(H * TR_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    dependency_wait();
     const int total = stream_prefix<H * TR_THREADS>(d.B, pre, [&](int i) {
         int row, nodes;
         const int ctx = tree_lengths(d, i, row, nodes);
@@ -414,6 +415,7 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
     tr_fence_before();
     __syncthreads();
     tr_fence_after();
+    dependency_release();
     const uint32_t tmem = *tmem_slot + half * TR_COLS;
     const int f0 = (int)min((long long)total, (long long)blockIdx.x * per), f1 = (int)min((long long)total, (long long)f0 + per);
     bool failed = false;
