@@ -105,6 +105,40 @@ def test_tree_repeats(bits, N):
     cache.check_status()
 
 
+def test_tree_next_to_other_kernels():
+    """Wide and narrow trees and a projection, which take tensor memory too, behind one another and on streams side by side."""
+    import pikv_b200
+    made = []
+    for N, bits in ((64, 8), (16, 8), (60, 4)):
+        cache, gen = filled_cache([2000 + 300 * i + N for i in range(6)], 4, bits, seed=N)
+        cache.length.copy_(torch.tensor([2000 + 300 * i for i in range(6)], dtype=torch.int32))
+        made.append((cache, torch.randn(6, N, 16, D, generator=gen, device="cuda").bfloat16(), random_trees(gen, 6, N)))
+    x = torch.randn(8192, 1024, generator=gen, device="cuda").bfloat16()
+    w = torch.randn(64, 1024, generator=gen, device="cuda").bfloat16()
+
+    def steps(first):
+        got = []
+        for i in range(3):
+            cache, q, mask = made[(first + i) % 3]
+            got += [pikv_b200.ops.lowrank_project(x, w), cache.decode_attention_tree(q, mask)]
+        return got
+
+    want = [steps(i) for i in range(3)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        got = []
+        for i, s in enumerate(streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(steps(i))
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        assert all(torch.equal(a, b) for x_, y_ in zip(got, want) for a, b in zip(x_, y_))
+    for cache, _, _ in made:
+        cache.check_status()
+
+
 def test_tree_zero_points():
     """4-bit rows of one value, whose zero points are millions, between ordinary ones; zero points that are not whole numbers."""
     ctx, N, n_kv = [150, 64], 9, 2
