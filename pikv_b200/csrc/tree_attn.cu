@@ -846,9 +846,10 @@ constexpr int TM_RESIDENT = 5;                                          // block
 
 // Joins the pieces of units that were cut, and answers for the rows that no unit has.  One warp per (stream, node, query head),
 // lane = 4 channels: O = sum_i O_i 2^(R_i - R), the denominator likewise.
-// Bound by the trips to the pieces (in L2): BATCH of them are on their way while as many are joined.  BATCH = 8 takes 96 registers and is right
-// while all rows' warps are resident with them (few rows have many pieces each: 1 stream x 8 nodes 6.7 us against 8.5 with 4);
-// more rows have fewer pieces and want the warps (16 streams x 32 nodes: 12.4 us with 4 against 16.0).
+// Bound by the trips to the pieces (in L2): BATCH of them are on their way at once, and where BATCH is 8 the next ones while they are
+// joined.  That takes 96 registers and is right while all rows' warps are resident with them (few rows have many pieces each: 1
+// stream x 8 nodes 6.7 us against 8.5 with 4); more rows have fewer pieces and want the warps (47 registers, 16 streams x 32 nodes:
+// 11.8 us against 16.0, and 14.8 with the next batch ahead).
 template <int BATCH>
 __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeParts parts) {
     dependency_release();
@@ -878,8 +879,9 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
     const int pieces = c1 - c0 + 1, stride = 2 * H * parts.rows;
     float M = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    // pieces in batches, the next one on its way while one is joined
-    float4 o[BATCH], next[BATCH];
+    // pieces in batches
+    constexpr bool AHEAD = BATCH == 8;
+    float4 o[BATCH], next[AHEAD ? BATCH : 1];
     float2 ml, next_ml;
     auto fetch = [&](int g, float4 (&to)[BATCH], float2& to_ml) {
         to_ml = g + lane < pieces && lane < BATCH ? ml0[(size_t)(g + lane) * stride + (g + lane ? 0 : H * parts.rows)] : make_float2(-INFINITY, 0.f);
@@ -889,7 +891,9 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
     };
     fetch(0, o, ml);
     for (int g = 0; g < pieces; g += BATCH) {
-        if (g + BATCH < pieces) fetch(g + BATCH, next, next_ml);
+        if constexpr (AHEAD) {
+            if (g + BATCH < pieces) fetch(g + BATCH, next, next_ml);
+        }
         const float top = fmaxf(M, warp_max(ml.x)), base = top == -INFINITY ? 0.f : top;
         const float keep = M == -INFINITY ? (den == 0.f ? 0.f : 1.f) : exp2f(M - base);
         // a piece that saw nothing has no weight; one that is not a number keeps it
@@ -904,13 +908,18 @@ __global__ void __launch_bounds__(TM_THREADS) tree_merge_kernel(TreeDev d, TreeP
             acc.x += o[u].x * w; acc.y += o[u].y * w; acc.z += o[u].z * w; acc.w += o[u].w * w;
             den += l * w;
         }
+        if constexpr (AHEAD) {
 #pragma unroll
-        for (int u = 0; u < BATCH; ++u) o[u] = next[u];
-        ml = next_ml;
+            for (int u = 0; u < BATCH; ++u) o[u] = next[u];
+            ml = next_ml;
+        } else if (g + BATCH < pieces) {
+            fetch(g + BATCH, o, ml);
+        }
     }
     const bool any = den != 0.f;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(any ? acc.x / den : 0.f, any ? acc.y / den : 0.f);
-    const __nv_bfloat162 hi = __floats2bfloat162_rn(any ? acc.z / den : 0.f, any ? acc.w / den : 0.f);
+    const float inv = any ? 1.f / den : 0.f;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(any ? acc.x * inv : 0.f, any ? acc.y * inv : 0.f);
+    const __nv_bfloat162 hi = __floats2bfloat162_rn(any ? acc.z * inv : 0.f, any ? acc.w * inv : 0.f);
     *out = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     if (lane == 0 && d.lse) d.lse[at] = any ? (M == -INFINITY ? 0.f : M) * 0.6931471805599453f + logf(den) : -INFINITY;
 }
