@@ -254,7 +254,10 @@ __global__ void __launch_bounds__(PB_THREADS, PB_CTAS) page_bounds_kernel(Bounds
         *reinterpret_cast<uint32_t*>(d.codes + unit * 256 + at) = ph;
         *reinterpret_cast<uint32_t*>(d.codes + unit * 256 + 128 + at) = pl;
         if (lane == 0) d.scale[unit] = odd ? INFINITY : exp2_int(e);
-        __syncwarp();                                             // the stage is copied into again
+        // The stage is copied into again: this warp's reads come before the proxy that copies.  (Every word read has been used by here,
+        // but nothing else would keep a read that the compiler moves down from a copy that lands under it.)
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
         if (++stage == PB_STAGES) stage = 0, phase ^= 1u;
     }
     if (late) {

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from paged_reference import D, PAGE, append_rows, attend64, bounds64, check_attention, chosen64, filled_cache, rows64
+from paged_reference import D, PAGE, append_rows, attend64, bounds64, check_attention, chosen64, filled_cache, rows64, step64
 
 pytestmark = pytest.mark.gpu
 # a logit: the query in 15 bits of its head's largest entry (2^-14 of it, summed against the keys: 2^-14 of the sum of sizes with the largest
@@ -358,3 +358,29 @@ def test_two_streams_at_once():
         assert all(torch.equal(x, y) for a, b in zip(got, want) for x, y in zip(a, b))
     for m in made:
         m[0].check_status()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_bounds_repeats(bits):
+    """Long enough for every warp to go round its ring of copied pages many times, into stages that it has just read: the same
+    bounds every time, those of 64 bits at both ends and in between."""
+    rows = [20000 + 331 * i for i in range(6)]
+    cache, gen = filled_cache(rows, 8, bits, seed=61)
+    cache.length.copy_(torch.tensor(rows, dtype=torch.int32))
+    first = cache.page_bounds()
+    cache.update_bounds(first)
+    for s, n in enumerate(rows):
+        k, _ = rows64(cache, s, n)
+        full = n // PAGE
+        pages = k[:full * PAGE].view(full, PAGE, 8, D)
+        hi, lo = pages.amax(1), pages.amin(1)
+        step = step64(torch.maximum(hi.abs(), lo.abs()).amax(-1))
+        at = cache.page_table[s, :full].long()
+        assert torch.equal(first.scale[at].double(), step)
+        assert torch.equal(first.codes[at].double(), torch.stack((torch.ceil(hi / step[..., None]), torch.floor(lo / step[..., None])), 2))
+    again = cache.page_bounds()
+    for _ in range(20):
+        again.codes.fill_(1)
+        cache.update_bounds(again)
+        assert torch.equal(again.codes * (again.scale > 0)[..., None, None], first.codes) and torch.equal(again.scale, first.scale)
+    cache.check_status()
