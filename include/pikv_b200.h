@@ -590,7 +590,8 @@ int pikv_tree_accept(const pikv_paged_cache* c, const int32_t* path, const int32
  *   bound_codes[page][h][0][c] = ceil(max K_c / s),  [1][c] = floor(min K_c / s)      int8
  * A page with a row whose scale (or zero point) is not below 2^112 in size, what is not finite among them, or with a key that
  * is not finite has scale +infinity and codes 0.  The pages that hold positions
- * start[b] .. seq_len[b] - 1 (start NULL: all) are computed anew.  Decodable formats (see bits). */
+ * start[b] .. seq_len[b] - 1 (start NULL: all) are computed anew; an entry of the table that is no page raises
+ * PIKV_ST_BAD_PAGE and writes nothing.  Decodable formats (see bits). */
 int pikv_page_bounds_update(const pikv_paged_cache* c, void* bound_codes, float* bound_scale, const int32_t* seq_ids,
                             const int32_t* start, const int32_t* seq_len, int32_t B, pikv_stream_t stream);
 

@@ -93,15 +93,17 @@ __global__ void __launch_bounds__(PB_THREADS, PB_CTAS) page_bounds_kernel(Bounds
     int f = (int)(it0 / n_kv), h = (int)(it0 % n_kv);
     int b = stream_of(pre, d.B, f), first, len;
     int row = range(b, first, len);
-    int lp = first + f - pre[b], page = stream_page(d.c, row, lp);
+    int lp = first + f - pre[b], page = stream_page(d.c, row, lp, -1);
     int to_copy = left;
     auto copy = [&](int stage) {
         if (to_copy == 0) return;
-        const size_t unit = (size_t)page * n_kv + h;
+        // an entry that is no page has no bounds to write either: page 0 stands in for it in the ring, with no rows
+        const size_t unit = (size_t)max(page, 0) * n_kv + h;
+        const int rows = page < 0 ? 0 : min(PIKV_PAGE_TOKENS, len - lp * PIKV_PAGE_TOKENS);
         unsigned char* to = ring + stage * GEO::STAGE;
         if (lane == 0) {
             const uint32_t dst = lr_smem_u32(to), bar = bar0 + 8 * stage;
-            *reinterpret_cast<int4*>(to + GEO::COPY) = make_int4((int)(uint32_t)unit, (int)(uint32_t)(unit >> 32), min(PIKV_PAGE_TOKENS, len - lp * PIKV_PAGE_TOKENS), 0);
+            *reinterpret_cast<int4*>(to + GEO::COPY) = make_int4((int)(uint32_t)unit, (int)(uint32_t)(unit >> 32), rows, 0);
             lr_mbar_expect_tx(bar, GEO::COPY);
             pb_bulk(dst, d.c.k_codes + unit * GEO::CODES, GEO::CODES, bar);
             pb_bulk(dst + GEO::CODES, d.c.k_scale + unit * 16, 32, bar);
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(PB_THREADS, PB_CTAS) page_bounds_kernel(Bounds
             row = range(b, first, len);
         }
         lp = first + f - pre[b];
-        page = stream_page(d.c, row, lp);
+        page = stream_page(d.c, row, lp, -1);
     };
     for (int i = 0; i < PB_STAGES - 1; ++i) copy(i);
     int stage = 0;
@@ -251,9 +253,11 @@ __global__ void __launch_bounds__(PB_THREADS, PB_CTAS) page_bounds_kernel(Bounds
             ph |= (uint32_t)(ih & 0xff) << (8 * k);
             pl |= (uint32_t)(il & 0xff) << (8 * k);
         }
-        *reinterpret_cast<uint32_t*>(d.codes + unit * 256 + at) = ph;
-        *reinterpret_cast<uint32_t*>(d.codes + unit * 256 + 128 + at) = pl;
-        if (lane == 0) d.scale[unit] = odd ? INFINITY : exp2_int(e);
+        if (rows > 0) {
+            *reinterpret_cast<uint32_t*>(d.codes + unit * 256 + at) = ph;
+            *reinterpret_cast<uint32_t*>(d.codes + unit * 256 + 128 + at) = pl;
+            if (lane == 0) d.scale[unit] = odd ? INFINITY : exp2_int(e);
+        }
         // The stage is copied into again: this warp's reads come before the proxy that copies.  (Every word read has been used by here,
         // but nothing else would keep a read that the compiler moves down from a copy that lands under it.)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -85,12 +85,12 @@ __device__ __forceinline__ int stream_row(const CacheDev& c, const int* seq_ids,
     const int seq = seq_ids ? __ldg(seq_ids + i) : i;
     return seq >= 0 && seq < c.num_seqs ? seq : -1;
 }
-// physical page of a logical one; 0 and a status bit where the table holds none
-__device__ __forceinline__ int stream_page(const CacheDev& c, int row, int page) {
+// physical page of a logical one; `none` and a status bit where the table holds none
+__device__ __forceinline__ int stream_page(const CacheDev& c, int row, int page, int none = 0) {
     const int p = page < c.max_pages ? __ldg(c.page_table + (size_t)row * c.max_pages + page) : -1;
     if (p >= 0 && p < c.num_pages) return p;
     if (c.status) atomicOr(c.status, PIKV_ST_BAD_PAGE);
-    return 0;
+    return none;
 }
 
 // The smallest power of two p >= 2^-126 with a <= 127 p, as its exponent; a finite and >= 0.  127 / 128 = 0x7e0000 of the
