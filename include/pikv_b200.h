@@ -580,7 +580,7 @@ int    pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params* p, pikv
  * A stream whose path is not ascending, leaves the cache or meets a bad page is left as it is (its new length is
  * ctx_len[b]) and raises PIKV_ST_BAD_INDEX or PIKV_ST_BAD_PAGE; one that an earlier entry of seq_ids names already
  * raises PIKV_ST_BAD_SEQ and has new_len 0.  Any cache format.  ctx_len may be the length array itself when
- * seq_ids is NULL. */
+ * seq_ids is NULL, and new_len may be ctx_len; length and new_len overlap no input otherwise (PIKV_EINVAL). */
 int pikv_tree_accept(const pikv_paged_cache* c, const int32_t* path, const int32_t* path_len, const int32_t* seq_ids,
                      const int32_t* ctx_len, int32_t B, int32_t depth, int32_t* length, int32_t* new_len, pikv_stream_t stream);
 

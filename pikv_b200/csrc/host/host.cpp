@@ -583,11 +583,19 @@ PyObject* accept(PyObject* const* a, Py_ssize_t) {
     holds(length, c.num_seqs, "the cache's length");
     const c10::cuda::OptionalCUDAGuard guard(path.device());
     const pikv_paged_cache cache = c.view(path);
-    const at::Tensor ctx = streams.get();
+    at::Tensor ctx = streams.get();
     if (ids.defined() && ptr(ctx) == ptr(length)) fail("ctx_len must have an entry per stream of the call, not per sequence of the cache");
+    // what lies in the cache's lengths is written while it is read: only a stream's own entry may be both
+    auto apart = [&](const at::Tensor& t) {
+        if (!t.defined()) return t;
+        const uintptr_t x = reinterpret_cast<uintptr_t>(t.data_ptr()), y = reinterpret_cast<uintptr_t>(length.data_ptr());
+        return x + t.nbytes() <= y || y + length.nbytes() <= x ? t : t.clone();
+    };
+    if (ptr(ctx) != ptr(length)) ctx = apart(ctx);
+    const at::Tensor way = apart(path), steps = apart(count), rows = apart(ids);
     at::Tensor fresh = at::empty({B}, on(path, at::kInt));
     if (B)
-        check(pikv_tree_accept(&cache, ptr<int32_t>(path), ptr<int32_t>(count), ptr<int32_t>(ids), ptr<int32_t>(ctx), (int32_t)B, (int32_t)depth,
+        check(pikv_tree_accept(&cache, ptr<int32_t>(way), ptr<int32_t>(steps), ptr<int32_t>(rows), ptr<int32_t>(ctx), (int32_t)B, (int32_t)depth,
                                ptr<int32_t>(length), ptr<int32_t>(fresh), stream()), "pikv_tree_accept");
     return wrap(fresh);
 }

@@ -6,6 +6,7 @@
 #include "tc_common.cuh"
 
 #include <type_traits>
+#include <utility>
 
 namespace pikv {
 
@@ -1109,6 +1110,11 @@ extern "C" int pikv_tree_attn(const pikv_paged_cache* c, const pikv_tree_params*
     return check_launch("tree_attn_kernel");
 }
 
+static bool apart(const int32_t* a, int64_t n, const int32_t* b, int64_t m) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return !a || !b || x + (uintptr_t)n * 4 <= y || y + (uintptr_t)m * 4 <= x;
+}
+
 extern "C" int pikv_tree_accept(const pikv_paged_cache* c, const int32_t* path, const int32_t* path_len, const int32_t* seq_ids,
                                 const int32_t* ctx_len, int32_t B, int32_t depth, int32_t* length, int32_t* new_len, pikv_stream_t stream) {
     AcceptDev d;
@@ -1117,6 +1123,13 @@ extern "C" int pikv_tree_accept(const pikv_paged_cache* c, const int32_t* path, 
     PIKV_REQUIRE((path || depth == 0) && ctx_len && new_len, PIKV_EINVAL, "tree_accept: null pointer");
     PIKV_REQUIRE(B > 0 && depth >= 0 && (seq_ids || B <= c->num_seqs), PIKV_EINVAL, "tree_accept: bad sizes");
     PIKV_REQUIRE(!(seq_ids && ctx_len == length), PIKV_EINVAL, "tree_accept: with seq_ids, ctx_len has an entry per stream of the call");
+    // a stream's CTA writes its lengths while others still read theirs
+    for (const auto& out : {std::make_pair((const int32_t*)length, (int64_t)c->num_seqs), std::make_pair((const int32_t*)new_len, (int64_t)B)}) {
+        auto lies_apart = [&](const int32_t* in, int64_t n) { return apart(out.first, out.second, in, n); };
+        PIKV_REQUIRE((out.first == ctx_len || lies_apart(ctx_len, B)) && lies_apart(path_len, B) && lies_apart(seq_ids, B) && lies_apart(path, (int64_t)B * depth),
+                     PIKV_EINVAL, "tree_accept: length and new_len overlap an input (only ctx_len itself may be either)");
+    }
+    PIKV_REQUIRE(apart(length, c->num_seqs, new_len, B), PIKV_EINVAL, "tree_accept: length and new_len overlap");
     d.depth = depth;
     d.all_ids = seq_ids;
     for (int b0 = 0; b0 < B; b0 += PIKV_STREAMS_PER_LAUNCH) {

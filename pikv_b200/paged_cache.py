@@ -184,7 +184,8 @@ class PagedKVCache(torch.nn.Module):
         ctx_len[b] + 1, ... and `length` of the stream becomes ctx_len[b] + path_len[b].  path int32 [B, depth]: node numbers,
         ascending (a node comes after its parent); path_len int32 [B] (default: depth).  Returns the new lengths int32 [B].  A path
         that is not ascending or leaves the cache moves nothing and shows in check_status(), as does a stream named twice (the
-        later entry is not carried out and returns 0).  Every cache format.  See pikv_tree_accept."""
+        later entry is not carried out and returns 0).  ctx_len may be a part of `length`: it is read as it was before the call.  Every
+        cache format.  See pikv_tree_accept."""
         return host().accept(self._buffers, self.num_seqs, self.n_kv, self.bits, self.symmetric, self.max_pages, self.num_pages,
                              path, path_len, seq_ids, ctx_len)
 

@@ -45,3 +45,24 @@ def test_bounds_of_pages_that_are_none(bits):
         assert int(cache.status) == 2
         cache.status.zero_()
         assert torch.equal(bounds.codes, want[0]) and torch.equal(bounds.scale, want[1])
+
+
+def test_accept_with_a_part_of_the_lengths():
+    """Contexts given as a slice of the cache's own lengths, of other streams than the entries' own: read as they were."""
+    S, N = 40, 5
+    lens = [17 + 3 * s for s in range(S)]
+    cache, gen = filled_cache([max(lens) + 3 + N] * S, 1, 8, seed=3)
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    path = torch.tensor([[1, 2, 4]] * (S - 1), dtype=torch.int32, device="cuda")
+    saved = {n: t.clone() for n, t in cache.named_buffers()}
+    for ids in (None, torch.arange(S - 2, -1, -1, dtype=torch.int32, device="cuda")):
+        got = []
+        for ctx in (length[1:].clone(), cache.length[1:]):
+            for n, t in cache.named_buffers():
+                t.copy_(saved[n])
+            cache.length.copy_(length)
+            new = cache.accept_tree(path, seq_ids=ids, ctx_len=ctx)
+            cache.check_status()
+            assert torch.equal(new, length[1:] + 3)
+            got.append([new] + [t.clone() for _, t in cache.named_buffers()])
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*got))

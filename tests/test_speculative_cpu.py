@@ -118,3 +118,21 @@ def test_abi_refusals():
     c.max_pages = 50000
     assert lib.pikv_sparse_attn(ref(c), ref(s), None) == -4
     assert lib.pikv_sparse_attn_workspace_bytes(4, 8, 2, 64, 16) > lib.pikv_decode_attn_workspace_bytes(4, 8, 2, 0, 0)
+
+
+def test_accept_overlapping_lengths():
+    """A part of the lengths, or of the new ones, as an input: another stream's entry would be read while it is written."""
+    from pikv_b200 import _lib
+    lib = _lib.lib()
+    words = (ctypes.c_uint32 * 64)()
+    at = (ctypes.addressof(words) + 15) & ~15                       # never read: every call is refused before a launch
+    c = _lib.PagedCache(page_table=at, num_seqs=4, max_pages=8, num_pages=32, n_kv=2, bits=8, symmetric=1, k_codes=at, v_codes=at, k_scale=at, v_scale=at)
+    apart, length, new = at + 160, at + 64, at + 96                 # `length`: four words, `new`: two
+
+    def call(path=apart, path_len=None, ids=None, ctx=apart, new_len=new):
+        return lib.pikv_tree_accept(ctypes.byref(c), path, path_len, ids, ctx, 2, 2, length, new_len, None), lib.pikv_last_error()
+
+    for over in (dict(ctx=length + 4), dict(ctx=length - 4), dict(ctx=length + 12, ids=apart), dict(ctx=new + 4), dict(ctx=new - 4), dict(path=length + 8),
+                 dict(path=new - 12), dict(path_len=length), dict(path_len=new), dict(ids=length + 12), dict(ids=new), dict(new_len=length + 12)):
+        rc, says = call(**over)
+        assert rc == -1 and b"overlap" in says, over
