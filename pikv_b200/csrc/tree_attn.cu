@@ -52,16 +52,20 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 //   9, 10  bulk copies of pages into two rings, K three tiles ahead, V two (one warp for both is late: 130 cycles a copy)
 //   11   the rows' scales in the forms that the converting warps and the softmax use
 // The query enters exactly: bf16 times a power of two per row that brings its largest entry to 2^14 is f16 down to 2^-38 of
-// that entry.  Keys and values enter as f16 of code * scale, in units of a power of two per tile (2^(e - 9), 2^e above the tile's
-// largest scale): one rounding, 2^-11 of the entry, the size of the weights' own; in return the softmax neither loads nor
-// multiplies by the scales (shared-memory reads of the scales by every row were the busiest pipe of the kernel that applied
-// them to exact integer products: 16 x 16384 x 32 nodes, 248 -> 221 us).
+// that entry.  Keys and values enter as f16 of code * scale, in units of a power of two per tile (2^(e + 9), 2^e above the tile's
+// largest scale): one rounding, 2^-11 of the entry, the size of the weights' own (decode_attention keeps the codes of K exact), and
+// 2^-25 of a unit where the entry is below f16's normal range; in return the softmax neither loads nor multiplies by the scales
+// (shared-memory reads of the scales by every row were the busiest pipe of the kernel that applied them to exact integer products:
+// 16 x 16384 x 32 nodes, 248 -> 221 us).
 //   logit = 2^(e_k + 9) / sqrt(128) q . K16
 //   O     = sum w V16,  w = f16(2^(logit - R + e_v + 9))
+// Where a row's scale lies more than 2^8 (4 bit: 2^4) below the tile's largest, every row has an e of its own, and the softmax applies
+// it to scores and weights: what a row holds, seen or not, takes no more than 2^-13 of another's largest entry from it.  (One such row in
+// every tile makes the call five times as long; a prompt has a few such tiles, at padding and at its first tokens.)
 // A 4-bit code has its zero point taken off first, exactly where that is a whole number below 2048 (with the zero points' parts
 // as products of their own in the softmax, it had to reload registers as well: 24 ragged streams to 6001, 103 -> 78 us, now 75).
-// R is a row's reference: the largest logit (log2 domain) plus e_v + 9 of the tile it was seen in, so that the weights sit at
-// the top of f16's range whatever the size of V; it moves only when a tile exceeds it by 2^TR_SLACK.  The denominator is
+// R is a row's reference: 2^TR_HEAD below the largest logit (log2 domain) plus e_v + 9 of the tile it was seen in, so that the weights sit
+// at the top of f16's range whatever the size of V; it moves only when a tile exceeds it by 2^TR_SLACK.  The denominator is
 // the fp32 sum of 2^(logit - R).  A row of V that is not finite enters as zeros and makes the result of the rows that see it
 // not a number; one that a row does not see does not reach it.
 //
@@ -74,7 +78,9 @@ constexpr int TR_K = 4, TR_V = 6, TR_MMA = 8, TR_COPY = 9, TR_SCALES = 11;      
 constexpr int TR_ROWS = 128;             // rows of a unit
 constexpr int TR_KEYS = 64;              // keys of a tile
 constexpr int TR_PAGES = TR_KEYS / PIKV_PAGE_TOKENS;
-constexpr float TR_SLACK = 8.f;
+constexpr float TR_HEAD = 7.f, TR_SLACK = 15.f;       // log2 of the largest weight where a reference is set, and where it is left
+template <int BITS> constexpr int TR_SPAN = BITS == 8 ? 8 : 4;      // binary orders that the scales of a tile with one unit may span
+constexpr uint32_t TR_ODD_V = 1, TR_OWN_V = 2, TR_OWN_K = 1u << 31;        // a row of V is not finite; the rows of K, of V have exponents of their own
 constexpr unsigned TR_WAIT_LIMIT = 1u << 24;
 constexpr uint32_t TR_COL_O = 0, TR_COL_S = 128, TR_COLS = 256;      // of a half: S of even and odd tiles, the weights in its first columns
 
@@ -93,9 +99,10 @@ template <int BITS, int H> struct TRSmem {
                          KMETA = VRING + TR_V_AHEAD * TR_PAGES * PAGE,         // [ahead][page] scales, zero points of K, of V
                          VMETA = KMETA + TR_K_AHEAD * TR_PAGES * META,
                          FACT = VMETA + TR_V_AHEAD * TR_PAGES * META,          // [sets][2][64] factors of the rows of K, of V
-                         VEXP = FACT + TR_SETS * 2 * TR_KEYS * FACTOR,         // [sets] 2^(e_k + 9), e_v + 9, 2^-(e_v + 9) as floats, whether a row of V is not finite
+                         VEXP = FACT + TR_SETS * 2 * TR_KEYS * FACTOR,         // [sets] 2^(e_k + 9), with the sign TR_OWN_K, e_v + 9, 2^-(e_v + 9) as floats, TR_ODD_V | TR_OWN_V
                          ODD = VEXP + TR_SETS * 16,                            // [sets][2] even and odd rows of V that are not finite, a bit each
-                         BARS = ODD + TR_SETS * 8, NBARS = 4 + 7 * H + 2 * TR_SETS + 2 * (TR_K_AHEAD + TR_V_AHEAD),
+                         EXPS = ODD + TR_SETS * 8,                             // [sets][2][64] exponents of the rows of K, of V that have their own
+                         BARS = EXPS + TR_SETS * 2 * TR_KEYS, NBARS = 4 + 7 * H + 2 * TR_SETS + 2 * (TR_K_AHEAD + TR_V_AHEAD),
                          PRE = BARS + NBARS * 8, MISC = PRE + (PIKV_STREAMS_PER_LAUNCH + 1) * 4, END = MISC + 16;
     static constexpr int BYTES = END + 1024;
 };
@@ -370,6 +377,59 @@ __device__ __forceinline__ void tr_weights(const float (&x)[32], uint32_t (&wgt)
     total += s0.x + s0.y;
 }
 
+// A tile whose rows have exponents of their own, sixteen scores of a row of S at a time: hardly ever met, and small so that the loops
+// around it keep their registers
+struct TROwn {
+    const unsigned char* at;              // bytes e of the 64 rows of K, of V
+    uint32_t all_k, all_v;                // or the tile's e four times
+    int ek;                               // the largest of K
+    bool k, v;
+    __device__ __forceinline__ TROwn(const unsigned char* exps, uint32_t flags, float of_k, float of_v) {
+        at = exps;
+        k = flags & TR_OWN_K;
+        v = flags & TR_OWN_V;
+        ek = (int)((__float_as_uint(of_k) >> 23) & 0xffu) - 136;
+        all_k = (uint32_t)(ek & 0xff) * 0x01010101u;
+        all_v = (uint32_t)(((int)of_v - 9) & 0xff) * 0x01010101u;
+    }
+    static __device__ __forceinline__ int byte(uint32_t w, int i) { return (int)(w << (24 - 8 * i)) >> 24; }
+    __device__ __forceinline__ uint32_t of_k(int j) const { return k ? *reinterpret_cast<const uint32_t*>(at + j) : all_k; }
+    __device__ __forceinline__ uint32_t of_v(int j) const { return v ? *reinterpret_cast<const uint32_t*>(at + TR_KEYS + j) : all_v; }
+    // returns the largest of the rows seen
+    __device__ __forceinline__ float scores(uint32_t taddr, uint64_t seen, float mul) const {
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < TR_KEYS; c += 16) {
+            float x[16];
+            uint32_t r[16];
+            lr_tmem_ld16(taddr + c, x);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int up = max(byte(of_k(c + (j & ~3)), j & 3) - ek, -126);
+                const float t = fmaf(x[j] * exp2_int(up), mul, (float)(byte(of_v(c + (j & ~3)), j & 3) + 9));
+                if ((seen >> (c + j)) & 1u) top = fmaxf(top, t);
+                r[j] = __float_as_uint(t);
+            }
+            tr_tmem_st16(taddr + c, r);
+        }
+        tr_tmem_st_wait();
+        return top;
+    }
+    // sum of 2^(logit + off) over the rows seen
+    __device__ __forceinline__ float total(uint32_t taddr, uint64_t seen, float off) const {
+        float sum = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < TR_KEYS; c += 16) {
+            float x[16];
+            lr_tmem_ld16(taddr + c, x);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if ((seen >> (c + j)) & 1u) sum += tr_ex2(x[j] + off - (float)(byte(of_v(c + (j & ~3)), j & 3) + 9));
+        }
+        return sum;
+    }
+};
+
 template <int BITS, int H>
 __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDev d, TreeParts parts) {
     using SM = TRSmem<BITS, H>;
@@ -526,28 +586,45 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                 // place that V of tile n - 3 left, behind the second product of tile n - 3 - H
                 cur.start(d, pre, f0);
                 const int count = f1 - f0;
-                auto side = [&](auto v_c, int n, int left, int s, uint32_t ph) {
-                    constexpr bool OF_V = decltype(v_c)::value;
-                    if (TR_RARE(!tr_wait((OF_V ? vr_full : kr_full) + 8 * s, ph))) return false;
-                    const unsigned char* own = smem + (OF_V ? SM::VMETA : SM::KMETA) + (s * TR_PAGES + (lane >> 3)) * SM::META;
-                    uint32_t two = 2 * lane < left ? *reinterpret_cast<const uint32_t*>(own + (lane & 7) * 4) : 0u;     // rows behind the end have none
-                    if (2 * lane + 1 == left) two &= 0xffffu;
+                // One piece of code for K and V: what this warp runs through pushes the loops of its neighbours out of the instruction cache
+                int ks = 0, vs = 0, left = 0, v_left = 0;
+                uint32_t kph = 0, vph = 0;
+#pragma unroll 1
+                for (int i = 0; i <= 2 * count; ++i) {                // K of 0; K of 1, V of 0; K of 2, V of 1; ..; V of count - 1
+                    const bool of_v = i > 0 && !(i & 1);
+                    const int n = of_v ? i / 2 - 1 : (i + 1) / 2, s = of_v ? vs : ks;
+                    if (!of_v) {
+                        v_left = left;
+                        if (n == count) continue;
+                        left = cur.end() - cur.tile * TR_KEYS;
+                    }
+                    if (TR_RARE(!tr_wait((of_v ? vr_full : kr_full) + 8 * s, of_v ? vph : kph))) { failed = true; break; }
+                    const int rows = of_v ? v_left : left;            // (none behind the end)
+                    const unsigned char* own = smem + (of_v ? SM::VMETA : SM::KMETA) + (s * TR_PAGES + (lane >> 3)) * SM::META;
+                    uint32_t two = 2 * lane < rows ? *reinterpret_cast<const uint32_t*>(own + (lane & 7) * 4) : 0u;
+                    if (2 * lane + 1 == rows) two &= 0xffffu;
                     const float s0 = __uint_as_float(two << 16), s1 = __uint_as_float(two & 0xffff0000u);
                     float z0 = 0.f, z1 = 0.f, top0 = s0, top1 = s1;               // top: a sixteenth of a row's largest entry, 4 bit
                     if (BITS == 4) {
-                        if (2 * lane < left) {
+                        if (2 * lane < rows) {
                             const float2 zp = *reinterpret_cast<const float2*>(own + 32 + (lane & 7) * 8);
                             z0 = zp.x;
-                            if (2 * lane + 1 < left) z1 = zp.y;
+                            if (2 * lane + 1 < rows) z1 = zp.y;
                         }
                         if (!(fabsf(z0) <= 16.f)) top0 = s0 * (fabsf(z0) * 0.0625f);
                         if (!(fabsf(z1) <= 16.f)) top1 = s1 * (fabsf(z1) * 0.0625f);
                     }
-                    const int e = __reduce_max_sync(0xffffffffu, max(tr_exponent(__float_as_uint(top0)), tr_exponent(__float_as_uint(top1))));
-                    const bool odd0 = !(fabsf(top0) < INFINITY), odd1 = !(fabsf(top1) < INFINITY);
+                    const int e0 = tr_exponent(__float_as_uint(top0)), e1 = tr_exponent(__float_as_uint(top1));
+                    const int e = __reduce_max_sync(0xffffffffu, max(e0, e1));
                     // a K that is not finite makes its logit so; a V enters as zeros
-                    const float up = exp2_int(15 - e), a0 = OF_V && odd0 ? 0.f : s0 * up, a1 = OF_V && odd1 ? 0.f : s1 * up;
-                    unsigned char* fact = smem + SM::FACT + ((tr_set(n) * 2 + OF_V) * TR_KEYS + 2 * lane) * SM::FACTOR;
+                    const bool odd0 = of_v && !(fabsf(top0) < INFINITY), odd1 = of_v && !(fabsf(top1) < INFINITY);
+                    // a row too far below the largest; what is 0 or below 2^-100, -100 here, has no say
+                    const bool far = __any_sync(0xffffffffu, min((uint32_t)(e0 + 99), (uint32_t)(e1 + 99)) < (uint32_t)max(e + 99 - TR_SPAN<BITS>, 0));
+                    const bool odd = __any_sync(0xffffffffu, odd0 || odd1);
+                    const int set = 2 * tr_set(n) + of_v;
+                    if (TR_RARE(far)) *reinterpret_cast<uint16_t*>(smem + SM::EXPS + set * TR_KEYS + 2 * lane) = (uint16_t)((e0 & 0xff) | (e1 & 0xff) << 8);
+                    const float a0 = odd0 ? 0.f : s0 * exp2_int(15 - (far ? e0 : e)), a1 = odd1 ? 0.f : s1 * exp2_int(15 - (far ? e1 : e));
+                    unsigned char* fact = smem + SM::FACT + (set * TR_KEYS + 2 * lane) * SM::FACTOR;
                     if constexpr (BITS == 8) {
                         *reinterpret_cast<uint32_t*>(fact) = tr_pack(a0, a1);
                     } else {
@@ -558,42 +635,34 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                             const float b = -z * UNIT * a - got.x * got.y;
                             return make_uint2(ac, tr_pack(b, b));
                         };
-                        const uint2 f0 = factors(a0, OF_V && odd0 ? 0.f : z0), f1 = factors(a1, OF_V && odd1 ? 0.f : z1);
+                        const uint2 f0 = factors(a0, odd0 ? 0.f : z0), f1 = factors(a1, odd1 ? 0.f : z1);
                         *reinterpret_cast<uint4*>(fact) = make_uint4(f0.x, f0.y, f1.x, f1.y);
                     }
-                    float* of = reinterpret_cast<float*>(smem + SM::VEXP + tr_set(n) * 16);
-                    if (OF_V) {
+                    if (TR_RARE(odd)) {
                         const uint32_t m0 = __ballot_sync(0xffffffffu, odd0), m1 = __ballot_sync(0xffffffffu, odd1);
-                        if (lane == 0) {
+                        if (lane == 0) *reinterpret_cast<uint2*>(smem + SM::ODD + tr_set(n) * 8) = make_uint2(m0, m1);
+                    }
+                    if (lane == 0) {
+                        float* of = reinterpret_cast<float*>(smem + SM::VEXP + tr_set(n) * 16);
+                        if (of_v) {
                             of[1] = (float)(e + 9);
-                            of[2] = exp2_int(-9 - e);
-                            of[3] = __uint_as_float(m0 | m1);
-                            *reinterpret_cast<uint2*>(smem + SM::ODD + tr_set(n) * 8) = make_uint2(m0, m1);
+                            *reinterpret_cast<float2*>(of + 2) = make_float2(exp2_int(-9 - e), __uint_as_float((odd ? TR_ODD_V : 0u) | (far ? TR_OWN_V : 0u)));
+                        } else {
+                            of[0] = __uint_as_float((uint32_t)(e + 136) << 23 | (far ? TR_OWN_K : 0u));
                         }
-                    } else if (lane == 0) {
-                        of[0] = exp2_int(e + 9);
                     }
                     tr_fence_smem();                                 // before the ring's place is given back
                     __syncwarp();
                     if (lane == 0) {
-                        lr_mbar_arrive((OF_V ? v_side : k_side) + 8 * tr_set(n));
-                        lr_mbar_arrive((OF_V ? vr_empty : kr_empty) + 8 * s);
+                        lr_mbar_arrive((of_v ? v_side : k_side) + 8 * tr_set(n));
+                        lr_mbar_arrive((of_v ? vr_empty : kr_empty) + 8 * s);
                     }
-                    return true;
-                };
-                int ks = 0, vs = 0, left = 0;
-                uint32_t kph = 0, vph = 0;
-                for (int n = 0; n <= count && !failed; ++n) {
-                    const int v_left = left;
-                    if (n < count) {
-                        left = cur.end() - cur.tile * TR_KEYS;
-                        if (TR_RARE(!side(std::false_type{}, n, left, ks, kph))) { failed = true; break; }
+                    if (of_v) {
+                        if (++vs == TR_V_AHEAD) vs = 0, vph ^= 1u;
+                    } else {
                         if (++ks == TR_K_AHEAD) ks = 0, kph ^= 1u;
                         if (n + 1 < count) cur.next(d, pre, f0 + n + 1);
                     }
-                    if (n == 0) continue;
-                    if (TR_RARE(!side(std::true_type{}, n - 1, v_left, vs, vph))) { failed = true; break; }
-                    if (++vs == TR_V_AHEAD) vs = 0, vph ^= 1u;
                 }
             }
         } else if (warp >= TR_K) {
@@ -650,21 +719,23 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
             int node = 0;
             bool live = false, warp_live = false;
             size_t out_row = 0;
-            // one tile: scores out, weights in.  EDGE: some of its positions lie behind the context
+            // One tile: scores out, weights in.  EDGE: some of its positions lie behind the context, or its rows have flags; a tile with
+            // flags is left to that form
+            enum { DONE, FAILED, FLAGGED };
             auto step = [&](auto edge_c, int n, int tile, bool first) {
                 constexpr bool EDGE = decltype(edge_c)::value;
-                if (TR_RARE(!tr_wait2(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u, v_side + 8 * tr_set(n), tr_set_phase(n)))) return false;
+                if (TR_RARE(!tr_wait2(s_full + 8 * (n & 1), (uint32_t)(n >> 1) & 1u, v_side + 8 * tr_set(n), tr_set_phase(n)))) return FAILED;
                 if (!warp_live) {
                     if (lane == 0) lr_mbar_arrive(p_full + 8 * (n & 1));
-                    return true;
+                    return DONE;
                 }
                 tr_fence_after();
                 const uint32_t scores = tmem + lanes + TR_COL_S + TR_KEYS * (n & 1);
                 float x0[32], x1[32];
                 tr_tmem_ld32(scores, x0);
                 tr_tmem_ld32(scores + 32, x1);
-                const float4 of = *reinterpret_cast<const float4*>(smem + SM::VEXP + tr_set(n) * 16);
-                float mul = qmul * of.x;
+                float4 of = *reinterpret_cast<const float4*>(smem + SM::VEXP + tr_set(n) * 16);
+                float mul = qmul * fabsf(of.x);
                 if (mul == 0.f) mul = 1.17549435e-38f;                   // (masked scores are -infinity: times 0 they would not be a number)
                 uint64_t seen = ~0ull;
                 if (EDGE) {
@@ -672,19 +743,9 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                     const int sh = cur.ctx - tile * TR_KEYS;             // the tree's first bit
                     seen = sh >= 0 ? (sh < 64 ? tree << sh : 0ull) | (sh < 64 ? (1ull << sh) - 1 : ~0ull) : (sh > -64 ? tree >> -sh : 0ull);
                 }
-                if (TR_RARE(__float_as_uint(of.w) != 0u)) {
-                    const uint2 odd = *reinterpret_cast<const uint2*>(smem + SM::ODD + tr_set(n) * 8);
-                    for (int j = 0; j < TR_KEYS; ++j)
-                        if (((j & 1 ? odd.y : odd.x) >> (j >> 1)) & (uint32_t)(seen >> j) & 1u) odd_v = __uint_as_float(0x7fffffffu);
-                }
-                tr_tmem_ld_wait(x0);
-                tr_tmem_ld_wait(x1);
-                const float mx = fmaxf(tr_scores<EDGE>(x0, (uint32_t)seen), tr_scores<EDGE>(x1, (uint32_t)(seen >> 32)));
-                // does the reference hold?  (-inf while nothing has been seen)
-                const float want = mx * mul + of.y;
-                const bool move = mx > -INFINITY && want > ref + TR_SLACK;
-                if (TR_RARE(__any_sync(0xffffffffu, move))) {
-                    const float next = move ? want : ref;
+                // the reference moves to `want` where `move`
+                auto refer = [&](float want, bool move) {
+                    const float next = move ? want - TR_HEAD : ref;
                     const float fac = move ? tr_ex2(ref - next) : 1.f;     // 0 from -inf
                     ref = next;
                     den *= fac;
@@ -702,7 +763,38 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                         }
                         tr_tmem_st_wait();
                     }
+                    return true;
+                };
+                const uint32_t flags = __float_as_uint(of.w) | (__float_as_uint(of.x) & TR_OWN_K);
+                if (TR_RARE(flags != 0u)) {
+                    tr_tmem_ld_wait(x0);                                 // (the loads above land before their registers are taken again)
+                    tr_tmem_ld_wait(x1);
+                    if constexpr (!EDGE) return FLAGGED;
+                    if (flags & TR_ODD_V) {
+                        const uint2 odd = *reinterpret_cast<const uint2*>(smem + SM::ODD + tr_set(n) * 8);
+                        for (int j = 0; j < TR_KEYS; ++j)
+                            if (((j & 1 ? odd.y : odd.x) >> (j >> 1)) & (uint32_t)(seen >> j) & 1u) odd_v = __uint_as_float(0x7fffffffu);
+                    }
+                    if (flags & (TR_OWN_K | TR_OWN_V)) {
+                        // scores in the reference's units, where they lie: logit + e_v + 9 of each row; the denominator's part as well
+                        const TROwn own_e(smem + SM::EXPS + tr_set(n) * 2 * TR_KEYS, flags, of.x, of.y);
+                        const float want = own_e.scores(scores, seen, mul);
+                        const bool move = want > ref + TR_SLACK;
+                        if (__any_sync(0xffffffffu, move) && !refer(want, move)) return FAILED;
+                        den += own_e.total(scores, seen, ref == -INFINITY ? 0.f : -ref);
+                        tr_tmem_ld32(scores, x0);
+                        tr_tmem_ld32(scores + 32, x1);
+                        mul = 1.f;
+                        of.y = of.z = 0.f;
+                    }
                 }
+                tr_tmem_ld_wait(x0);
+                tr_tmem_ld_wait(x1);
+                const float mx = fmaxf(tr_scores<EDGE>(x0, (uint32_t)seen), tr_scores<EDGE>(x1, (uint32_t)(seen >> 32)));
+                // does the reference hold?  (-inf while nothing has been seen)
+                const float want = mx * mul + of.y;
+                const bool move = mx > -INFINITY && want > ref + TR_SLACK;
+                if (TR_RARE(__any_sync(0xffffffffu, move)) && !refer(want, move)) return FAILED;
                 const float off = of.y - (ref == -INFINITY ? 0.f : ref);
                 float total = 0.f;
                 // the weights take the place of the scores that they come from, two to a column
@@ -716,7 +808,7 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                 tr_fence_before();
                 __syncwarp();
                 if (lane == 0) lr_mbar_arrive(p_full + 8 * (n & 1));
-                return true;
+                return DONE;
             };
             for (int n = 0, f = f0; f < f1;) {
                 // ---- a unit, or the part of it that this CTA has: tiles t0 .. t1 - 1 ----
@@ -779,8 +871,13 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                         if (node == i) tree = (uint64_t)m1 << 32 | m0;
                     }
                 }
-                for (int t = t0; t < edge && !failed; ++t, ++n) failed = !step(std::false_type{}, n, t, t == t0);
-                for (int t = edge; t < t1 && !failed; ++t, ++n) failed = !step(std::true_type{}, n, t, t == t0);
+                for (int t = t0; t < t1; ++t, ++n) {
+                    int did = DONE;
+                    for (; t < edge; ++t, ++n)
+                        if ((did = step(std::false_type{}, n, t, t == t0)) != DONE) break;
+                    if (did == FAILED || (t < t1 && step(std::true_type{}, n, t, t == t0) == FAILED)) { failed = true; break; }
+                    if (t >= t1) break;
+                }
                 if (failed) break;
                 // ---- this CTA's share of the unit is done ----
                 if (TR_RARE(!tr_wait(pv_done + 8 * ((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u))) { failed = true; break; }

@@ -66,3 +66,95 @@ def test_accept_with_a_part_of_the_lengths():
             assert torch.equal(new, length[1:] + 3)
             got.append([new] + [t.clone() for _, t in cache.named_buffers()])
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*got))
+
+
+# ---- rows of unlike sizes -------------------------------------------------------------------------------------------
+# K and V of a row enter as f16: 2^-11 of each entry, and 2^-25 of a unit (2^9 times the power of two above the tile's largest scale, or
+# the row's own) where the entry is below f16's normal range.  Rows up to 2^8 (8 bit; largest entry 127 scales) or 2^4 (4 bit; 7.5 scales)
+# below their tile's largest scale share its unit, so that this is at most 2^-25 2^9 2^9 / 127 < 2^-13, or 2^-25 2^9 2^5 / 7.5 < 2^-13,
+# of the row's largest entry.  A weight: 2^-11, and 2^-25 of a reference that the largest weighted row exceeds by 2^7 / 2^9 at least.
+def weighted_bound(q, k, v, sees):
+    """want [R, n_q, 128] and how far a kernel may be off it, relative to what each row really brings in: a logit's error is that of
+    its own key, a value's that of its own row."""
+    R, n_q, _ = q.shape
+    L, n_kv, _ = k.shape
+    x = q.double().view(R, n_kv, n_q // n_kv, D)
+    shut = ~sees[:, None, None]
+    s = torch.einsum("rhgd,lhd->rhgl", x, k).masked_fill(shut, -math.inf) / math.sqrt(D)
+    p = torch.softmax(s, -1)
+    slip = torch.einsum("rhgd,lhd->rhgl", x.abs(), (2.0 ** -11 + 264 * 2.0 ** -24) * k.abs() + 2.0 ** -13 * k.abs().amax(-1, keepdim=True)) / math.sqrt(D)
+    slip = torch.minimum(slip + 2.0 ** -20 * (1 + s.abs().nan_to_num(posinf=0)), torch.ones_like(slip)).masked_fill(shut, 0)
+    size = v.abs().amax(-1).permute(1, 0)[None, :, None]                                              # [1, n_kv, 1, L]
+    whole = (p * size).sum(-1)
+    off = (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -13 + L * 2.0 ** -23 + 2.0 ** -20) * whole + (p * slip * size).sum(-1) + (p * slip).sum(-1) * whole
+    want = torch.einsum("rhgl,lhd->rhgd", p, v).reshape(R, n_q, D)
+    return want, 2.0 ** -8 * want.abs() + 1.1 * off.reshape(R, n_q, 1)
+
+
+def check_weighted(cache, q, mask, ctx, out, nodes=None):
+    for b in range(q.shape[0]):
+        n, N = int(ctx[b]), q.shape[1]
+        k, v = rows64(cache, b, n + N)
+        sees = torch.cat([torch.ones(N, n, dtype=torch.bool, device="cuda"), mask[b] if mask.dim() == 3 else mask], 1)
+        want, far = weighted_bound(q[b], k, v, sees)
+        off = (out[b].double() - want).abs()
+        assert bool((off <= far).all()), f"stream {b}: off by {float((off / far).max())} of what its roundings allow"
+
+
+def grow(cache, stream, pos, factor, which):
+    """A row times a power of two, exactly."""
+    getattr(cache, which + "_scale")[int(cache.page_table[stream, pos // PAGE]), :, pos % PAGE] *= factor
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("size", [4, 8, 9, 14, 20, 30, 70])
+@pytest.mark.parametrize("n_kv,G,N", [(2, 4, 8), (1, 8, 64)])
+def test_tree_row_that_is_not_seen(bits, which, size, n_kv, G, N):
+    """A drafted row that most nodes do not see, 2^size times the others: those nodes' results are as exact as without it."""
+    ctx = [150, 1000]
+    cache, gen = filled_cache([n + N for n in ctx], n_kv, bits, seed=size)
+    q = torch.randn(2, N, n_kv * G, D, generator=gen, device="cuda").bfloat16()
+    mask = torch.eye(N, dtype=torch.bool, device="cuda")
+    mask[5, 4] = True
+    length = torch.tensor(ctx, dtype=torch.int32, device="cuda")
+    for b, n in enumerate(ctx):
+        grow(cache, b, n + 4, 2.0 ** size, which)
+    out, lse = cache.decode_attention_tree(q, mask, ctx_len=length, want_lse=True)
+    cache.check_status()
+    check_weighted(cache, q, mask, length, out)
+    for b, n in enumerate(ctx):
+        k, v = rows64(cache, b, n + N)
+        sees = torch.cat([torch.ones(N, n, dtype=torch.bool, device="cuda"), mask], 1)
+        rest = [i for i in range(N) if i not in (4, 5)]
+        want = attend64(q[b], k, v, sees)[1]
+        assert bool(((lse[b].double() - want).abs()[rest] <= 2.0 ** -7).all())
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("size", [6, 16, 24, 40])
+def test_tree_rows_of_unlike_sizes(bits, size):
+    """Context rows whose keys and values lie up to 2^size apart, in every tile and in tiles of their own; large values under small
+    weights, so that rows of all sizes have their share in the result; rows of zeros."""
+    n_kv, G, N, ctx = 2, 4, 12, [700, 64, 130]
+    cache, gen = filled_cache([n + N for n in ctx], n_kv, bits, seed=size + 100)
+    for b, n in enumerate(ctx):
+        L = n + N
+        k, v = (torch.randn(L, n_kv, D, generator=gen, device="cuda") for _ in range(2))
+        e = torch.randint(0, size + 1, (L, 1, 1), generator=gen, device="cuda").float()
+        if b == 0:
+            e[:320] = torch.randint(0, size + 1, (5, 1, 1), generator=gen, device="cuda").float().repeat_interleave(64, 0)
+        # the key's first channel makes a logit smaller by e ln 2 with a query of -sqrt(128) there: a value 2^e larger weighs the same
+        k[..., 0] = e[..., 0] * math.log(2)
+        v = v * 2.0 ** e
+        k[3::17] *= 2.0 ** -size
+        k[5::23], v[5::23] = 0, 0
+        append_rows(cache, b, 0, k.reshape(L, -1).bfloat16(), v.reshape(L, -1).bfloat16())
+    q = torch.randn(len(ctx), N, n_kv * G, D, generator=gen, device="cuda")
+    q[..., 0] = -math.sqrt(D)
+    q = q.bfloat16()
+    mask = torch.rand(len(ctx), N, N, generator=gen, device="cuda") < 0.5
+    length = torch.tensor(ctx, dtype=torch.int32, device="cuda")
+    out = cache.decode_attention_tree(q, mask, ctx_len=length)
+    cache.check_status()
+    check_weighted(cache, q, mask, length, out)
