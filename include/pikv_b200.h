@@ -563,7 +563,11 @@ typedef struct {
  *   mask: bytes [N, N], or [B, N, N] with mask_per_stream != 0
  *   nodes (optional) [B]: nodes of each stream, 0 .. N; those behind are neither seen nor computed, their rows
  *   of out are zero and their lse -infinity, as for a node that sees nothing
- *   lse (optional) [B, N, n_q] fp32 log-sum-exp of the scaled scores */
+ *   lse (optional) [B, N, n_q] fp32 log-sum-exp of the scaled scores
+ * K and V are taken as f16 in units of a power of two that follows their rows' scales (2^-11 of an entry, at most 2^-13 of
+ * its row's largest; pikv_decode_attn_q8 keeps the codes of K exact), whatever other rows hold.  A row whose scale, or 4-bit
+ * scale times zero point / 16, is not below 2^117 counts as not finite.  What is not finite, K, V or the query itself, makes
+ * the results not a number that it takes part in, and no others. */
 typedef struct {
     const void* q; void* out; float* lse;
     int32_t B, N, n_q;

@@ -236,10 +236,12 @@ __device__ __forceinline__ uint32_t tr_pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// exponent of a scale, for the reference; what is not finite has no say in it
+// exponent of a scale, for the reference; what is not finite has no say in it.  2^(e + 9) and 2^-(e + 9) are finite up to TR_MOST
+constexpr int TR_MOST = 117;
+constexpr float TR_HUGE = 1.661534995e35f;              // 2^117: a row whose scale is not below it counts as not finite
 __device__ __forceinline__ int tr_exponent(uint32_t bits) {
     const int e = (int)((bits >> 23) & 0xffu);
-    return e == 255 ? -100 : min(100, max(-100, e - 126));
+    return e == 255 ? -100 : min(TR_MOST, max(-100, e - 126));
 }
 // position of a channel inside its group of eight in the 4-bit tiles: nibbles leave a word as (0, 4), (1, 5), (2, 6), (3, 7)
 template <int BITS> __device__ __forceinline__ constexpr int tr_channel(int at) { return BITS == 8 ? at : (at & ~7) | ((at & 7) >> 1) | ((at & 1) << 2); }
@@ -617,7 +619,7 @@ __global__ void __launch_bounds__(H * TR_THREADS, 2 / H) tree_attn_kernel(TreeDe
                     const int e0 = tr_exponent(__float_as_uint(top0)), e1 = tr_exponent(__float_as_uint(top1));
                     const int e = __reduce_max_sync(0xffffffffu, max(e0, e1));
                     // a K that is not finite makes its logit so; a V enters as zeros
-                    const bool odd0 = of_v && !(fabsf(top0) < INFINITY), odd1 = of_v && !(fabsf(top1) < INFINITY);
+                    const bool odd0 = of_v && !(fabsf(top0) < TR_HUGE), odd1 = of_v && !(fabsf(top1) < TR_HUGE);
                     // a row too far below the largest; what is 0 or below 2^-100, -100 here, has no say
                     const bool far = __any_sync(0xffffffffu, min((uint32_t)(e0 + 99), (uint32_t)(e1 + 99)) < (uint32_t)max(e + 99 - TR_SPAN<BITS>, 0));
                     const bool odd = __any_sync(0xffffffffu, odd0 || odd1);

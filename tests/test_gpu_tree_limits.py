@@ -158,3 +158,26 @@ def test_tree_rows_of_unlike_sizes(bits, size):
     out = cache.decode_attention_tree(q, mask, ctx_len=length)
     cache.check_status()
     check_weighted(cache, q, mask, length, out)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("size", [1e31, 1e33, 1e35])
+def test_tree_large_values(bits, size):
+    """Keys and values up to the size where a row counts as not finite (scales of 2^117), queries that bring the logits back."""
+    N, n_kv, G = 6, 2, 4
+    cache, gen = filled_cache([300], n_kv, bits, seed=17)
+    k, v = (torch.randn(300, n_kv * D, generator=gen, device="cuda") * size for _ in range(2))
+    append_rows(cache, 0, 0, k.bfloat16(), v.bfloat16())
+    q = (torch.randn(1, N, n_kv * G, D, generator=gen, device="cuda") / size).bfloat16()
+    mask = torch.ones(N, N, dtype=torch.bool, device="cuda").tril()
+    ctx = torch.tensor([300 - N], dtype=torch.int32, device="cuda")
+    out = cache.decode_attention_tree(q, mask, ctx_len=ctx)
+    cache.check_status()
+    check_weighted(cache, q, mask, ctx, out)
+    # one row of them, seen by none of the others, among rows of 1
+    n = 300 - N
+    append_rows(cache, 0, 0, torch.randn(n, n_kv * D, generator=gen, device="cuda").bfloat16(), torch.randn(n, n_kv * D, generator=gen, device="cuda").bfloat16())
+    q = torch.randn(1, N, n_kv * G, D, generator=gen, device="cuda").bfloat16()
+    mask = torch.zeros(N, N, dtype=torch.bool, device="cuda")
+    out = cache.decode_attention_tree(q, mask, ctx_len=ctx)
+    check_weighted(cache, q, mask, ctx, out)
