@@ -225,6 +225,16 @@ __global__ void __launch_bounds__(PB_THREADS, PB_CTAS) page_bounds_kernel(Bounds
                     }
                 }
             }
+            // a bound too small for its quotient by the step to be a float is a step all the same: 2^-40 of the largest stands for it
+            float a = 0.f;
+#pragma unroll
+            for (int k = 0; k < CH; ++k) a = fmaxf(a, fmaxf(hi[k], -lo[k]));
+            const float some = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a))) * 9.094947e-13f;
+#pragma unroll
+            for (int k = 0; k < CH; ++k) {
+                if (hi[k] > 0.f) hi[k] = fmaxf(hi[k], some);
+                if (lo[k] < 0.f) lo[k] = fminf(lo[k], -some);
+            }
         }
         int at = 4 * lane;
         if (BITS == 4) {

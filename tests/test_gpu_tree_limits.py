@@ -68,6 +68,30 @@ def test_accept_with_a_part_of_the_lengths():
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*got))
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+def test_bounds_of_unlike_rows(bits):
+    """A channel whose keys are so far below the page's largest that their quotient by a step is no float: bounds still lie outside."""
+    cache, gen = filled_cache([48], 1, bits, seed=29)
+    k = torch.randn(48, D, generator=gen, device="cuda") * 2.0 ** -70
+    k[3] = torch.randn(D, generator=gen, device="cuda") * 2.0 ** 100
+    k[20] = k[3] * 2.0 ** -100
+    k[3, 40:60], k[20, 40:60] = 0, 0
+    k[16:32, 50:] = k[16:32, 50:].abs()
+    k[16:32, :10] = -k[16:32, :10].abs()
+    append_rows(cache, 0, 0, k.bfloat16(), k.bfloat16())
+    if bits == 4:                                                      # the quantiser has no scales that small
+        page = int(cache.page_table[0, 0])
+        cache.k_scale[page, 0, [i for i in range(16) if i != 3]] *= 2.0 ** -60
+    bounds = cache.page_bounds()
+    cache.update_bounds(bounds, seq_len=torch.tensor([48], dtype=torch.int32, device="cuda"))
+    cache.check_status()
+    rows, _ = rows64(cache, 0, 48)
+    for p in range(3):
+        codes, scale = bounds64(rows[p * PAGE:(p + 1) * PAGE])
+        page = int(cache.page_table[0, p])
+        assert torch.equal(bounds.scale[page].double(), scale) and torch.equal(bounds.codes[page].double(), codes)
+
+
 # ---- rows of unlike sizes -------------------------------------------------------------------------------------------
 # K and V of a row enter as f16: 2^-11 of each entry, and 2^-25 of a unit (2^9 times the power of two above the tile's largest scale, or
 # the row's own) where the entry is below f16's normal range.  Rows up to 2^8 (8 bit; largest entry 127 scales) or 2^4 (4 bit; 7.5 scales)
