@@ -384,3 +384,87 @@ def test_bounds_repeats(bits):
         cache.update_bounds(again)
         assert torch.equal(again.codes * (again.scale > 0)[..., None, None], first.codes) and torch.equal(again.scale, first.scale)
     cache.check_status()
+
+
+# an infinite page among ordinary ones stretches the range that the selection cuts into bins, so that nearly all of them lie in one bin
+# and are cut again, by several orders; all of them equal, too; several of them; more than there is room for
+@pytest.mark.parametrize("pages", [60, 700, 1500])
+@pytest.mark.parametrize("infinite", [1, 3, 1900])
+@pytest.mark.parametrize("equal", [False, True])
+def test_selection_with_infinite_pages(pages, infinite, equal):
+    P = 2048
+    cache, gen = filled_cache([P * PAGE], 1, 8, seed=pages + infinite)
+    lens = torch.tensor([P * PAGE], dtype=torch.int32, device="cuda")
+    bounds = cache.page_bounds()
+    cache.update_bounds(bounds, seq_len=lens)
+    at = cache.page_table[0].long()
+    if equal:
+        bounds.codes[at] = bounds.codes[at[:1]].clone()
+        bounds.scale[at] = bounds.scale[at[:1]].clone()
+    bounds.scale[at[torch.randperm(P, generator=gen, device="cuda")[:infinite]]] = math.inf
+    for size in (1.0, 1e-4):                                           # scores of both signs, and small ones
+        q = (torch.randn(1, 4, D, generator=gen, device="cuda") * size).bfloat16()
+        for first, recent in ((0, 1), (2, 5)):
+            got = cache.decode_attention_sparse(q, bounds, pages, seq_len=lens, first=first, recent=recent, want_pages=True)[1]
+            assert got[0, 0].tolist() == chosen64(q[0], bounds.codes[at], bounds.scale[at], pages, first, recent)[0]
+    cache.check_status()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("rows,pages,n_kv,G", [([9000, 3001, 777], 300, 1, 4), ([40000], 600, 2, 4), ([5000, 5016], 40, 3, 8)])
+def test_sparse_reads_the_chosen_pages(bits, rows, pages, n_kv, G):
+    """Each page's values are its own number (K alike, so that all rows weigh the same): the result is the mean over the pages
+    read, and one page more, less or another one shows."""
+    cache, gen = filled_cache(rows, n_kv, bits, seed=71)
+    lens = torch.tensor(rows, dtype=torch.int32, device="cuda")
+    bounds = cache.page_bounds()
+    cache.update_bounds(bounds, seq_len=lens)
+    q = torch.randn(len(rows), n_kv * G, D, generator=gen, device="cuda").bfloat16()
+    # the choice is by these bounds; then all keys become 0 and a page's values a pattern of its number in base 2
+    bit = 2 ** (torch.arange(D, device="cuda") % 12)
+    for s, n in enumerate(rows):
+        page = torch.arange(n, device="cuda") // PAGE
+        v = torch.where((page[:, None] & bit) > 0, 1.0, -1.0).repeat(1, n_kv)
+        append_rows(cache, s, 0, torch.zeros(n, n_kv * D, device="cuda").bfloat16(), v.bfloat16())
+    out, lse, chosen = cache.decode_attention_sparse(q, bounds, pages, seq_len=lens, want_lse=True, want_pages=True)
+    cache.check_status()
+    for b, n in enumerate(rows):
+        at = cache.page_table[b, :(n + PAGE - 1) // PAGE].long()
+        want = chosen64(q[b], bounds.codes[at], bounds.scale[at], pages, 0, 1)
+        _, v = rows64(cache, b, n)
+        for h in range(n_kv):
+            sees = torch.zeros(len(at), PAGE, dtype=torch.bool, device="cuda")
+            sees[want[h]] = True
+            seen = sees.view(-1)[:n]
+            L = int(seen.sum())
+            mean = v[seen, h].mean(0)
+            heads = slice(h * G, (h + 1) * G)
+            # Logits are exactly 0, so all weights are equal: their rounding and that of their product with the values' scale to f16 are
+            # 2^-11 each of the mean (at most 1), sums in fp32 far below; then the rounding to bf16.  A page more or less moves the
+            # log-sum-exp by 1 / pages and a channel whose mean is near 0 by as much, another page the channels in which they differ by twice that
+            assert bool(((out[b, heads].double() - mean).abs() <= 2.0 ** -8 * mean.abs() + 2.0 ** -10).all())
+            assert bool(((lse[b, heads].double() - math.log(L)).abs() <= 2.0 ** -20 * math.log(L)).all())
+
+
+def test_dense_decode_with_garbage_behind_the_end():
+    """Rows behind a stream's end on its last page, with scales and zero points that are not finite, do not reach decode_attention."""
+    for bits in (8, 4):
+        rows = [1, 17, 100, 333, 2000]
+        cache, gen = filled_cache(rows, 2, bits, seed=81)              # what it leaves unwritten is NaN
+        clean, _ = filled_cache(rows, 2, bits, seed=81)
+        for name, t in clean.named_buffers():
+            if name.endswith(("_scale", "_zp")):
+                t.nan_to_num_(0)
+        lens = torch.tensor(rows, dtype=torch.int32, device="cuda")
+        for G in (1, 4, 8):
+            q = torch.randn(len(rows), 2 * G, D, generator=gen, device="cuda").bfloat16()
+            for fill in (math.nan, math.inf, -math.inf):
+                for name in ("k_scale", "v_scale") + (("k_zp", "v_zp") if bits == 4 else ()):
+                    t = getattr(cache, name)
+                    t[torch.isnan(t) | torch.isinf(t)] = fill
+                got, want = cache.decode_attention(q, seq_len=lens), clean.decode_attention(q, seq_len=lens)
+                assert bool(torch.isfinite(got).all()) and torch.equal(got, want)
+                for name in ("k_scale", "v_scale") + (("k_zp", "v_zp") if bits == 4 else ()):
+                    t = getattr(cache, name)
+                    t[torch.isinf(t)] = math.nan
+        cache.check_status()

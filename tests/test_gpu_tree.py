@@ -358,3 +358,46 @@ def test_accept_refused_paths():
     assert int(cache.status) == 2 and new.tolist() == [41]
     cache.status.zero_()
     assert all(torch.equal(t.view(torch.uint8), held[n].view(torch.uint8)) for n, t in buffers(cache).items())
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_accept_many_streams(bits):
+    """More streams than one launch takes, without ids and with ids in any order; a stream named in both launches is carried out once."""
+    S, N, n_kv = 600, 6, 1
+    ctx = [3 + (i * 37) % 60 for i in range(S)]
+    cache, gen = filled_cache([n + N for n in ctx], n_kv, bits, seed=18)
+    length = torch.tensor(ctx, dtype=torch.int32, device="cuda")
+    path = torch.stack([torch.randperm(N, generator=gen, device="cuda")[:4].sort().values for _ in range(S)]).int()
+    count = torch.randint(0, 5, (S,), generator=gen, device="cuda").int()
+    saved = {n: t.clone() for n, t in cache.named_buffers()}
+    before = [rows64(cache, s, ctx[s] + N) for s in range(S)]
+
+    def check(streams, new):
+        for b, s in enumerate(streams):
+            c = int(count[b])
+            at = torch.arange(ctx[s] + N, device="cuda")
+            at[ctx[s]:ctx[s] + c] = ctx[s] + path[b, :c].long()
+            assert int(new[b]) == ctx[s] + c == int(cache.length[s])
+            assert all(torch.equal(x, y[at]) for x, y in zip(rows64(cache, s, ctx[s] + N), before[s]))
+
+    cache.length.copy_(length)
+    new = cache.accept_tree(path, count)                               # the cache's own lengths, read and written
+    cache.check_status()
+    check(range(S), new)
+    for twice in (False, True):
+        for n, t in cache.named_buffers():
+            t.copy_(saved[n])
+        cache.length.copy_(length)
+        ids = torch.randperm(S, generator=gen, device="cuda").int()
+        if twice:
+            ids[530] = ids[7]                                          # 7 goes with the first launch, 530 with the second
+        new = cache.accept_tree(path, count, seq_ids=ids, ctx_len=length[ids.long()].contiguous())
+        if twice:
+            assert int(cache.status) == 1 and int(new[530]) == 0
+            cache.status.zero_()
+            keep = [b for b in range(S) if b != 530]
+            left_out = set(range(S)) - set(ids.tolist())
+            assert all(torch.equal(x, y) for s in left_out for x, y in zip(rows64(cache, s, ctx[s] + N), before[s]))
+            path, count, new, ids = path[keep], count[keep], new[keep], ids[keep]
+        cache.check_status()
+        check(ids.tolist(), new)
