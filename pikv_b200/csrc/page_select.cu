@@ -399,7 +399,9 @@ __global__ void __launch_bounds__(PS_THREADS, PS_CTAS) page_score_kernel(SelectD
                 qf[w] = pos;
                 qf[8 + w] = neg;
             }
-            const float sq = fin && r < d.G ? exp2_int(e) : 0.f;
+            // only ratios matter: relative to the group's largest step, and so small that products with a page's step stay in fp32's range
+            const int e_most = __reduce_max_sync(0xffffffffu, fin && r < d.G ? e : -126);
+            const float sq = fin && r < d.G ? exp2_int(max(-126, e - e_most - 23)) : 0.f;
             sq0 = __shfl_sync(0xffffffffu, sq, 8 * j);
             sq1 = __shfl_sync(0xffffffffu, sq, 8 * j + 4);
         }
@@ -432,8 +434,8 @@ __global__ void __launch_bounds__(PS_THREADS, PS_CTAS) page_score_kernel(SelectD
             ps_mma(acc, wl[i].x, wh[i].x, wl[i].y, wh[i].y, qf[4 * i], qf[4 * i + 1]);
             ps_mma(acc, wl[i].z, wh[i].z, wl[i].w, wh[i].w, qf[4 * i + 2], qf[4 * i + 3]);
         }
-        // (whole number * page step) * query step, and the best of the group's heads
-        auto score = [&](int dot, float sp, float sq) { return sq > 0.f ? ((float)dot * sp) * sq : -INFINITY; };
+        // (whole number below 2^23 * query step) * page step, and the best of the group's heads
+        auto score = [&](int dot, float sp, float sq) { return sq > 0.f ? ((float)dot * sq) * sp : -INFINITY; };
         float t_lo = fmaxf(score(acc[0], s_lo, sq0), score(acc[1], s_lo, sq1));
         float t_hi = fmaxf(score(acc[2], s_hi, sq0), score(acc[3], s_hi, sq1));
 #pragma unroll

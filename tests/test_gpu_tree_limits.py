@@ -205,3 +205,21 @@ def test_tree_large_values(bits, size):
     mask = torch.zeros(N, N, dtype=torch.bool, device="cuda")
     out = cache.decode_attention_tree(q, mask, ctx_len=ctx)
     check_weighted(cache, q, mask, ctx, out)
+
+
+# ---- the choice of pages ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("key,query", [(-60, -118), (108, 10), (-100, -40), (100, 100)])
+def test_page_scores_of_any_size(key, query):
+    """Scores whose sizes are beyond fp32's are ranked all the same: only their ratios matter."""
+    P, G = 300, 4
+    cache, gen = filled_cache([P * PAGE], 2, 8, seed=23)
+    lens = torch.tensor([P * PAGE], dtype=torch.int32, device="cuda")
+    bounds = cache.page_bounds()
+    cache.update_bounds(bounds, seq_len=lens)
+    q = torch.randn(1, 2 * G, D, generator=gen, device="cuda").bfloat16()
+    q[:, 1] *= 2.0 ** -9                                               # heads of a group of unlike sizes
+    _, want = cache.decode_attention_sparse(q, bounds, 20, seq_len=lens, want_pages=True)
+    bounds.scale *= 2.0 ** key
+    _, got = cache.decode_attention_sparse((q.float() * 2.0 ** query).bfloat16(), bounds, 20, seq_len=lens, want_pages=True)
+    cache.check_status()
+    assert torch.equal(got, want)
