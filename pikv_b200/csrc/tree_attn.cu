@@ -29,7 +29,7 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
     nodes = row < 0 ? 0 : d.nodes ? max(0, min(__ldg(d.nodes + i), d.N)) : d.N;
     const int most = d.c.max_pages * PIKV_PAGE_TOKENS;
     const int ctx = row < 0 ? 0 : max(0, min(__ldg(d.ctx_len + i), most));
-    if (ctx + nodes > most) {                                   // the tree does not fit behind its context
+    if (nodes > most - ctx) {                                   // the tree does not fit behind its context (whose end may be next to 2^31)
         nodes = most - ctx;
         if (d.c.status) atomicOr(d.c.status, PIKV_ST_BAD_INDEX);
     }
@@ -120,7 +120,8 @@ struct TreeParts {
     int halves;                          // of a CTA
 };
 
-__device__ __forceinline__ int tree_tiles(int ctx, int nodes) { return (ctx + nodes + TR_KEYS - 1) / TR_KEYS; }
+// (the rows are below 2^31, not so with the rounding up)
+__device__ __forceinline__ int tree_tiles(int ctx, int nodes) { return (int)(((uint32_t)(ctx + nodes) + TR_KEYS - 1) / TR_KEYS); }
 // units of a head: TR_ROWS rows for each half of a CTA
 __device__ __forceinline__ int tree_row_tiles(int nodes, int G, int halves) { return (nodes * G + halves * TR_ROWS - 1) / (halves * TR_ROWS); }
 
@@ -1069,7 +1070,7 @@ __global__ void __launch_bounds__(TA_THREADS) tree_accept_kernel(AcceptDev d) {
                 wrong |= PIKV_ST_BAD_INDEX;
                 continue;
             }
-            const int ps = table[(ctx + at) / PIKV_PAGE_TOKENS], pd = ctx + i < most ? table[(ctx + i) / PIKV_PAGE_TOKENS] : -1;
+            const int ps = table[(ctx + at) / PIKV_PAGE_TOKENS], pd = i < most - ctx ? table[(ctx + i) / PIKV_PAGE_TOKENS] : -1;
             if (ps < 0 || ps >= d.c.num_pages || pd < 0 || pd >= d.c.num_pages) wrong |= PIKV_ST_BAD_PAGE;
         }
     const int seq_bad = __syncthreads_or(wrong & PIKV_ST_BAD_SEQ);

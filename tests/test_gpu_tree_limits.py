@@ -223,3 +223,36 @@ def test_page_scores_of_any_size(key, query):
     _, got = cache.decode_attention_sparse((q.float() * 2.0 ** query).bfloat16(), bounds, 20, seq_len=lens, want_pages=True)
     cache.check_status()
     assert torch.equal(got, want)
+
+
+# ---- the largest cache ------------------------------------------------------------------------------------------------
+def test_positions_next_to_2_31():
+    """A stream whose pages end 16 rows before 2^31 (all of them one page of the pool): trees and paths that do not fit there."""
+    import pikv_b200
+    most = 2 ** 31 - 16
+    cache = pikv_b200.PagedKVCache(1, most, 1, num_pages=1, identity_table=False)
+    cache.page_table.zero_()
+    gen = torch.Generator(device="cuda").manual_seed(37)
+    v = torch.randn(16, D, generator=gen, device="cuda").bfloat16()
+    append_rows(cache, 0, 0, torch.zeros_like(v), v)
+    k, v = rows64(cache, 0, 16)
+    N = 20
+    q = torch.randn(1, N, 2, D, generator=gen, device="cuda").bfloat16()
+    mask = torch.ones(N, N, dtype=torch.bool, device="cuda")
+    out, lse = cache.decode_attention_tree(q, mask, ctx_len=torch.tensor([most - 10], dtype=torch.int32, device="cuda"), want_lse=True)
+    assert int(cache.status) == 8 and not out[0, 10:].any() and bool((lse[0, 10:] == -math.inf).all())
+    cache.status.zero_()
+    # Every row weighs the same.  A block adds up 2^31 / 64 / 296 tiles of four products each in fp32, 2^-23 a sum at most
+    off = 2 ** 31 / 64 / 296 * 4 * 2.0 ** -23
+    assert bool(((out[0, :10].double() - v.mean(0)).abs() <= (2 * off + 2.0 ** -8) * v.abs().max()).all())
+    assert bool(((lse[0, :10].double() - math.log(most)).abs() <= off).all())
+    assert not cache.decode_attention_tree(q, mask, ctx_len=torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda"),
+                                           nodes=torch.zeros(1, dtype=torch.int32, device="cuda")).any()
+    # nothing of these paths fits, is ascending, or is a length
+    held = [t.clone() for _, t in cache.named_buffers()]
+    path = torch.arange(40, dtype=torch.int32, device="cuda")[None].contiguous()
+    for ctx, p in ((most - 10, path), (most, path), (most - 30, path.flip(1).contiguous()), (most - 5, torch.zeros_like(path)), (2 ** 31 - 1, path)):
+        new = cache.accept_tree(p, ctx_len=torch.tensor([ctx], dtype=torch.int32, device="cuda"))
+        assert int(cache.status) == 8 and int(new[0]) == ctx
+        cache.status.zero_()
+        assert all(torch.equal(a, t) for a, (_, t) in zip(held, cache.named_buffers()))
