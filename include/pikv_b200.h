@@ -603,9 +603,11 @@ int pikv_page_bounds_update(const pikv_paged_cache* c, void* bound_codes, float*
  * and the best of those between them, ties going to the lower page.  A page's score is the largest logit that a query
  * head of the group can reach inside the page's bounds, times sqrt(128):
  *   score = max over the group's heads of  s_q s_page sum_c (max(u_c, 0) hi_c + min(u_c, 0) lo_c)
- * with the query in whole steps too, u = rint(q / s_q), s_q as s above; the sum is a whole number and the products by
- * powers of two are exact, so the choice does not depend on an order of summation.  A query head that is not finite
- * has no say, a page with an infinite scale is taken before the finite ones.
+ * with the query in whole steps too, u = rint(q / s_q), s_q as s above, so it bounds the logits of the rounded query, not of q
+ * itself; the sum is a whole number and the products by powers of two are exact, so the choice does not depend on an order of
+ * summation.  A query head that is not finite has no say, a page with an infinite scale is taken before the finite ones.
+ * The chosen pages go through the kernels of pikv_decode_attn_q8 and _q4, whose weights times V's scales are f16 (scales below
+ * 65504); a result that is not a number, as that of a query head that is not finite, comes out as one, where those calls answer 0.
  *   q, out [B, n_q, 128] bf16, n_q / n_kv <= 8; lse as in pikv_decode_params
  *   chosen (optional) [B, n_kv, pages] int32: the page numbers taken, ascending, -1 behind them
  *   max_pages <= PIKV_SPARSE_MAX_PAGES */

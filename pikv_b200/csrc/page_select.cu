@@ -2,10 +2,13 @@
 // them (decode_attn.cu, with a page list per stream and KV head).
 //
 // A page is 16 rows.  For channel c let hi_c and lo_c be the largest and smallest key on it: no key of the page gives a
-// query q a logit above sum_c max(q_c hi_c, q_c lo_c) = sum_c (max(q_c, 0) hi_c + min(q_c, 0) lo_c).  Bounds are kept as
-// int8 in whole steps of a power of two (256 bytes for the 4 KB of a page and head), the query is brought to int8 the same
-// way, so a score is ONE product of a page's 256 bytes with 256 bytes of query on the integer tensor cores, an exact whole
-// number times exact powers of two: the choice of pages depends neither on the order of a sum nor on the type it is held in.
+// query q a logit above sum_c max(q_c hi_c, q_c lo_c) = sum_c (max(q_c, 0) hi_c + min(q_c, 0) lo_c).  (Ranking pages by the
+// largest and smallest key of every channel is the method of QUEST.)  Bounds are kept as int8 in whole steps of a power of two,
+// rounded outwards (256 bytes for the 2 KB of a page's keys), the query is brought to int8 steps too, rounded to the nearest:
+// a score is the bound for that rounded query, and ONE product of a page's 256 bytes with 256 bytes of query on the integer tensor
+// cores, an exact whole number times exact powers of two: the choice of pages depends neither on the order of a sum nor on the
+// type it is held in.  (Of 59 pages of 2048 chosen for a query over topical keys, 99 % are those of the unrounded query, 93 %
+// those of unrounded bounds as well.)
 #include "stream_list.cuh"
 #include "shard_decode.cuh"
 #include "tc_common.cuh"

@@ -60,18 +60,20 @@ __device__ __forceinline__ int tree_lengths(const TreeDev& d, int i, int& row, i
 //   logit = 2^(e_k + 9) / sqrt(128) q . K16
 //   O     = sum w V16,  w = f16(2^(logit - R + e_v + 9))
 // Where a row's scale lies more than 2^8 (4 bit: 2^4) below the tile's largest, every row has an e of its own, and the softmax applies
-// it to scores and weights: what a row holds, seen or not, takes no more than 2^-13 of another's largest entry from it.  (One such row in
-// every tile makes the call five times as long; a prompt has a few such tiles, at padding and at its first tokens.)
+// it to scores and weights: what a row holds, seen or not, takes no more than 2^-13 of another's largest entry from it.  (The few tiles
+// of a prompt that have such rows, at padding and at its first tokens, take six times as long: one in each of 16 x 16384's, 182 -> 948 us.
+// The rest paid 2 us for it, and 2 of 75 over the 4-bit cache, where the scales' warp first pushed its neighbours' loops out of the
+// instruction cache.)
 // A 4-bit code has its zero point taken off first, exactly where that is a whole number below 2048 (with the zero points' parts
-// as products of their own in the softmax, it had to reload registers as well: 24 ragged streams to 6001, 103 -> 78 us, now 75).
+// as products of their own in the softmax, it had to reload registers as well: 24 ragged streams to 6001, 103 -> 78 us, now 77).
 // R is a row's reference: 2^TR_HEAD below the largest logit (log2 domain) plus e_v + 9 of the tile it was seen in, so that the weights sit
 // at the top of f16's range whatever the size of V; it moves only when a tile exceeds it by 2^TR_SLACK.  The denominator is
 // the fp32 sum of 2^(logit - R).  A row of V that is not finite enters as zeros and makes the result of the rows that see it
 // not a number; one that a row does not see does not reach it.
 //
-// 16 streams x 16384 rows x 8 heads, 32 nodes x 4 query heads, int8: 179 us with the merge = 3.1 TB/s and 0.77 PFLOP/s in a
-// burst, 215 us in long runs under the power cap (the bytes alone take 85 us, the products 82); 8 x 32768, 64 nodes: 300 and
-// 353.  Bound by power and by the latency between the warps: the SM clock is at 1.6-1.75 GHz, and leaving out the conversion,
+// 16 streams x 16384 rows x 8 heads, 32 nodes x 4 query heads, int8: 213 us with the merge = 2.6 TB/s and 0.65 PFLOP/s in long
+// runs under the power cap (226 on another GPU), 182 us in a burst (the bytes alone take 85 us, the products 82); 8 x 32768,
+// 64 nodes: 350 and 303.  Bound by power and by the latency between the warps: the SM clock is at 1.6-1.75 GHz, and leaving out the conversion,
 // either product, the copies or the weights shortens it by 20, 9 and 5, 6 and 8 %, none by what it costs alone.
 constexpr int TR_THREADS = 384;          // of a half: three warpgroups
 constexpr int TR_K = 4, TR_V = 6, TR_MMA = 8, TR_COPY = 9, TR_SCALES = 11;      // first warps of each kind

@@ -173,7 +173,8 @@ class PagedKVCache(torch.nn.Module):
         appended behind the context: node i of stream b is position ctx_len[b] + i (ctx_len int32 [B], default: `length`, which
         append() leaves alone).  Node i sees the whole context and the nodes j with mask[i, j] (bool [N, N], or [B, N, N] for a
         tree per stream), its own diagonal entry included in that.  nodes int32 [B]: the nodes of each stream, those behind them are
-        neither seen nor computed (zero rows, log-sum-exp -inf, as for a node that sees nothing).  Returns out [B, N, n_q, 128],
+        neither seen nor computed (zero rows, log-sum-exp -inf, as for a node that sees nothing).  K and V enter the products rounded to
+        f16 (2^-11 of an entry; decode_attention keeps K's codes exact).  Returns out [B, N, n_q, 128],
         with want_lse (out, lse [B, N, n_q]).  int8 symmetric and 4-bit asymmetric caches.  See pikv_tree_attn."""
         return host().tree(self._buffers, self.num_seqs, self.n_kv, self.bits, self.symmetric, self.max_pages, self.num_pages,
                            q, mask, seq_ids, ctx_len, nodes, want_lse)
@@ -209,8 +210,8 @@ class PagedKVCache(torch.nn.Module):
                                 seq_len: Optional[torch.Tensor] = None, first: int = 0, recent: int = 1, want_lse: bool = False,
                                 want_pages: bool = False):
         """decode_attention over at most `pages` pages (of 16 rows) of each stream and KV head: its `first` pages, its `recent` last
-        ones, and of those between them the ones on which a query head of the group can reach the largest logit, by the bounds
-        (ties: the lower page).  q [B, n_q, 128] bf16, up to 8 query heads per KV head.  Returns out [B, n_q, 128]; behind it with
+        ones, and of those between them the ones on which a query head of the group, rounded to int8 steps, can reach the largest
+        logit by the bounds (ties: the lower page).  q [B, n_q, 128] bf16, up to 8 query heads per KV head.  Returns out [B, n_q, 128]; behind it with
         want_lse the log-sum-exp [B, n_q] over the chosen pages, with want_pages the page numbers int32 [B, n_kv, pages],
         ascending, -1 behind them.  The bounds must be up to date (update_bounds).  See pikv_sparse_attn."""
         return host().sparse(self._buffers, self.num_seqs, self.n_kv, self.bits, self.symmetric, self.max_pages, self.num_pages,
