@@ -207,6 +207,50 @@ def test_tree_large_values(bits, size):
     check_weighted(cache, q, mask, ctx, out)
 
 
+@pytest.mark.parametrize("bits,N", [(8, 32), (4, 32), (8, 64), (4, 50)])
+def test_tree_repeats_of_unlike_rows(bits, N):
+    """Exponents of the rows' own in many tiles of long contexts, next to tiles without: the same bits every time."""
+    ctx = [4000 + 37 * i for i in range(12)]
+    cache, gen = filled_cache([n + N for n in ctx], 8, bits, seed=N + bits)
+    for name in ("k_scale", "v_scale"):
+        t = getattr(cache, name)
+        few = torch.rand(t.shape, generator=gen, device="cuda") < 0.01
+        t[few] *= 2.0 ** torch.randint(-30, 14, (int(few.sum()),), generator=gen, device="cuda").float()
+    q = torch.randn(len(ctx), N, 32, D, generator=gen, device="cuda").bfloat16()
+    mask = torch.rand(len(ctx), N, N, generator=gen, device="cuda") < 0.4
+    length = torch.tensor(ctx, dtype=torch.int32, device="cuda")
+    first = cache.decode_attention_tree(q, mask, ctx_len=length)
+    for _ in range(12):
+        assert torch.equal(cache.decode_attention_tree(q, mask, ctx_len=length), first)
+    cache.check_status()
+    check_weighted(cache, q[:2], mask[:2], length, first)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("N,G", [(9, 4), (64, 8)])
+def test_tree_unlike_rows_that_are_not_finite(bits, N, G):
+    """Rows that are not finite next to rows of unlike sizes, in one tile: what a node does not see does not reach it."""
+    n_kv, ctx = 1, torch.tensor([200], dtype=torch.int32, device="cuda")
+    cache, gen = filled_cache([200 + N], n_kv, bits, seed=N)
+    q = torch.randn(1, N, n_kv * G, D, generator=gen, device="cuda").bfloat16()
+    mask = torch.eye(N, dtype=torch.bool, device="cuda")
+    mask[6, 3] = mask[7, 5] = True
+    for which in ("k", "v"):
+        grow(cache, 0, 150, 2.0 ** -12, which)
+        grow(cache, 0, 204, 2.0 ** 15, which)
+    want, want_lse = cache.decode_attention_tree(q, mask, ctx_len=ctx, want_lse=True)
+    check_weighted(cache, q, mask, ctx, want)
+    for which in ("k_scale", "v_scale"):
+        for node, x in ((3, math.nan), (5, math.inf)):
+            getattr(cache, which)[int(cache.page_table[0, (200 + node) // PAGE]), 0, (200 + node) % PAGE] = x
+        out, lse = cache.decode_attention_tree(q, mask, ctx_len=ctx, want_lse=True)
+        hit = [3, 5, 6, 7]
+        rest = [i for i in range(N) if i not in hit]
+        assert torch.equal(out[0, rest], want[0, rest]) and torch.equal(lse[0, rest], want_lse[0, rest])
+        assert bool((~torch.isfinite(out[0, hit])).any(-1).all())
+    cache.check_status()
+
+
 # ---- the choice of pages ----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("key,query", [(-60, -118), (108, 10), (-100, -40), (100, 100)])
 def test_page_scores_of_any_size(key, query):
